@@ -77,7 +77,7 @@ int vnm_prune_magnitude_f32(const float *w, int64_t ldw, int M, int K, int V, in
  * vnm_compress_f16 (with its mask) give for the weights rounded to fp16, bit for bit, without the mask or the masked
  * matrix ever being written.  w: fp16 or fp32 [M, K], leading dimension ldw.  A (row, group) of a block that keeps nothing counts
  * as a violation, as there.  Needs K % m == 0 and m <= 64 (VNM_ERR_UNSUPPORTED otherwise). */
-enum { VNM_F32 = 0, VNM_F16 = 1 };
+enum { VNM_F32 = 0, VNM_F16 = 1, VNM_BF16 = 2 /* VNM_BF16: the vnm_fp8_* entry points only */ };
 int vnm_sparsify_magnitude(const void *w, int w_type, int64_t ldw, int M, int K, int V, int n, int m,
                            void *values, uint32_t *meta, uint32_t *colloc, unsigned long long *violations, void *stream);
 
@@ -257,6 +257,52 @@ int vnm_handle_info(vnm_handle_t handle, int *M, int *K, int *V, int *m, int *ma
 /* Kernel configuration that vnm_spmm_f16 would launch for this handle and N (for reporting).  `stages`: 2 = the kernel on
  * pairs of SMs, 1 = the kernel for few tiles, else the number of producer warps of the gather kernel. */
 int vnm_spmm_config(vnm_handle_t handle, int N, int *tile_m, int *tile_n, int *stages, int *grid, int *smem_bytes);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Block-scaled 8-bit operands: values of e4m3 or e5m2 with a power of two for each block of 128 along a row.  No counterpart in the
+ * reference; the 8-bit form of a linear that is not pruned, and of what its training keeps.
+ *
+ * A matrix [rows, cols] is two arrays:
+ *   data    8-bit floats, row r at data + r * ld; ld a multiple of 16 and at least cols, base 16-byte aligned.  Entry points that write it also
+ *           write zeros up to the next multiple of 8 columns (of 16 for a transpose), those that read it ignore what lies past cols.
+ *   scales  one byte for each row and block, the exponent + 127 of a power of two: byte ((kb / 4) * rows + r) * 4 + kb % 4 for
+ *           block kb = columns 128 kb .. 128 kb + 127, in all vnm_fp8_scale_bytes(rows, cols); bytes past the last block are 0.  4-byte aligned.
+ * The scale of a block is the smallest power of two s >= 2^-127 with amax / s <= 448 (e4m3) or 57344 (e5m2), amax the largest finite magnitude in it;
+ * values are x / s rounded once, to nearest even.  NaN stays NaN, infinities become NaN in e4m3 and stay in e5m2; neither changes the others' scale.
+ * A block of zeros has the smallest scale.  x_type and the types of y, dx, out, bias and column sums: VNM_F32, VNM_F16 or VNM_BF16.  ldx >= cols;
+ * rows that are 16-byte aligned are read fastest.  Empty matrices are allowed (nothing is written but column sums, which are zero). */
+enum { VNM_E4M3 = 0, VNM_E5M2 = 1 };
+int64_t vnm_fp8_scale_bytes(int rows, int cols);
+
+/* x -> 8 bits.  square != 0: blocks of 128 x 128 (their scale repeated for each of the rows), so that a matrix and its transpose hold the same values.
+ *   data, scales      x [rows, cols] (both null: not wanted)
+ *   data_t, scales_t  its transpose [cols, rows], blocks of 128 rows of x, from the same pass (both null: not wanted)
+ *   colsum            sums of x over its rows, [cols] of colsum_type, summed in fp32 in a fixed order (null: not wanted; needs data_t)
+ *   workspace         4 * ceil(rows / 128) * cols bytes where column sums are wanted, free again when the call's work is done */
+int vnm_fp8_quantize(const void *x, int x_type, int64_t ldx, int rows, int cols, int f8_type, int square, void *data, int64_t ldd, void *scales,
+                     void *data_t, int64_t ldt, void *scales_t, void *colsum, int colsum_type, void *workspace, void *stream);
+/* The values that data and scales stand for, rounded to out_type. */
+int vnm_fp8_dequantize(const void *data, int64_t ldd, const void *scales, int f8_type, int rows, int cols, void *out, int out_type, int64_t ldo, void *stream);
+
+/* GELU with what its gradient and the following product need, in one pass over x: tanh_form 0 = x Phi(x), 1 = the tanh form.
+ *   y                 gelu(x) in the type of x (null: not wanted; not together with data_t)
+ *   data.., data_t..  gelu(x) in e4m3, rounded from fp32, as vnm_fp8_quantize gives them (null: not wanted)
+ *   ckpt, ckpt_scales an e4m3 checkpoint of x for vnm_fp8_gelu_grad (null: not wanted) */
+int vnm_fp8_gelu(const void *x, int x_type, int64_t ldx, int rows, int cols, int tanh_form, void *y, int64_t ldy, void *data, int64_t ldd, void *scales,
+                 void *data_t, int64_t ldt, void *scales_t, void *ckpt, int64_t ldc, void *ckpt_scales, void *stream);
+/* dx = dy * gelu'(h), h what the checkpoint holds; dx in the type of dy (null: not wanted; not together with data_t) and / or quantised from fp32;
+ * colsum and workspace as in vnm_fp8_quantize, of dx before its rounding. */
+int vnm_fp8_gelu_grad(const void *dy, int dy_type, int64_t ldy, int rows, int cols, int tanh_form, const void *ckpt, int64_t ldc, const void *ckpt_scales, void *dx,
+                      int64_t lddx, int f8_type, void *data, int64_t ldd, void *scales, void *data_t, int64_t ldt, void *scales_t, void *colsum, int colsum_type,
+                      void *workspace, void *stream);
+
+/* out[m, n] = sum over k of A[m, k] B[n, k] (+ bias[n]), A [M, K] and B [N, K] in 8 bits (types may differ), sums in fp32, rounded once; out [M, N] with
+ * leading dimension ldo >= N.  K >= 1. */
+int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, int a_type, const void *b, int64_t ldb, const void *b_scales, int b_type, int M, int N, int K,
+                   const void *bias, int bias_type, void *out, int out_type, int64_t ldo, void *stream);
+/* Reads and clears the sticky device-side status word of the 8-bit products on the current device, as vnm_device_status does for a handle.
+ * Synchronises `stream`. */
+int vnm_fp8_device_status(int *status, void *stream);
 
 /* ---------------------------------------------------------------------------------------------------------
  * Multi-GPU launcher: the dense operand and the result sharded by columns (N) over the GPUs of one node, the

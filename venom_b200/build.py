@@ -20,7 +20,8 @@ NVCC_BASE = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "
 NVCC_FLAGS = NVCC_BASE + ["--use_fast_math"]
 # Translation units whose floating-point results are compared bit for bit with the reference are built WITHOUT
 # --use_fast_math: the magnitude pruner sums fp32 scores, and flush-to-zero would change them for denormal weights.
-EXACT_FP_UNITS = {"vnm_prune.cu"}
+# The 8-bit quantiser scales denormal values by exact powers of two.
+EXACT_FP_UNITS = {"vnm_prune.cu", "vnm_fp8_quant.cu"}
 OBJ_DIR = os.path.join(PKG, "build")
 
 
@@ -32,8 +33,9 @@ def _stale(target, sources):
 
 
 def _sources():
-    cu = [os.path.join(CSRC, f) for f in ("vnm_format.cu", "vnm_prune.cu", "vnm_spmm.cu", "vnm_spmm_dense_b2.cu", "vnm_spmm_small.cu", "vnm_capi.cu", "vnm_noalloc.cu", "vnm_mgpu.cu")]
-    hdr = [os.path.join(CSRC, f) for f in ("vnm_common.cuh", "vnm_internal.h")] + [os.path.join(ROOT, "include", "venom_b200.h")]
+    cu = [os.path.join(CSRC, f) for f in ("vnm_format.cu", "vnm_prune.cu", "vnm_spmm.cu", "vnm_spmm_dense_b2.cu", "vnm_spmm_small.cu", "vnm_capi.cu", "vnm_noalloc.cu", "vnm_mgpu.cu",
+                                          "vnm_fp8_quant.cu", "vnm_fp8_small.cu", "vnm_fp8_api.cu")]
+    hdr = [os.path.join(CSRC, f) for f in ("vnm_common.cuh", "vnm_internal.h", "vnm_fp8.h")] + [os.path.join(ROOT, "include", "venom_b200.h")]
     return cu, hdr
 
 
@@ -74,8 +76,8 @@ def build_cli(force=False):
 def build_spatha(force=False):
     """pybind torch extension `spatha` (same module name and spmm() signature as the reference's
     end2end/spatha_mod extension).  Built in-tree next to this file."""
-    src = os.path.join(CSRC, "spatha_torch.cpp")
-    if not os.path.exists(src):
+    srcs = [os.path.join(CSRC, f) for f in ("spatha_torch.cpp", "fp8_torch.cpp")]
+    if not all(os.path.exists(s) for s in srcs):
         return None
     import sysconfig
     import torch
@@ -83,7 +85,7 @@ def build_spatha(force=False):
     build_lib(force)
     suffix = sysconfig.get_config_var("EXT_SUFFIX")
     out = os.path.join(PKG, "spatha" + suffix)
-    if not force and not _stale(out, [src, LIB]):
+    if not force and not _stale(out, srcs + [LIB]):
         return out
     inc = []
     for p in cpp_extension.include_paths():
@@ -91,8 +93,15 @@ def build_spatha(force=False):
     inc += ["-I", sysconfig.get_paths()["include"], "-I", "/usr/local/cuda/include"]
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
     abi = "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", abi, "-DTORCH_EXTENSION_NAME=spatha",
-           "-DTORCH_API_INCLUDE_EXTENSION_H"] + inc + ["-o", out, src, "-L" + PKG, "-lvenom_b200",
+    flags = ["g++", "-O2", "-std=c++17", "-fPIC", abi, "-DTORCH_EXTENSION_NAME=spatha", "-DTORCH_API_INCLUDE_EXTENSION_H"]
+    from concurrent.futures import ThreadPoolExecutor
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    objs = [os.path.join(OBJ_DIR, os.path.basename(s)[:-4] + ".o") for s in srcs]
+    hdr = os.path.join(ROOT, "include", "venom_b200.h")
+    jobs = [flags + inc + ["-c", "-o", o, s] for s, o in zip(srcs, objs) if force or _stale(o, [s, hdr])]
+    with ThreadPoolExecutor(max_workers=2) as ex:
+        list(ex.map(subprocess.check_call, jobs))
+    cmd = ["g++", "-shared", "-o", out] + objs + ["-L" + PKG, "-lvenom_b200",
            "-L" + tlib, "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_python", "-lc10_cuda", "-ltorch_cuda",
            "-L/usr/local/cuda/lib64", "-lcudart", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + tlib]
     subprocess.check_call(cmd)

@@ -84,6 +84,17 @@ def lib():
         L.vnm_set_max_ctas.restype = C.c_int
         L.vnm_handle_info.argtypes = [C.c_void_p] + [C.POINTER(C.c_int)] * 5
         L.vnm_handle_info.restype = C.c_int
+        vp, i64, i32 = C.c_void_p, C.c_int64, C.c_int
+        for name, args in (("quantize", [vp, i32, i64, i32, i32, i32, i32, vp, i64, vp, vp, i64, vp, vp, i32, vp, vp]),
+                           ("dequantize", [vp, i64, vp, i32, i32, i32, vp, i32, i64, vp]),
+                           ("gelu", [vp, i32, i64, i32, i32, i32, vp, i64, vp, i64, vp, vp, i64, vp, vp, i64, vp, vp]),
+                           ("gelu_grad", [vp, i32, i64, i32, i32, i32, vp, i64, vp, vp, i64, i32, vp, i64, vp, vp, i64, vp, vp, i32, vp, vp]),
+                           ("matmul", [vp, i64, vp, i32, vp, i64, vp, i32, i32, i32, i32, vp, i32, vp, i32, i64, vp]),
+                           ("device_status", [C.POINTER(C.c_int), vp])):
+            getattr(L, "vnm_fp8_" + name).argtypes = args
+            getattr(L, "vnm_fp8_" + name).restype = i32
+        L.vnm_fp8_scale_bytes.argtypes = [i32, i32]
+        L.vnm_fp8_scale_bytes.restype = i64
         ip = C.POINTER(C.c_int)
         L.vnm_mgpu_shard.argtypes = [C.c_int] * 4 + [ip, ip]
         L.vnm_mgpu_unique_id.argtypes = [C.c_void_p]

@@ -422,6 +422,8 @@ PyMethodDef fast_calls[] = {
 
 }  // namespace
 
+void define_fp8(pybind11::module &mod);   // fp8_torch.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod)
 {
     mod.def("spmm", &spmm, "V:N:M sparse x dense product (returns [B_num_cols, A_num_rows])", pybind11::arg("A_metadata"), pybind11::arg("A_indices"),
@@ -435,4 +437,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod)
     mod.def("clear_cache", &clear_cache, "Drop every cached prepared operand");
     mod.def("cache_size", &cache_size, "Cached operands");
     mod.def("cached_copies", &cached_copies, "Device copies they hold: one or two (gather form, dense-B form) each");
+    define_fp8(mod);
 }

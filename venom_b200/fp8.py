@@ -1,0 +1,350 @@
+"""Linears in block-scaled 8 bits, with 8-bit activation checkpoints for their backward pass.
+
+What nmv.SrnmSpmm is for a weight that may be pruned, Fp8Linear is for one that may not: every value is kept, in 8 bits, with a power of
+two for each block of 128 along a row (for each 128 x 128 of a weight).  The product's operands are both in that form and are scaled inside the tensor
+core; sums have 32 bits.  For training, what a layer keeps of its input until the backward pass is 8 bits a value too: the transpose that the weight's
+gradient multiplies with, written in the same pass as the operand of the forward product.
+
+  quantize, BlockFp8         the format and its conversions (capi.compress and decompress of this form)
+  matmul                     a @ b.T of two of them
+  linear, gelu, mlp          differentiable: linear layer, GELU from an 8-bit checkpoint, and linear - GELU - linear with the GELU between them fused into
+                             the quantiser, forwards and backwards
+  Fp8Linear, Fp8Mlp, linear_to_fp8   modules, as nmv.SrnmSpmm and nmv.linear_to_spmm
+
+Everything runs on the CUDA device of its operands and on torch's current stream there; nothing synchronises, and calls may be captured into a graph.
+There is no CPU path.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import spatha_module
+from .capi import VenomError
+
+E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
+_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+
+_ext = None
+
+
+def _call(name, *args):
+    global _ext
+    if _ext is None:
+        _ext = spatha_module()
+    try:
+        return getattr(_ext, name)(*args)
+    except RuntimeError as e:
+        raise VenomError(str(e).split("\nException raised from")[0]) from None
+
+
+class BlockFp8:
+    """A matrix in 8 bits: `data` float8_e4m3fn or float8_e5m2 [rows, cols], rows a multiple of 16 bytes apart, and `scales` float8_e8m0fnu
+    [ceil(cols / 512), rows, 4]: scales[kb // 4, r, kb % 4] is that of columns 128 kb .. 128 kb + 127 of row r.  Both are used as they lie."""
+
+    __slots__ = ("data", "scales")
+
+    def __init__(self, data, scales):
+        self.data, self.scales = data, scales
+
+    @property
+    def shape(self):
+        return self.data.shape
+
+    @property
+    def dtype(self):
+        return self.data.dtype
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def dequantize(self, dtype=torch.float32):
+        """The values that it stands for, [rows, cols] of `dtype` (float16, bfloat16 or float32)."""
+        return _call("fp8_dequantize", self.data, self.scales, dtype)
+
+    def __repr__(self):
+        return "BlockFp8(%d x %d, %s, %s)" % (self.shape[0], self.shape[1], self.dtype, self.device)
+
+
+def quantize(x, dtype=E4M3, square=False, both=False):
+    """x [rows, cols] (float16, bfloat16 or float32 on a CUDA device) -> BlockFp8 of float8_e4m3fn or float8_e5m2.
+
+    A block's scale is the smallest power of two that brings its largest finite magnitude to at most 448 (e4m3) or 57344 (e5m2); values are
+    rounded to nearest even.  NaN stays NaN, infinities become NaN in e4m3 and stay in e5m2.  Blocks are 128 values of a row, or with `square` 128 x 128,
+    so that a matrix and its transpose hold the same values.  both: also the transpose, as (BlockFp8 of x, BlockFp8 of x.T), from one read of x."""
+    a, sa, t, st, _ = _call("fp8_quantize", x, dtype, square, True, both, None)
+    return (BlockFp8(a, sa), BlockFp8(t, st)) if both else BlockFp8(a, sa)
+
+
+def matmul(a, b, bias=None, dtype=torch.float16):
+    """a @ b.T (+ bias): BlockFp8 [M, K] and [N, K] -> [M, N] of `dtype` (float16, bfloat16 or float32).  The 8-bit types of a and b may differ.
+    bias: N values, added in 32 bits."""
+    return _call("fp8_matmul", a.data, a.scales, b.data, b.scales, bias, dtype)
+
+
+def _check_input(x, what):
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise VenomError("%s: a CUDA tensor expected (there is no CPU path)" % what)
+    if x.dtype not in _FLOATS:
+        raise VenomError("%s: float16, bfloat16 or float32 expected, not %s" % (what, x.dtype))
+    if x.dim() < 1:
+        raise VenomError("%s: at least one dimension expected" % what)
+
+
+def _flat(x):
+    """[..., features] as rows."""
+    return x if x.dim() == 2 else x.reshape(x.numel() // max(1, x.shape[-1]), x.shape[-1])
+
+
+def _check_linear(x, weight, bias, what):
+    _check_input(x, what)
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.dtype not in _FLOATS or weight.device != x.device:
+        raise VenomError("%s: the weight must be a float16, bfloat16 or float32 matrix on the input's device" % what)
+    if x.shape[-1] != weight.shape[1] or weight.shape[1] < 1:
+        raise VenomError("%s: an input of %s does not match a weight of %s" % (what, tuple(x.shape), tuple(weight.shape)))
+    if bias is not None and (bias.shape != weight.shape[:1] or bias.dtype not in _FLOATS or bias.device != x.device):
+        raise VenomError("%s: the bias must be a vector of %d values on the input's device" % (what, weight.shape[0]))
+
+
+def _check_grad_dtype(grad_dtype, what):
+    if grad_dtype not in (E4M3, E5M2):
+        raise VenomError("%s: gradients are kept in float8_e4m3fn or float8_e5m2, not %s" % (what, grad_dtype))
+
+
+def _apply(function, tensors, *rest):
+    if torch.cuda.is_current_stream_capturing() and torch.is_grad_enabled():
+        _call("fp8_check_capture", list(tensors))
+    return function.apply(*tensors, *rest)
+
+
+def _weight_grad(dy_t, x_t, dtype):
+    """dy.T @ x from the transposes' 8 bits; zeros without any token."""
+    if dy_t[0].shape[1] == 0:
+        return torch.zeros((dy_t[0].shape[0], x_t[0].shape[0]), dtype=dtype, device=dy_t[0].device)
+    return _call("fp8_matmul", dy_t[0], dy_t[1], x_t[0], x_t[1], None, dtype)
+
+
+def _product(a, b, bias, dtype):
+    return _call("fp8_matmul", a[0], a[1], b[0], b[1], None if bias is None else bias.detach().contiguous(), dtype)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, grad_dtype):
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        flat = _flat(x)
+        xa, xs, xt, xts, _ = _call("fp8_quantize", flat, E4M3, False, True, need_w, None)
+        wa, ws, wt, wts, _ = _call("fp8_quantize", weight, E4M3, True, True, need_x, None)
+        y = _product((xa, xs), (wa, ws), bias, x.dtype)
+        ctx.save_for_backward(xt, xts, wt, wts)
+        ctx.types = weight.dtype, None if bias is None else bias.dtype, grad_dtype, x.shape, x.dtype
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xt, xts, wt, wts = ctx.saved_tensors
+        w_dtype, b_dtype, grad_dtype, shape, x_dtype = ctx.types
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        ga, gs, gt, gts, db = _call("fp8_quantize", _flat(dy), grad_dtype, False, need_x, need_w or need_b, b_dtype if need_b else None)
+        dx = _product((ga, gs), (wt, wts), None, x_dtype).reshape(shape) if need_x else None
+        dw = _weight_grad((gt, gts), (xt, xts), w_dtype) if need_w else None
+        return dx, dw, db, None
+
+
+def linear(x, weight, bias=None, grad_dtype=E4M3):
+    """x @ weight.T + bias for x [..., in], weight [out, in] and bias [out], differentiable in all three; the result has the type of x.
+
+    x is rounded in blocks of 128 along its features, the weight in blocks of 128 x 128, gradients in blocks of 128 of `grad_dtype` (float8_e4m3fn
+    or float8_e5m2) along whichever way they are summed.  Kept until the backward pass: the 8-bit transposes of x (where the weight wants a gradient)
+    and of the weight (where x does)."""
+    _check_linear(x, weight, bias, "fp8.linear")
+    _check_grad_dtype(grad_dtype, "fp8.linear")
+    return _apply(_Linear, (x, weight, bias), grad_dtype)
+
+
+def _tanh_form(approximate, what):
+    if approximate not in ("none", "tanh"):
+        raise VenomError("%s: approximate is 'none' or 'tanh', not %r" % (what, approximate))
+    return approximate == "tanh"
+
+
+class _Gelu(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, tanh_form):
+        y, _, _, _, _, h, hs = _call("fp8_gelu", _flat(x), tanh_form, True, False, False, ctx.needs_input_grad[0])
+        ctx.save_for_backward(h, hs)
+        ctx.tanh_form, ctx.dtype = tanh_form, x.dtype
+        return y.reshape(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        h, hs = ctx.saved_tensors
+        dx = _call("fp8_gelu_grad", _flat(dy), h, hs, ctx.tanh_form, True, E4M3, False, False, None)[0]
+        return dx.reshape(dy.shape), None
+
+
+def gelu(x, approximate="none"):
+    """GELU of x [..., features] like torch.nn.functional.gelu; what is kept for the backward pass is x in 8 bits."""
+    _check_input(x, "fp8.gelu")
+    return _apply(_Gelu, (x,), _tanh_form(approximate, "fp8.gelu"))
+
+
+class _Mlp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w1, b1, w2, b2, tanh_form, grad_dtype):
+        need_x, need_w1, need_b1, need_w2, need_b2 = ctx.needs_input_grad[:5]
+        inner = need_x or need_w1 or need_b1            # whether the gradient goes back through the GELU
+        flat = _flat(x)
+        xa, xs, xt, xts, _ = _call("fp8_quantize", flat, E4M3, False, True, need_w1, None)
+        w1a, w1s, w1t, w1ts, _ = _call("fp8_quantize", w1, E4M3, True, True, need_x, None)
+        h = _product((xa, xs), (w1a, w1s), b1, x.dtype)
+        _, aa, as_, at, ats, hc, hcs = _call("fp8_gelu", h, tanh_form, False, True, need_w2, inner)
+        del h
+        w2a, w2s, w2t, w2ts, _ = _call("fp8_quantize", w2, E4M3, True, True, inner, None)
+        y = _product((aa, as_), (w2a, w2s), b2, x.dtype)
+        ctx.save_for_backward(xt, xts, w1t, w1ts, at, ats, hc, hcs, w2t, w2ts)
+        ctx.types = w1.dtype, None if b1 is None else b1.dtype, w2.dtype, None if b2 is None else b2.dtype, tanh_form, grad_dtype, x.shape, x.dtype
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], w2.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xt, xts, w1t, w1ts, at, ats, hc, hcs, w2t, w2ts = ctx.saved_tensors
+        w1_dtype, b1_dtype, w2_dtype, b2_dtype, tanh_form, grad_dtype, shape, x_dtype = ctx.types
+        need_x, need_w1, need_b1, need_w2, need_b2 = ctx.needs_input_grad[:5]
+        inner = need_x or need_w1 or need_b1
+        ga, gs, gt, gts, db2 = _call("fp8_quantize", _flat(dy), grad_dtype, False, inner, need_w2 or need_b2, b2_dtype if need_b2 else None)
+        dw2 = _weight_grad((gt, gts), (at, ats), w2_dtype) if need_w2 else None
+        dx = dw1 = db1 = None
+        if inner:
+            da = _product((ga, gs), (w2t, w2ts), None, x_dtype)
+            _, ha, hs, ht, hts, db1 = _call("fp8_gelu_grad", da, hc, hcs, tanh_form, False, grad_dtype, need_x, need_w1 or need_b1, b1_dtype if need_b1 else None)
+            dx = _product((ha, hs), (w1t, w1ts), None, x_dtype).reshape(shape) if need_x else None
+            dw1 = _weight_grad((ht, hts), (xt, xts), w1_dtype) if need_w1 else None
+        return dx, dw1, db1, dw2, db2, None, None
+
+
+def mlp(x, w1, b1, w2, b2, approximate="none", grad_dtype=E4M3):
+    """linear(gelu(linear(x, w1, b1)), w2, b2) for x [..., in], w1 [hidden, in], w2 [out, hidden], differentiable in all five.
+
+    The GELU's result is rounded to 8 bits straight from 32 (there is no copy of it in the type of x), its gradient likewise.  Kept until the
+    backward pass, all in 8 bits: the transposes of x, of the GELU's result and of the weights, and the GELU's input."""
+    _check_linear(x, w1, b1, "fp8.mlp")
+    if not isinstance(w2, torch.Tensor) or w2.dim() != 2 or w2.dtype not in _FLOATS or w2.device != x.device or w2.shape[1] != w1.shape[0] or w2.shape[1] < 1:
+        raise VenomError("fp8.mlp: the second weight must be a float16, bfloat16 or float32 matrix of %d columns on the input's device" % w1.shape[0])
+    if b2 is not None and (b2.shape != w2.shape[:1] or b2.dtype not in _FLOATS or b2.device != x.device):
+        raise VenomError("fp8.mlp: the second bias must be a vector of %d values on the input's device" % w2.shape[0])
+    _check_grad_dtype(grad_dtype, "fp8.mlp")
+    return _apply(_Mlp, (x, w1, b1, w2, b2), _tanh_form(approximate, "fp8.mlp"), grad_dtype)
+
+
+class _Held(torch.nn.Module):
+    """A frozen weight's 8 bits as buffers.  They are kept as bytes, which Module.half() and its like leave alone, with the rows' padding, which a copy to
+    another device would drop."""
+
+    def _hold(self, name, weight):
+        q = quantize(weight.detach(), square=True)
+        rows, cols = q.shape
+        ld = -(-cols // 16) * 16
+        self.register_buffer(name + "_data", q.data.view(torch.uint8).as_strided((rows, ld), (ld, 1)))
+        self.register_buffer(name + "_scales", q.scales.view(torch.uint8))
+        self._views[name] = (cols, None, None)
+
+    def _weight(self, name):
+        """The buffers as an operand; the views are made anew when a buffer was replaced."""
+        cols, of, q = self._views[name]
+        data = self._buffers[name + "_data"]
+        if of is not data:
+            q = BlockFp8(data.view(E4M3)[:, :cols], self._buffers[name + "_scales"].view(torch.float8_e8m0fnu))
+            self._views[name] = (cols, data, q)
+        return q
+
+    def _refuse_gradients(self, x, *others):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x,) + others):
+            raise VenomError("%s holds a frozen weight: build it with trainable=True for gradients" % type(self).__name__)
+
+
+class Fp8Linear(_Held):
+    """Drop-in replacement of torch.nn.Linear whose products run in 8 bits.
+
+    trainable=False: the weight is quantised once and held in 8 bits only, like SrnmSpmm's, for inference.  trainable=True: the layer keeps the parameters
+    of `original`, quantises the weight in every call and is differentiable (see linear)."""
+
+    def __init__(self, original, trainable=False, grad_dtype=E4M3):
+        super().__init__()
+        self._views = {}
+        _check_grad_dtype(grad_dtype, "Fp8Linear")
+        self.in_features, self.out_features = original.in_features, original.out_features
+        self.trainable, self.grad_dtype = bool(trainable), grad_dtype
+        self.bias = original.bias
+        if self.trainable:
+            self.weight = original.weight
+        else:
+            _check_input(original.weight, "Fp8Linear")
+            self._hold("weight", original.weight)
+
+    def forward(self, input):
+        if self.trainable:
+            return linear(input, self.weight, self.bias, self.grad_dtype)
+        self._refuse_gradients(input, self.bias)
+        _check_input(input, "Fp8Linear")
+        flat = _flat(input)
+        q = quantize(flat)
+        y = matmul(q, self._weight("weight"), self.bias, input.dtype)
+        return y if input.dim() == 2 else y.reshape(*input.shape[:-1], self.out_features)
+
+    def extra_repr(self):
+        return "in_features=%d, out_features=%d, bias=%s, trainable=%s" % (self.in_features, self.out_features, self.bias is not None, self.trainable)
+
+
+class Fp8Mlp(_Held):
+    """The feed-forward block proj(gelu(fc(x))) of two torch.nn.Linear in 8 bits, the GELU fused into the quantiser (see mlp).  trainable as in Fp8Linear."""
+
+    def __init__(self, fc, proj, approximate="none", trainable=False, grad_dtype=E4M3):
+        super().__init__()
+        self._views = {}
+        _check_grad_dtype(grad_dtype, "Fp8Mlp")
+        if fc.out_features != proj.in_features:
+            raise VenomError("Fp8Mlp: %d features do not match %d" % (fc.out_features, proj.in_features))
+        self.tanh_form, self.approximate = _tanh_form(approximate, "Fp8Mlp"), approximate
+        self.trainable, self.grad_dtype = bool(trainable), grad_dtype
+        self.out_features = proj.out_features
+        self.fc_bias, self.proj_bias = fc.bias, proj.bias
+        if self.trainable:
+            self.fc_weight, self.proj_weight = fc.weight, proj.weight
+        else:
+            _check_input(fc.weight, "Fp8Mlp")
+            _check_input(proj.weight, "Fp8Mlp")
+            self._hold("fc", fc.weight)
+            self._hold("proj", proj.weight)
+
+    def forward(self, input):
+        if self.trainable:
+            return mlp(input, self.fc_weight, self.fc_bias, self.proj_weight, self.proj_bias, self.approximate, self.grad_dtype)
+        self._refuse_gradients(input, self.fc_bias, self.proj_bias)
+        _check_input(input, "Fp8Mlp")
+        h = matmul(quantize(_flat(input)), self._weight("fc"), self.fc_bias, input.dtype)
+        _, a, sa, _, _, _, _ = _call("fp8_gelu", h, self.tanh_form, False, True, False, False)
+        y = matmul(BlockFp8(a, sa), self._weight("proj"), self.proj_bias, input.dtype)
+        return y if input.dim() == 2 else y.reshape(*input.shape[:-1], self.out_features)
+
+
+def linear_to_fp8(mod, skip=(), trainable=False, grad_dtype=E4M3):
+    """Replaces every torch.nn.Linear below `mod` by Fp8Linear, but for the names in `skip` (nmv.linear_to_spmm's walk)."""
+    if isinstance(mod, torch.nn.Linear):
+        return Fp8Linear(mod, trainable, grad_dtype)
+    for name, child in mod.named_children():
+        if name in skip:
+            continue
+        if isinstance(child, torch.nn.Linear):
+            setattr(mod, name, Fp8Linear(child, trainable, grad_dtype))
+        else:
+            linear_to_fp8(child, skip, trainable, grad_dtype)
+    return mod
+
+
+def device_status():
+    """0, or VenomError if a bounded device-side wait of an 8-bit product on the current device has given up since the last call (its result is then
+    void).  Synchronises the current stream."""
+    return _call("fp8_device_status")
