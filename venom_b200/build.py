@@ -34,7 +34,7 @@ def _stale(target, sources):
 
 def _sources():
     cu = [os.path.join(CSRC, f) for f in ("vnm_format.cu", "vnm_prune.cu", "vnm_spmm.cu", "vnm_spmm_dense_b2.cu", "vnm_spmm_small.cu", "vnm_capi.cu", "vnm_noalloc.cu", "vnm_mgpu.cu",
-                                          "vnm_fp8_quant.cu", "vnm_fp8_small.cu", "vnm_fp8_api.cu")]
+                                          "vnm_fp8_quant.cu", "vnm_fp8_small.cu", "vnm_fp8_pair.cu", "vnm_fp8_api.cu")]
     hdr = [os.path.join(CSRC, f) for f in ("vnm_common.cuh", "vnm_internal.h", "vnm_fp8.h")] + [os.path.join(ROOT, "include", "venom_b200.h")]
     return cu, hdr
 

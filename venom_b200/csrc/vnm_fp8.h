@@ -52,7 +52,7 @@ struct Fp8MatmulParams {
     int a_f8, b_f8;
     int mt, nt;               // tiles along M and N
     int split;                // CTAs of a cluster that share one tile's k
-    int band;                 // order of the tiles
+    int band;                 // pair kernel: order of the tiles (tile_coords)
     int *status;
 };
 
@@ -62,6 +62,11 @@ struct Fp8Plan {
     int grid;
 };
 
+// On pairs of SMs: tiles of 256 x (192 .. 256).
+cudaError_t fp8_pair_init();
+float fp8_pair_config(int M, int N, int K, Fp8Plan *plan);   // an estimate in microseconds, < 0: not for this problem
+cudaError_t launch_fp8_pair(const Fp8Plan &plan, const CUtensorMap &map_a, const CUtensorMap &map_b, const Fp8MatmulParams &p, cudaStream_t stream);
+// One SM a tile: 128 rows of B x (16 .. 128) rows of A, k split over a cluster where tiles are few.
 cudaError_t fp8_small_init();
 float fp8_small_config(int M, int N, int ktiles, Fp8Plan *plan);
 cudaError_t launch_fp8_small(const Fp8Plan &plan, const CUtensorMap &map_a, const CUtensorMap &map_b, const Fp8MatmulParams &p, cudaStream_t stream);

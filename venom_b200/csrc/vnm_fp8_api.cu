@@ -98,7 +98,7 @@ int device_ready(int **status)
     std::lock_guard<std::mutex> lock(g_mutex);
     Device &d = g_devices[dev];
     if (!d.ready) {
-        if ((e = fp8_small_init()) != cudaSuccess) return done(e, "cudaFuncSetAttribute(max dynamic shared memory)");
+        if ((e = fp8_small_init()) != cudaSuccess || (e = fp8_pair_init()) != cudaSuccess) return done(e, "cudaFuncSetAttribute(max dynamic shared memory)");
         void *at = nullptr;
         if ((e = cudaGetSymbolAddress(&at, g_status)) != cudaSuccess) return done(e, "cudaGetSymbolAddress");
         d.status = static_cast<int *>(at);
@@ -115,6 +115,18 @@ CUresult encode_operand(EncodeTiledFn enc, CUtensorMap *map, const void *data, i
     const cuuint32_t boxes[2] = {128, (cuuint32_t)box}, steps[2] = {1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(data), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+// Band of the tile order of the pair kernel (tile_coords).  A band's operand stays in L2 while the other one streams past: row bands read A once and B once per
+// band, column bands the other way round.
+int tile_band(int M, int N, int K, int mt, int nt, int bn)
+{
+    const int64_t room = 32 << 20;
+    int64_t g = room / (256 * (int64_t)K), q = room / (bn * (int64_t)K);
+    g = g < 1 ? 1 : g > mt ? mt : g;
+    q = q < 1 ? 1 : q > nt ? nt : q;
+    const int64_t a = (int64_t)M * K, b = (int64_t)N * K;
+    return a + b * ((mt + g - 1) / g) <= b + a * ((nt + q - 1) / q) ? (int)g : -(int)q;
 }
 
 }  // namespace
@@ -241,15 +253,24 @@ extern "C" int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, 
     p.M = M; p.N = N; p.K = K; p.ktiles = (K + 127) / 128;
     p.a_f8 = a_type; p.b_f8 = b_type;
     p.status = status;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Fp8Plan small = {}, pair = {};
+    const float small_us = fp8_small_config(M, N, p.ktiles, &small), pair_us = fp8_pair_config(M, N, K, &pair);
+    const bool on_pairs = pair_us >= 0.0f && pair_us < small_us;
+    const Fp8Plan &plan = on_pairs ? pair : small;
     CUtensorMap map_a, map_b;
-    Fp8Plan small = {};
-    fp8_small_config(M, N, p.ktiles, &small);
-    if (encode_operand(enc, &map_a, a, lda, M, K, small.bn) != CUDA_SUCCESS || encode_operand(enc, &map_b, b, ldb, N, K, 128) != CUDA_SUCCESS)
+    if (encode_operand(enc, &map_a, a, lda, M, K, on_pairs ? 128 : plan.bn) != CUDA_SUCCESS || encode_operand(enc, &map_b, b, ldb, N, K, on_pairs ? plan.bn / 2 : 128) != CUDA_SUCCESS)
         return fail(VNM_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", name);
-    p.mt = (M + small.bn - 1) / small.bn;
+    p.split = plan.split;
+    if (on_pairs) {
+        p.mt = (M + 255) / 256;
+        p.nt = (N + plan.bn - 1) / plan.bn;
+        p.band = tile_band(M, N, K, p.mt, p.nt, plan.bn);
+        return done(launch_fp8_pair(plan, map_a, map_b, p, s), name);
+    }
+    p.mt = (M + plan.bn - 1) / plan.bn;
     p.nt = (N + 127) / 128;
-    p.split = small.split;
-    return done(launch_fp8_small(small, map_a, map_b, p, static_cast<cudaStream_t>(stream)), name);
+    return done(launch_fp8_small(plan, map_a, map_b, p, s), name);
 }
 
 extern "C" int vnm_fp8_device_status(int *status, void *stream)

@@ -304,11 +304,13 @@ cudaError_t fp8_small_init()
 float fp8_small_config(int M, int N, int ktiles, Fp8Plan *plan)
 {
     plan->bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const int64_t tiles = (int64_t)((M + plan->bn - 1) / plan->bn) * ((N + 127) / 128);
+    const int64_t tiles = ((int64_t)M + plan->bn - 1) / plan->bn * (((int64_t)N + 127) / 128);
     plan->split = 1;
     while (plan->split < 8 && tiles * plan->split * 2 <= 296 && ktiles >= 4 * plan->split) plan->split *= 2;
     plan->grid = (int)(tiles * plan->split);
-    return 1.0f;
+    if (M <= 128) return 0.0f;
+    const int64_t waves = ((int64_t)plan->grid + 295) / 296;
+    return (float)waves * ((float)(ktiles + plan->split - 1) / plan->split * 0.35f + 1.0f);
 }
 
 cudaError_t launch_fp8_small(const Fp8Plan &plan, const CUtensorMap &map_a, const CUtensorMap &map_b, const Fp8MatmulParams &p, cudaStream_t stream)
