@@ -335,9 +335,9 @@ def test_linear_shared_weight_and_strided_gradients():
 
 def test_linear_refusals():
     x, w = matrix(4, 64, 1, torch.float16), matrix(8, 64, 2, torch.float16)
-    for call, match in ((lambda: fp8.linear(x[:, :32], w), "does not match"), (lambda: fp8.linear(x, w, vector(7, 1, torch.float16)), "bias"), (lambda: fp8.linear(x.double(), w), "expected"),
+    for call, match in ((lambda: fp8.linear(x[:, :32], w), "do not match"), (lambda: fp8.linear(x, w, vector(7, 1, torch.float16)), "bias"), (lambda: fp8.linear(x.double(), w), "expected"),
                         (lambda: fp8.linear(x, w.cpu()), "device"), (lambda: fp8.linear(x, w, grad_dtype=torch.float16), "gradients"), (lambda: fp8.linear(x.long(), w), "expected"),
-                        (lambda: fp8.gelu(x, "fast"), "approximate"), (lambda: fp8.mlp(x, w, None, w, None), "second weight")):
+                        (lambda: fp8.gelu(x, "fast"), "approximate"), (lambda: fp8.mlp(x, w, None, w, None), "do not match")):
         with pytest.raises(capi.VenomError, match=match):
             call()
     y = fp8.linear(leaf(x), leaf(w))
@@ -472,6 +472,27 @@ def test_mlp_gives_only_the_gradients_that_are_wanted():
         fp8.mlp(*some).backward(dy)
         for i in range(5):
             assert (some[i].grad is None) if not mask >> i & 1 else torch.equal(some[i].grad, full[i]), (mask, i)
+
+
+@pytest.mark.parametrize("first,second", [(True, False), (False, True), (False, False)])
+def test_mlp_with_some_biases(first, second):
+    values = [t.detach() for t in block(50, 96, 200, 72, torch.float16)]
+    dy = matrix(50, 72, 9, torch.float16)
+    zero = [leaf(t) for t in values]
+    for i, there in ((2, first), (4, second)):
+        if not there:
+            zero[i].data.zero_()
+    want = torch.autograd.grad(fp8.mlp(*zero), zero, dy)
+    for mask in range(1, 8):
+        some = [leaf(t) if i in (2, 4) or mask >> (i if i < 2 else 2) & 1 else t for i, t in enumerate(values)]
+        if not first:
+            some[2] = None
+        if not second:
+            some[4] = None
+        fp8.mlp(*some).backward(dy)
+        for i in range(5):
+            if some[i] is not None and some[i].requires_grad:
+                assert torch.equal(some[i].grad, want[i]), (mask, i)
 
 
 def test_mlp_without_biases_and_tokens():

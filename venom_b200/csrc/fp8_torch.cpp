@@ -1,9 +1,12 @@
-// The block-scaled 8-bit operators in the `spatha` extension: checks, allocations and the C ABI's calls, on torch's current stream.
-// The autograd functions and modules on top are in fp8.py.
+// The block-scaled 8-bit operators in the `spatha` extension: checks, allocations and the C ABI's calls, on torch's current stream, and the
+// differentiable operators as autograd nodes (a step of a small layer takes as long as the host takes to queue it: in Python 85 us for a GELU and its
+// gradient, see fp8.py for what the calls mean).
 #include <torch/extension.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include "../../include/venom_b200.h"
@@ -184,19 +187,225 @@ GeluGrad gelu_grad(const Tensor &dy_in, const Tensor &ckpt, const Tensor &ckpt_s
     return GeluGrad(opt(dx), opt(a.data), opt(a.scales), opt(t.data), opt(t.scales), opt(sums));
 }
 
+// ---- differentiable operators ----
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
+
 // A call that records a graph while its stream is being captured: the node that takes a leaf's gradient lives as long as any graph of the leaf, and belongs to
 // the stream of the graph that made it.  A backward pass inside the capture that meets one of another stream waits for that stream, which ends the
 // capture (and, thrown from the autograd engine's threads, may end the process), so it is refused here.
-void check_capture(const std::vector<OptTensor> &inputs)
+void check_capture(std::initializer_list<const Tensor *> inputs)
 {
-    for (const OptTensor &t : inputs) {
-        if (!t.has_value() || !t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    if (!at::GradMode::is_enabled() || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+    for (const Tensor *t : inputs) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
         const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
         if (!node) continue;
         const auto stream = node->stream();
         TORCH_CHECK(!stream.has_value() || *stream == c10::cuda::getCurrentCUDAStream(t->device().index()).unwrap(),
                     "a graph of the same leaf recorded on another stream still lives: free it (the tensors that hold it) before this call is captured");
     }
+}
+
+// Gradients that can not be differentiated again: doing so raises instead of giving zeros.
+variable_list once(variable_list grads, const variable_list &incoming)
+{
+    if (!at::GradMode::is_enabled()) return grads;
+    bool any = false;
+    for (const Tensor &g : incoming) any = any || wants_grad(g);
+    if (!any) return grads;
+    variable_list defined;
+    for (Tensor &g : grads)
+        if (g.defined()) defined.push_back(g.detach().requires_grad_());
+    auto node = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function of venom_b200.fp8", (int64_t)defined.size());
+    variable_list out = (*node)(std::move(defined));
+    size_t i = 0;
+    for (Tensor &g : grads)
+        if (g.defined()) g = out[i++];
+    return grads;
+}
+
+bool is_float(c10::ScalarType t) { return t == torch::kFloat16 || t == torch::kBFloat16 || t == torch::kFloat32; }
+
+void check_input(const Tensor &x, const char *what)
+{
+    TORCH_CHECK(x.is_cuda(), what, ": a CUDA tensor expected (there is no CPU path)");
+    TORCH_CHECK(is_float(x.scalar_type()), what, ": float16, bfloat16 or float32 expected, not ", x.scalar_type());
+    TORCH_CHECK(x.dim() >= 1, what, ": at least one dimension expected");
+}
+void check_weight(const Tensor &x, int64_t features, const Tensor &w, const Tensor &bias, const char *what)
+{
+    TORCH_CHECK(w.dim() == 2 && is_float(w.scalar_type()) && w.device() == x.device(), what, ": a weight must be a float16, bfloat16 or float32 matrix on the input's device");
+    TORCH_CHECK(features == w.size(1) && features >= 1, what, ": ", features, " features do not match a weight of ", w.sizes());
+    TORCH_CHECK(!bias.defined() || (bias.dim() == 1 && bias.size(0) == w.size(0) && is_float(bias.scalar_type()) && bias.device() == x.device()), what,
+                ": the bias must be a vector of ", w.size(0), " values on the input's device");
+}
+void check_grad_dtype(c10::ScalarType t, const char *what)
+{
+    TORCH_CHECK(t == torch::kFloat8_e4m3fn || t == torch::kFloat8_e5m2, what, ": gradients are kept in float8_e4m3fn or float8_e5m2, not ", t);
+}
+
+Tensor flat(const Tensor &x) { return x.dim() == 2 ? x : x.reshape({x.size(-1) ? x.numel() / x.size(-1) : x.numel(), x.size(-1)}); }
+Tensor shaped(const Tensor &y, at::IntArrayRef shape)
+{
+    if (shape.size() == 2) return y;
+    std::vector<int64_t> s(shape.begin(), shape.end());
+    s.back() = y.size(1);
+    return y.view(s);
+}
+
+struct Operand {
+    Tensor data, scales;
+};
+struct Both {
+    Operand rows, cols;
+    Tensor sums;
+};
+Tensor or_undefined(const OptTensor &t) { return t.has_value() ? *t : Tensor(); }
+c10::optional<c10::ScalarType> type_of(bool wanted, c10::ScalarType t) { return wanted ? c10::optional<c10::ScalarType>(t) : c10::nullopt; }
+
+Both quantized(const Tensor &x, c10::ScalarType f8, bool square, bool rows, bool cols, c10::optional<c10::ScalarType> sums)
+{
+    if (!rows && !cols) return {};
+    const Quantized q = quantize(x, f8, square, rows, cols, sums);
+    return {{or_undefined(std::get<0>(q)), or_undefined(std::get<1>(q))}, {or_undefined(std::get<2>(q)), or_undefined(std::get<3>(q))}, or_undefined(std::get<4>(q))};
+}
+Tensor product(const Operand &a, const Operand &b, const Tensor &bias, c10::ScalarType type)
+{
+    return matmul(a.data, a.scales, b.data, b.scales, bias.defined() ? OptTensor(bias.detach().contiguous()) : c10::nullopt, type);
+}
+// dy^T x from the transposes; zeros without any token
+Tensor weight_grad(const Operand &dy_t, const Operand &x_t, c10::ScalarType type)
+{
+    if (dy_t.data.size(1) == 0) return torch::zeros({dy_t.data.size(0), x_t.data.size(0)}, dy_t.data.options().dtype(type));
+    return product(dy_t, x_t, Tensor(), type);
+}
+
+struct Linear : torch::autograd::Function<Linear> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &opt_bias, c10::ScalarType grad_type, bool record)
+    {
+        const Tensor bias = or_undefined(opt_bias);
+        const bool need_x = record && wants_grad(x), need_w = record && wants_grad(w);
+        Both xs = quantized(flat(x), torch::kFloat8_e4m3fn, false, true, need_w, c10::nullopt);
+        Both ws = quantized(w, torch::kFloat8_e4m3fn, true, true, need_x, c10::nullopt);
+        const Tensor y = product(xs.rows, ws.rows, bias, x.scalar_type());
+        ctx->save_for_backward({xs.cols.data, xs.cols.scales, ws.cols.data, ws.cols.scales});
+        ctx->saved_data["shape"] = x.sizes().vec();
+        ctx->saved_data["x"] = (int64_t)x.scalar_type();
+        ctx->saved_data["w"] = (int64_t)w.scalar_type();
+        ctx->saved_data["b"] = (int64_t)(bias.defined() ? bias.scalar_type() : x.scalar_type());
+        ctx->saved_data["grad"] = (int64_t)grad_type;
+        ctx->saved_data["bias"] = bias.defined();
+        return shaped(y, x.sizes());
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list dys)
+    {
+        const variable_list saved = ctx->get_saved_variables();
+        // counted over the tensors that there are
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
+        auto type = [&](const char *k) { return (c10::ScalarType)ctx->saved_data[k].toInt(); };
+        const Both g = quantized(flat(dys[0]), type("grad"), false, need_x, need_w || need_b, type_of(need_b, type("b")));
+        Tensor dx, dw;
+        if (need_x) dx = product(g.rows, {saved[2], saved[3]}, Tensor(), type("x")).view(ctx->saved_data["shape"].toIntVector());
+        if (need_w) dw = weight_grad(g.cols, {saved[0], saved[1]}, type("w"));
+        return once({dx, dw, g.sums, Tensor(), Tensor()}, dys);
+    }
+};
+
+Tensor linear(const Tensor &x, const Tensor &w, const OptTensor &bias, c10::ScalarType grad_type)
+{
+    const Tensor b = or_undefined(bias);
+    check_input(x, "fp8.linear");
+    check_weight(x, x.size(-1), w, b, "fp8.linear");
+    check_grad_dtype(grad_type, "fp8.linear");
+    check_capture({&x, &w, &b});
+    return Linear::apply(x, w, bias, grad_type, at::GradMode::is_enabled());
+}
+
+struct Gelu8 : torch::autograd::Function<Gelu8> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, bool tanh_form, bool record)
+    {
+        const Gelu g = gelu(flat(x), tanh_form, true, false, false, record && wants_grad(x));
+        ctx->save_for_backward({or_undefined(std::get<5>(g)), or_undefined(std::get<6>(g))});
+        ctx->saved_data["tanh"] = tanh_form;
+        ctx->saved_data["shape"] = x.sizes().vec();
+        return std::get<0>(g)->view(x.sizes());
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list dys)
+    {
+        const variable_list saved = ctx->get_saved_variables();
+        const GeluGrad g = gelu_grad(flat(dys[0]), saved[0], saved[1], ctx->saved_data["tanh"].toBool(), true, torch::kFloat8_e4m3fn, false, false, c10::nullopt);
+        return once({std::get<0>(g)->view(ctx->saved_data["shape"].toIntVector()), Tensor(), Tensor()}, dys);
+    }
+};
+
+Tensor gelu8(const Tensor &x, bool tanh_form)
+{
+    check_input(x, "fp8.gelu");
+    check_capture({&x});
+    return Gelu8::apply(x, tanh_form, at::GradMode::is_enabled());
+}
+
+struct Mlp : torch::autograd::Function<Mlp> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w1, const OptTensor &opt_b1, const Tensor &w2, const OptTensor &opt_b2, bool tanh_form,
+                          c10::ScalarType grad_type, bool record)
+    {
+        const Tensor b1 = or_undefined(opt_b1), b2 = or_undefined(opt_b2);
+        const bool need_x = record && wants_grad(x), need_w1 = record && wants_grad(w1), need_b1 = record && wants_grad(b1), need_w2 = record && wants_grad(w2);
+        const bool inner = need_x || need_w1 || need_b1;      // whether the gradient goes back through the GELU
+        Both xs = quantized(flat(x), torch::kFloat8_e4m3fn, false, true, need_w1, c10::nullopt);
+        Both w1s = quantized(w1, torch::kFloat8_e4m3fn, true, true, need_x, c10::nullopt);
+        Gelu a = gelu(product(xs.rows, w1s.rows, b1, x.scalar_type()), tanh_form, false, true, need_w2, inner);
+        Both w2s = quantized(w2, torch::kFloat8_e4m3fn, true, true, inner, c10::nullopt);
+        const Tensor y = product({*std::get<1>(a), *std::get<2>(a)}, w2s.rows, b2, x.scalar_type());
+        ctx->save_for_backward({xs.cols.data, xs.cols.scales, w1s.cols.data, w1s.cols.scales, or_undefined(std::get<3>(a)), or_undefined(std::get<4>(a)),
+                                or_undefined(std::get<5>(a)), or_undefined(std::get<6>(a)), w2s.cols.data, w2s.cols.scales});
+        ctx->saved_data["shape"] = x.sizes().vec();
+        ctx->saved_data["x"] = (int64_t)x.scalar_type();
+        ctx->saved_data["w1"] = (int64_t)w1.scalar_type();
+        ctx->saved_data["w2"] = (int64_t)w2.scalar_type();
+        ctx->saved_data["b1"] = (int64_t)(b1.defined() ? b1.scalar_type() : x.scalar_type());
+        ctx->saved_data["b2"] = (int64_t)(b2.defined() ? b2.scalar_type() : x.scalar_type());
+        ctx->saved_data["grad"] = (int64_t)grad_type;
+        ctx->saved_data["tanh"] = tanh_form;
+        ctx->saved_data["bias1"] = b1.defined();
+        ctx->saved_data["bias2"] = b2.defined();
+        return shaped(y, x.sizes());
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list dys)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        const bool has_b1 = ctx->saved_data["bias1"].toBool(), has_b2 = ctx->saved_data["bias2"].toBool();
+        const size_t at_w2 = has_b1 ? 3 : 2;      // counted over the tensors that there are
+        const bool need_x = ctx->needs_input_grad(0), need_w1 = ctx->needs_input_grad(1), need_b1 = has_b1 && ctx->needs_input_grad(2), need_w2 = ctx->needs_input_grad(at_w2),
+                   need_b2 = has_b2 && ctx->needs_input_grad(at_w2 + 1), inner = need_x || need_w1 || need_b1;
+        auto type = [&](const char *k) { return (c10::ScalarType)ctx->saved_data[k].toInt(); };
+        const Both g = quantized(flat(dys[0]), type("grad"), false, inner, need_w2 || need_b2, type_of(need_b2, type("b2")));
+        Tensor dx, dw1, db1, dw2;
+        if (need_w2) dw2 = weight_grad(g.cols, {s[4], s[5]}, type("w2"));
+        if (inner) {
+            const Tensor da = product(g.rows, {s[8], s[9]}, Tensor(), type("x"));
+            const GeluGrad h = gelu_grad(da, s[6], s[7], ctx->saved_data["tanh"].toBool(), false, type("grad"), need_x, need_w1 || need_b1, type_of(need_b1, type("b1")));
+            db1 = or_undefined(std::get<5>(h));
+            if (need_x) dx = product({*std::get<1>(h), *std::get<2>(h)}, {s[2], s[3]}, Tensor(), type("x")).view(ctx->saved_data["shape"].toIntVector());
+            if (need_w1) dw1 = weight_grad({*std::get<3>(h), *std::get<4>(h)}, {s[0], s[1]}, type("w1"));
+        }
+        return once({dx, dw1, db1, dw2, g.sums, Tensor(), Tensor(), Tensor()}, dys);
+    }
+};
+
+Tensor mlp(const Tensor &x, const Tensor &w1, const OptTensor &bias1, const Tensor &w2, const OptTensor &bias2, bool tanh_form, c10::ScalarType grad_type)
+{
+    const Tensor b1 = or_undefined(bias1), b2 = or_undefined(bias2);
+    check_input(x, "fp8.mlp");
+    check_weight(x, x.size(-1), w1, b1, "fp8.mlp");
+    check_weight(x, w1.size(0), w2, b2, "fp8.mlp");
+    check_grad_dtype(grad_type, "fp8.mlp");
+    check_capture({&x, &w1, &b1, &w2, &b2});
+    return Mlp::apply(x, w1, bias1, w2, bias2, tanh_form, grad_type, at::GradMode::is_enabled());
 }
 
 int64_t device_status()
@@ -216,6 +425,8 @@ void define_fp8(pybind11::module &mod)
     mod.def("fp8_matmul", &matmul, "vnm_fp8_matmul with its allocation", release());
     mod.def("fp8_gelu", &gelu, "vnm_fp8_gelu with its allocations", release());
     mod.def("fp8_gelu_grad", &gelu_grad, "vnm_fp8_gelu_grad with its allocations", release());
-    mod.def("fp8_check_capture", &check_capture, "Refuses to record a graph under capture beside a graph of the same leaves on another stream");
+    mod.def("fp8_linear", &linear, "A differentiable linear layer in 8 bits", release());
+    mod.def("fp8_gelu8", &gelu8, "GELU with an 8-bit checkpoint for its gradient", release());
+    mod.def("fp8_mlp", &mlp, "A differentiable feed-forward block in 8 bits", release());
     mod.def("fp8_device_status", &device_status, "vnm_fp8_device_status", release());
 }

@@ -21,7 +21,7 @@ struct Fp8QuantParams {
     int rows, cols;
     int f8;                  // type of data and data_t
     int tanh_form;           // GELU by tanh
-    int vec_in;              // rows of x may be read in pieces of 16 bytes
+    int align_x, align_y;    // what the addresses of the rows of x and y are a multiple of: 16, 4 or fewer bytes
     uint8_t *data;           // [rows, ldd] or null
     int64_t ldd;
     uint8_t *scales;         // [groups][rows][4]

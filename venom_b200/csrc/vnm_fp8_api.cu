@@ -26,7 +26,7 @@ int64_t elem_size(int type) { return type == VNM_F32 ? 4 : 2; }
 bool known_type(int type) { return type == VNM_F32 || type == VNM_F16 || type == VNM_BF16; }
 bool aligned(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-// A tiles kernel launch has a block for each 128 x 128, a rows kernel a lane for each eight values: both counts stay in 31 bits.
+// The tiles kernel has a block for each 128 x 128, the rows kernel counts pieces of 512 columns (and runs a grid past the last one): both in 32 bits.
 int check_shape(const char *name, const void *x, int type, int64_t ldx, int rows, int cols)
 {
     if (rows < 0 || cols < 0) return fail(VNM_ERR_BAD_ARG, "%s: negative size (%d, %d)", name, rows, cols);
@@ -35,7 +35,8 @@ int check_shape(const char *name, const void *x, int type, int64_t ldx, int rows
     if (!x) return fail(VNM_ERR_BAD_ARG, "%s: null input", name);
     if (ldx < cols) return fail(VNM_ERR_BAD_ARG, "%s: leading dimension %lld is less than %d columns", name, (long long)ldx, cols);
     if (!aligned(x, (uintptr_t)elem_size(type))) return fail(VNM_ERR_BAD_ARG, "%s: input is not aligned to its type", name);
-    if (((int64_t)rows + 127) / 128 * (((int64_t)cols + 127) / 128) > INT32_MAX) return fail(VNM_ERR_UNSUPPORTED, "%s: %d x %d is too large", name, rows, cols);
+    if (((int64_t)rows + 127) / 128 * (((int64_t)cols + 127) / 128) > INT32_MAX || (int64_t)rows * (((int64_t)cols + 511) / 512) > INT32_MAX - (1 << 20) || cols > INT32_MAX - 512)
+        return fail(VNM_ERR_UNSUPPORTED, "%s: %d x %d is too large", name, rows, cols);
     return VNM_OK;
 }
 
@@ -65,7 +66,11 @@ int check_sums(const char *name, const void *colsum, int type, const void *works
     return VNM_OK;
 }
 
-bool pieces(const void *x, int type, int64_t ld) { return aligned(x, 16) && ld * elem_size(type) % 16 == 0; }
+int row_alignment(const void *x, int type, int64_t ld)
+{
+    const uintptr_t both = reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ld * elem_size(type));
+    return (both & 15) == 0 ? 16 : (both & 3) == 0 ? 4 : 2;
+}
 
 #define VNM_TRY(call)               \
     do {                            \
@@ -151,7 +156,7 @@ extern "C" int vnm_fp8_quantize(const void *x, int x_type, int64_t ldx, int rows
     if (!data && !data_t) return fail(VNM_ERR_BAD_ARG, "%s: nothing is wanted", name);
     Fp8QuantParams p = {};
     p.x = x; p.ldx = ldx; p.rows = rows; p.cols = cols; p.f8 = f8_type;
-    p.vec_in = pieces(x, x_type, ldx);
+    p.align_x = row_alignment(x, x_type, ldx);
     p.data = static_cast<uint8_t *>(data); p.ldd = ldd; p.scales = static_cast<uint8_t *>(scales);
     p.data_t = static_cast<uint8_t *>(data_t); p.ldt = ldt; p.scales_t = static_cast<uint8_t *>(scales_t);
     p.partial = colsum ? static_cast<float *>(workspace) : nullptr;
@@ -188,8 +193,8 @@ extern "C" int vnm_fp8_gelu(const void *x, int x_type, int64_t ldx, int rows, in
     if (!y && !data && !data_t) return fail(VNM_ERR_BAD_ARG, "%s: nothing is wanted", name);
     Fp8QuantParams p = {};
     p.x = x; p.ldx = ldx; p.rows = rows; p.cols = cols; p.f8 = VNM_E4M3; p.tanh_form = tanh_form != 0;
-    p.vec_in = pieces(x, x_type, ldx);
-    p.y = y; p.ldy = ldy;
+    p.align_x = row_alignment(x, x_type, ldx);
+    p.y = y; p.ldy = ldy; p.align_y = row_alignment(y, x_type, ldy);
     p.data = static_cast<uint8_t *>(data); p.ldd = ldd; p.scales = static_cast<uint8_t *>(scales);
     p.data_t = static_cast<uint8_t *>(data_t); p.ldt = ldt; p.scales_t = static_cast<uint8_t *>(scales_t);
     p.ckpt = static_cast<uint8_t *>(ckpt); p.ldc = ldc; p.ckpt_scales = static_cast<uint8_t *>(ckpt_scales);
@@ -216,8 +221,8 @@ extern "C" int vnm_fp8_gelu_grad(const void *dy, int dy_type, int64_t ldy, int r
     if (!dx && !data && !data_t) return fail(VNM_ERR_BAD_ARG, "%s: nothing is wanted", name);
     Fp8QuantParams p = {};
     p.x = dy; p.ldx = ldy; p.rows = rows; p.cols = cols; p.f8 = f8_type; p.tanh_form = tanh_form != 0;
-    p.vec_in = pieces(dy, dy_type, ldy);
-    p.y = dx; p.ldy = lddx;
+    p.align_x = row_alignment(dy, dy_type, ldy);
+    p.y = dx; p.ldy = lddx; p.align_y = row_alignment(dx, dy_type, lddx);
     p.data = static_cast<uint8_t *>(data); p.ldd = ldd; p.scales = static_cast<uint8_t *>(scales);
     p.data_t = static_cast<uint8_t *>(data_t); p.ldt = ldt; p.scales_t = static_cast<uint8_t *>(scales_t);
     p.ckpt = static_cast<uint8_t *>(const_cast<void *>(ckpt)); p.ldc = ldc; p.ckpt_scales = static_cast<uint8_t *>(const_cast<void *>(ckpt_scales));

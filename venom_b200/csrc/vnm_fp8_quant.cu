@@ -21,9 +21,6 @@ template <> struct Elem<T_F32> { using type = float; };
 template <> struct Elem<T_F16> { using type = __half; };
 template <> struct Elem<T_BF16> { using type = __nv_bfloat16; };
 
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <int TYPE>
 __device__ __forceinline__ typename Elem<TYPE>::type from_float(float x)
 {
@@ -32,60 +29,86 @@ __device__ __forceinline__ typename Elem<TYPE>::type from_float(float x)
     else return __float2bfloat16_rn(x);
 }
 
-// Eight neighbouring values of a row from column c on; what lies past `cols` is zero.
+// Eight neighbouring values of a row as they lie: four words of 16-bit values or eight of 32.
 template <int TYPE>
-__device__ __forceinline__ void load8(const void *x, int64_t at, int c, int cols, bool vec, float (&v)[8])
+struct Raw {
+    static constexpr int WORDS = TYPE == T_F32 ? 8 : 4;
+    uint32_t w[WORDS];
+};
+// `align`: what the rows' addresses are a multiple of, 16 or 4 bytes or the type's size.  What lies past `cols` is zero.
+template <int TYPE>
+__device__ __forceinline__ Raw<TYPE> load_raw(const void *x, int64_t at, int c, int cols, int align)
 {
     using E = typename Elem<TYPE>::type;
+    Raw<TYPE> r;
     const E *src = reinterpret_cast<const E *>(x) + at + c;
-    if (vec && c + 8 <= cols) {
-        if constexpr (TYPE == T_F32) {
-            const float4 a = __ldg(reinterpret_cast<const float4 *>(src)), b = __ldg(reinterpret_cast<const float4 *>(src) + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 q = __ldg(reinterpret_cast<const uint4 *>(src));
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    if (c + 8 <= cols && align >= 4) {
+        if (align == 16) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if constexpr (TYPE == T_F16) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                    v[2 * i] = f.x;
-                    v[2 * i + 1] = f.y;
-                } else {
-                    v[2 * i] = __uint_as_float(w[i] << 16);
-                    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-                }
+            for (int i = 0; i < Raw<TYPE>::WORDS / 4; i++) {
+                const uint4 q = __ldg(reinterpret_cast<const uint4 *>(src) + i);
+                r.w[4 * i] = q.x; r.w[4 * i + 1] = q.y; r.w[4 * i + 2] = q.z; r.w[4 * i + 3] = q.w;
             }
-        }
-    } else {
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = c + i < cols ? to_float(src[i]) : 0.0f;
+            for (int i = 0; i < Raw<TYPE>::WORDS; i++) r.w[i] = __ldg(reinterpret_cast<const uint32_t *>(src) + i);
+        }
+    } else if constexpr (TYPE == T_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) r.w[i] = c + i < cols ? __ldg(reinterpret_cast<const uint32_t *>(src) + i) : 0u;
+    } else {
+        const unsigned short *h = reinterpret_cast<const unsigned short *>(src);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t lo = c + 2 * i < cols ? __ldg(h + 2 * i) : 0u, hi = c + 2 * i + 1 < cols ? __ldg(h + 2 * i + 1) : 0u;
+            r.w[i] = lo | (hi << 16);
+        }
+    }
+    return r;
+}
+template <int TYPE>
+__device__ __forceinline__ void to_floats(const Raw<TYPE> &r, float (&v)[8])
+{
+#pragma unroll
+    for (int i = 0; i < Raw<TYPE>::WORDS; i++) {
+        if constexpr (TYPE == T_F32) {
+            v[i] = __uint_as_float(r.w[i]);
+        } else if constexpr (TYPE == T_F16) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r.w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        } else {
+            v[2 * i] = __uint_as_float(r.w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(r.w[i] & 0xFFFF0000u);
+        }
     }
 }
 
 template <int TYPE>
-__device__ __forceinline__ void store8(void *y, int64_t at, int c, int cols, bool vec, const float (&v)[8])
+__device__ __forceinline__ void store8(void *y, int64_t at, int c, int cols, int align, const float (&v)[8])
 {
     using E = typename Elem<TYPE>::type;
     E *dst = reinterpret_cast<E *>(y) + at + c;
-    if (vec && c + 8 <= cols) {
-        if constexpr (TYPE == T_F32) {
-            reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            uint32_t w[4];
+    if (c + 8 <= cols && align >= 4) {
+        uint32_t w[Raw<TYPE>::WORDS];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if constexpr (TYPE == T_F16) {
-                    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t *>(&h);
-                } else {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t *>(&h);
-                }
+        for (int i = 0; i < Raw<TYPE>::WORDS; i++) {
+            if constexpr (TYPE == T_F32) {
+                w[i] = __float_as_uint(v[i]);
+            } else if constexpr (TYPE == T_F16) {
+                const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
             }
-            *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (align == 16) {
+#pragma unroll
+            for (int i = 0; i < Raw<TYPE>::WORDS / 4; i++) reinterpret_cast<uint4 *>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < Raw<TYPE>::WORDS; i++) reinterpret_cast<uint32_t *>(dst)[i] = w[i];
         }
     } else {
 #pragma unroll
@@ -95,64 +118,91 @@ __device__ __forceinline__ void store8(void *y, int64_t at, int c, int cols, boo
 }
 
 // ---- scales ----
-constexpr uint32_t INF_BITS = 0x7F800000u;
-
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
-__device__ __forceinline__ uint32_t finite_bits(float x) { const uint32_t b = abs_bits(x); return b < INF_BITS ? b : 0u; }
-
-// The scale's byte (its exponent + 127) for a block whose largest finite magnitude has these bits.
-__device__ __forceinline__ uint32_t scale_code(uint32_t amax_bits, int f8)
+// The scale's byte (its exponent + 127) for a block whose largest finite magnitude is amax.
+__device__ __forceinline__ uint32_t scale_code(float amax, int f8)
 {
-    const int e = (int)((amax_bits + 0x1FFFFFu) >> 23) - (f8 == F8_E4M3 ? 8 : 15);
+    const int e = (int)((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - (f8 == F8_E4M3 ? 8 : 15);
     return e > 0 ? (uint32_t)e : 0u;
 }
 __device__ __forceinline__ float inverse_scale(uint32_t code) { return __uint_as_float((254u - code) << 23); }
 __device__ __forceinline__ float scale_value(uint32_t code) { return code ? __uint_as_float(code << 23) : __uint_as_float(0x00400000u); }
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < __uint_as_float(0x7F800000u); }
 
-// (a, b) / s in 8 bits, a in the low byte.  `odd`: the block holds values that are not finite.
-__device__ __forceinline__ uint32_t round2(float a, float b, float inv, int f8, bool odd)
+// The maximum passes over NaN; an infinity shows in it, and takes its block (`odd`) through the slow forms below.
+__device__ __forceinline__ float amax8(const float (&v)[8])
+{
+    const float a = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), b = fmaxf(fmaxf(fabsf(v[4]), fabsf(v[5])), fmaxf(fabsf(v[6]), fabsf(v[7])));
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float finite_amax8(const float (&v)[8])
+{
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = finite(v[i]) ? fmaxf(m, fabsf(v[i])) : m;
+    return m;
+}
+
+// (a, b) / s in 8 bits, a in the low byte.
+__device__ __forceinline__ uint32_t round2(float a, float b, float inv, int f8)
 {
     const float2 v = make_float2(a * inv, b * inv);
-    const __nv_fp8_interpretation_t kind = f8 == F8_E4M3 ? __NV_E4M3 : __NV_E5M2;
-    if (odd) return __nv_cvt_float2_to_fp8x2(v, __NV_NOSAT, kind);   // an infinity stays one or becomes NaN
     if (f8 == F8_E4M3) return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
     return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E5M2);
 }
-__device__ __forceinline__ uint2 round8(const float (&v)[8], float inv, int f8, bool odd)
+__device__ __forceinline__ uint2 round8(const float (&v)[8], float inv, int f8)
 {
     uint2 r;
-    r.x = round2(v[0], v[1], inv, f8, odd) | (round2(v[2], v[3], inv, f8, odd) << 16);
-    r.y = round2(v[4], v[5], inv, f8, odd) | (round2(v[6], v[7], inv, f8, odd) << 16);
+    r.x = __byte_perm(round2(v[0], v[1], inv, f8), round2(v[2], v[3], inv, f8), 0x5410);
+    r.y = __byte_perm(round2(v[4], v[5], inv, f8), round2(v[6], v[7], inv, f8), 0x5410);
     return r;
 }
+// Four rounded values of a block with infinities, which the conversion has made the largest value: they stay infinities in e5m2 and become NaN in e4m3.
+__device__ __forceinline__ uint32_t mend4(uint32_t w, float a, float b, float c, float d, int f8)
+{
+    const float v[4] = {a, b, c, d};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t bits = __float_as_uint(v[i]);
+        if ((bits & 0x7FFFFFFFu) == 0x7F800000u) w = (w & ~(0xFFu << (8 * i))) | ((((bits >> 24) & 0x80u) | (f8 == F8_E4M3 ? 0x7Fu : 0x7Cu)) << (8 * i));
+    }
+    return w;
+}
+__device__ __forceinline__ uint2 mend8(uint2 r, const float (&v)[8], int f8)
+{
+    return make_uint2(mend4(r.x, v[0], v[1], v[2], v[3], f8), mend4(r.y, v[4], v[5], v[6], v[7], f8));
+}
 
-// Largest of the sixteen lanes that share a row's block.
-__device__ __forceinline__ uint32_t max16(uint32_t b)
+// Largest of sixteen lanes for four values at once: lanes exchange the values that they do not keep, so that five shuffles do, and each lane ends with
+// value (lane >> 2) & 3 ...
+__device__ __forceinline__ float max16_of4(float a0, float a1, float a2, float a3)
 {
-#pragma unroll
-    for (int o = 8; o; o >>= 1) {
-        const uint32_t n = __shfl_xor_sync(0xffffffffu, b, o);
-        b = n > b ? n : b;
-    }
-    return b;
+    const bool h8 = (threadIdx.x & 8) != 0, h4 = (threadIdx.x & 4) != 0;
+    const float r0 = __shfl_xor_sync(0xffffffffu, h8 ? a0 : a2, 8), r1 = __shfl_xor_sync(0xffffffffu, h8 ? a1 : a3, 8);
+    const float b0 = fmaxf(h8 ? a2 : a0, r0), b1 = fmaxf(h8 ? a3 : a1, r1);
+    float c = fmaxf(h4 ? b1 : b0, __shfl_xor_sync(0xffffffffu, h4 ? b0 : b1, 4));
+    c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, 2));
+    return fmaxf(c, __shfl_xor_sync(0xffffffffu, c, 1));
 }
-// The block of eight values a lane: bits of the largest finite magnitude, and whether others are in it.
-__device__ __forceinline__ uint32_t row_amax(const float (&v)[8], bool *odd)
+// ... whose byte goes back to all sixteen: byte i of the result belongs to value i.
+__device__ __forceinline__ uint32_t bytes_of4(uint32_t code)
 {
-    uint32_t b = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) { const uint32_t a = abs_bits(v[i]); b = a > b ? a : b; }
-    b = max16(b);
-    *odd = b >= INF_BITS;
-    if (__any_sync(0xffffffffu, *odd)) {
-        uint32_t f = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) { const uint32_t a = finite_bits(v[i]); f = a > f ? a : f; }
-        f = max16(f);
-        if (*odd) b = f;
-    }
-    return b;
+    uint32_t w = code << (8 * ((threadIdx.x >> 2) & 3));
+    w |= __shfl_xor_sync(0xffffffffu, w, 4);
+    w |= __shfl_xor_sync(0xffffffffu, w, 8);
+    return w;
 }
+// Codes of four blocks of eight values a lane; bit i of *odd: block i has an infinity.
+__device__ __forceinline__ uint32_t codes_of4(const float (&v)[4][8], int f8, uint32_t *odd)
+{
+    float m = max16_of4(amax8(v[0]), amax8(v[1]), amax8(v[2]), amax8(v[3]));
+    *odd = 0;
+    if (__any_sync(0xffffffffu, !finite(m))) {
+        *odd = bytes_of4(finite(m) ? 0u : 1u);
+        m = max16_of4(finite_amax8(v[0]), finite_amax8(v[1]), finite_amax8(v[2]), finite_amax8(v[3]));
+    }
+    return bytes_of4(scale_code(m, f8));
+}
+__device__ __forceinline__ uint32_t byte_of(uint32_t w, int i) { return (w >> (8 * i)) & 0xFFu; }
 
 // Byte of block `kb` in the scales of a matrix of `n` rows; the last block's writer also sets what pads its word.
 __device__ __forceinline__ void store_scale(uint8_t *scales, int64_t n, int64_t row, int kb, int blocks, uint32_t code)
@@ -164,60 +214,74 @@ __device__ __forceinline__ void store_scale(uint8_t *scales, int64_t n, int64_t 
 }
 
 // ---- GELU ----
+__device__ __forceinline__ float fast_exp2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float fast_rcp(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 // The exact form by a published approximation of erfc (Abramowitz and Stegun, 7.1.26, |error| <= 1.5e-7): with t = 1 / (1 + p |z|), z = x / sqrt 2,
 // erfc |z| = (a1 t + .. + a5 t^5) exp(-z^2).  The exponential is the density's as well, which the derivative needs, so one exponential and one reciprocal
-// give both.  The tail of negative x has no cancellation.
-__device__ __forceinline__ void gelu_erf(float x, float *cdf, float *density)
+// give both.  With h = erfc |z| / 2, gelu(x) = max(x, 0) - |x| h: no cancellation in the tail of negative x.
+__device__ __forceinline__ float half_erfc(float x, float *e)
 {
-    const float z = fabsf(x) * 0.70710678118654752f;
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
-    const float e = exp2f(x * x * -0.72134752044448170f);
-    float poly = fmaf(1.061405429f, t, -1.453152027f);
-    poly = fmaf(poly, t, 1.421413741f);
-    poly = fmaf(poly, t, -0.284496736f);
-    poly = fmaf(poly, t, 0.254829592f);
-    const float half_erfc = 0.5f * poly * t * e;
-    *cdf = x < 0.0f ? half_erfc : 1.0f - half_erfc;
-    *density = e * 0.39894228040143268f;
+    const float t = fast_rcp(fmaf(0.3275911f * 0.70710678118654752f, fabsf(x), 1.0f));
+    *e = fast_exp2(x * (x * -0.72134752044448170f));
+    float poly = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    poly = fmaf(poly, t, 0.5f * 1.421413741f);
+    poly = fmaf(poly, t, 0.5f * -0.284496736f);
+    poly = fmaf(poly, t, 0.5f * 0.254829592f);
+    return poly * t * *e;
 }
 // The tanh form: (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
 __device__ __forceinline__ float gelu_sigmoid(float x, float *du2)
 {
-    x = x > 64.0f ? 64.0f : x < -64.0f ? -64.0f : x;   // the square of a large x would overflow beside a zero; NaN stays
     const float x2 = x * x;
-    const float u2 = x * fmaf(0.0713548162726f, x2, 1.59576912160573f);
     *du2 = fmaf(0.214064448817801f, x2, 1.59576912160573f);
-    return __fdividef(1.0f, 1.0f + exp2f(-1.4426950408889634f * u2));
+    return fast_rcp(1.0f + fast_exp2(x * fmaf(0.0713548162726f * -1.4426950408889634f, x2, 1.59576912160573f * -1.4426950408889634f)));
 }
+__device__ __forceinline__ float max_nan(float a, float b)   // a NaN stays
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b)
+{
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// Beyond 64 either form is x or 0 and the derivative 1 or 0; the square of a far larger x would overflow beside a zero.  So -inf gives 0.
+__device__ __forceinline__ float near(float x) { return max_nan(min_nan(x, 64.0f), -64.0f); }
 __device__ __forceinline__ float gelu(float x, int tanh_form)
 {
-    if (tanh_form) {
-        float d;
-        return x * gelu_sigmoid(x, &d);
-    }
-    float cdf, density;
-    gelu_erf(x, &cdf, &density);
-    return x * cdf;
+    float d;
+    if (tanh_form) return max_nan(x, -64.0f) * gelu_sigmoid(near(x), &d);
+    return fmaf(-min_nan(fabsf(x), 64.0f), half_erfc(x, &d), max_nan(x, 0.0f));
 }
 __device__ __forceinline__ float gelu_grad(float x, int tanh_form)
 {
+    float d;
     if (tanh_form) {
-        float d;
+        x = near(x);
         const float s = gelu_sigmoid(x, &d);
-        x = x > 64.0f ? 64.0f : x < -64.0f ? -64.0f : x;
         return fmaf(x * s * (1.0f - s), d, s);
     }
-    float cdf, density;
-    gelu_erf(x, &cdf, &density);
-    return fmaf(x, density, cdf);
+    const float h = half_erfc(x, &d);
+    return fmaf(x, d * 0.39894228040143268f, x < 0.0f ? h : 1.0f - h);
 }
 
-// Eight values of an e4m3 checkpoint.
-__device__ __forceinline__ void load_ckpt8(const Fp8QuantParams &p, int64_t row, int c, float (&h)[8])
+// Eight values of an e4m3 checkpoint whose block has this code.
+__device__ __forceinline__ void ckpt_values(uint2 q, uint32_t code, float (&h)[8])
 {
-    const uint2 q = __ldg(reinterpret_cast<const uint2 *>(p.ckpt + row * p.ldc + c));
-    const int kb = c >> 7;
-    const float s = scale_value(__ldg(p.ckpt_scales + ((int64_t)(kb >> 2) * p.rows + row) * 4 + (kb & 3)));
+    const float s = scale_value(code);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint32_t w = (i < 2 ? q.x : q.y) >> (16 * (i & 1));
@@ -228,62 +292,95 @@ __device__ __forceinline__ void load_ckpt8(const Fp8QuantParams &p, int64_t row,
     }
 }
 
-// ---- rows only: sixteen lanes a block, several blocks a lane ----
-// Reads and writes every value once; bound by HBM, and by launch and latency for few rows.
+// ---- rows only ----
+// Sixteen lanes take four blocks of a row, whose bytes are one scale word; a lane holds eight values of each.  The next four blocks are on their way while these
+// are worked on.  Every value is read and written once; bound by HBM, and by launch and latency for few rows.
 constexpr int ROWS_THREADS = 256;
-constexpr int ROWS_UNROLL = 4;
 
 template <int TYPE, int OP>
-__global__ void __launch_bounds__(ROWS_THREADS) fp8_rows_kernel(const Fp8QuantParams p)
+__global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN ? 2 : 3) fp8_rows_kernel(const Fp8QuantParams p)
 {
     grid_dependency_wait();
     grid_launch_dependents();
-    const int blocks = (int)(((int64_t)p.cols + 127) >> 7);
-    const int64_t total = (int64_t)p.rows * blocks;
-    const int64_t first = ((int64_t)blockIdx.x * ROWS_THREADS + threadIdx.x) >> 4;
-    const int64_t step = (int64_t)gridDim.x * (ROWS_THREADS / 16);
+    const uint32_t groups = (uint32_t)(((int64_t)p.cols + 511) >> 9), total = groups * (uint32_t)p.rows;
+    const uint32_t first = (blockIdx.x * ROWS_THREADS + threadIdx.x) >> 4, step = gridDim.x * (ROWS_THREADS / 16);
+    const uint32_t step_rows = step / groups, step_groups = step - step_rows * groups;
     const int sub = (int)(threadIdx.x & 15) * 8;
-    const bool vec_y = OP != FP8_PLAIN && p.y && ((p.ldy * (int64_t)sizeof(typename Elem<TYPE>::type)) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
-    for (int64_t u0 = first; u0 - (threadIdx.x >> 4) % 2 < total; u0 += step * ROWS_UNROLL) {   // both halves of a warp stay until its first one is through
-        float v[ROWS_UNROLL][8];
+    uint32_t u = first, row = first / groups, g = first - row * groups;
+
+    Raw<TYPE> next[4];
+    uint2 next_h[4];
+    uint32_t next_codes = 0;
+    auto fetch = [&](uint32_t unit, uint32_t r, uint32_t gr) {
+        const int c = (int)gr * 512 + sub;
 #pragma unroll
-        for (int j = 0; j < ROWS_UNROLL; j++) {
-            const int64_t u = u0 + j * step;
-            const int64_t row = u / blocks;
-            const int c = (int)(u - row * blocks) * 128 + sub;
-            load8<TYPE>(p.x, row * p.ldx, c, u < total ? p.cols : 0, p.vec_in != 0, v[j]);
+        for (int i = 0; i < 4; i++) next[i] = load_raw<TYPE>(p.x, (int64_t)r * p.ldx, c + 128 * i, unit < total ? p.cols : 0, p.align_x);
+        if constexpr (OP == FP8_GELU_GRAD) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                next_h[i] = unit < total && c + 128 * i < p.cols ? __ldg(reinterpret_cast<const uint2 *>(p.ckpt + (int64_t)r * p.ldc + c + 128 * i)) : make_uint2(0u, 0u);
+            next_codes = unit < total ? __ldg(reinterpret_cast<const uint32_t *>(p.ckpt_scales) + (int64_t)gr * p.rows + r) : 0u;
         }
+    };
+    fetch(u, row, g);
+    for (; u - ((threadIdx.x >> 4) & 1) < total;) {          // the halves of a warp stay together
+        const bool on = u < total;
+        const int64_t r = row;
+        const int c = (int)g * 512 + sub;
+        const int64_t word = (int64_t)g * p.rows + r;
+        float v[4][8];
 #pragma unroll
-        for (int j = 0; j < ROWS_UNROLL; j++) {
-            const int64_t u = u0 + j * step;
-            const bool on = u < total;
-            const int64_t row = on ? u / blocks : 0;
-            const int kb = on ? (int)(u - row * blocks) : 0, c = kb * 128 + sub;
-            const bool in = on && c < p.cols;
-            bool odd;
-            if constexpr (OP == FP8_GELU) {
-                if (p.ckpt) {
-                    const uint32_t code = scale_code(row_amax(v[j], &odd), F8_E4M3);
-                    if (in) *reinterpret_cast<uint2 *>(p.ckpt + row * p.ldc + c) = round8(v[j], inverse_scale(code), F8_E4M3, odd);
-                    if (on && sub == 0) store_scale(p.ckpt_scales, p.rows, row, kb, blocks, code);
+        for (int i = 0; i < 4; i++) to_floats<TYPE>(next[i], v[i]);
+        uint2 h[4];
+        uint32_t h_codes = 0;
+        if constexpr (OP == FP8_GELU_GRAD) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) h[i] = next_h[i];
+            h_codes = next_codes;
+        }
+        u += step;
+        row += step_rows;
+        g += step_groups;
+        if (g >= groups) { g -= groups; row++; }
+        fetch(u, row, g);
+
+        auto store = [&](uint8_t *data, int64_t ld, uint8_t *scales, int f8) {
+            uint32_t odd;
+            const uint32_t codes = codes_of4(v, f8, &odd);
+            if (on) {
+                uint8_t *dst = data + r * ld + c;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float inv = inverse_scale(byte_of(codes, i));
+                    uint2 q = round8(v[i], inv, f8);
+                    if (byte_of(odd, i)) q = mend8(q, v[i], f8);
+                    if (c + 128 * i < p.cols) *reinterpret_cast<uint2 *>(dst + 128 * i) = q;
                 }
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[j][i] = gelu(v[j][i], p.tanh_form);
-            } else if constexpr (OP == FP8_GELU_GRAD) {
-                if (in) {
-                    float h[8];
-                    load_ckpt8(p, row, c, h);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v[j][i] *= gelu_grad(h[i], p.tanh_form);
-                }
+                // blocks past the last one are zeros, whose code is 0
+                if (sub == 0) reinterpret_cast<uint32_t *>(scales)[word] = codes;
             }
-            if (OP != FP8_PLAIN && p.y && in) store8<TYPE>(p.y, row * p.ldy, c, p.cols, vec_y, v[j]);
-            if (p.data) {
-                const uint32_t code = scale_code(row_amax(v[j], &odd), p.f8);
-                if (in) *reinterpret_cast<uint2 *>(p.data + row * p.ldd + c) = round8(v[j], inverse_scale(code), p.f8, odd);
-                if (on && sub == 0) store_scale(p.scales, p.rows, row, kb, blocks, code);
+        };
+        if constexpr (OP == FP8_GELU) {
+            if (p.ckpt) store(p.ckpt, p.ldc, p.ckpt_scales, F8_E4M3);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[i][j] = gelu(v[i][j], p.tanh_form);
+        } else if constexpr (OP == FP8_GELU_GRAD) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float x[8];
+                ckpt_values(h[i], byte_of(h_codes, i), x);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[i][j] *= gelu_grad(x[j], p.tanh_form);
             }
         }
+        if (OP != FP8_PLAIN && p.y && on) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (c + 128 * i < p.cols) store8<TYPE>(p.y, r * p.ldy, c + 128 * i, p.cols, p.align_y, v[i]);
+        }
+        if (p.data) store(p.data, p.ldd, p.scales, p.f8);
     }
 }
 
@@ -296,9 +393,9 @@ template <int TYPE, int OP, bool SQUARE>
 __global__ void __launch_bounds__(TILE_THREADS, 2) fp8_tiles_kernel(const Fp8QuantParams p)
 {
     __shared__ uint32_t image[128 * 32];
-    __shared__ uint32_t amax_of[16][128];
+    __shared__ float amax_of[16][128];
     __shared__ float inv_of[128];
-    __shared__ uint32_t all[16], all_finite[16];
+    __shared__ float all[16];
     grid_dependency_wait();
     grid_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -308,95 +405,108 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) fp8_tiles_kernel(const Fp8Qua
     const int c = tc * 128 + group * 8;
     const int64_t r0 = (int64_t)tr * 128 + warp * 8 + half * 4;
     const bool in = c < p.cols;
+    const int own_row = (lane >> 2) & 3;                       // the row whose code this lane stores (lanes 0, 4, 8, 12 of a half)
 
     float v[4][8];
+    {
+        Raw<TYPE> raw[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) load8<TYPE>(p.x, (r0 + j) * p.ldx, c, r0 + j < p.rows ? p.cols : 0, p.vec_in != 0, v[j]);
-    if constexpr (OP == FP8_GELU) {
-        if (p.ckpt) {
+        for (int j = 0; j < 4; j++) raw[j] = load_raw<TYPE>(p.x, (r0 + j) * p.ldx, c, r0 + j < p.rows ? p.cols : 0, p.align_x);
+        uint2 q[4];
+        uint32_t codes[4];
+        if constexpr (OP == FP8_GELU_GRAD) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                bool odd;
-                const uint32_t code = scale_code(row_amax(v[j], &odd), F8_E4M3);
-                if (in && r0 + j < p.rows) *reinterpret_cast<uint2 *>(p.ckpt + (r0 + j) * p.ldc + c) = round8(v[j], inverse_scale(code), F8_E4M3, odd);
-                if (group == 0 && r0 + j < p.rows) store_scale(p.ckpt_scales, p.rows, r0 + j, tc, cblocks, code);
+                const bool there = in && r0 + j < p.rows;
+                q[j] = there ? __ldg(reinterpret_cast<const uint2 *>(p.ckpt + (r0 + j) * p.ldc + c)) : make_uint2(0u, 0u);
+                codes[j] = there ? __ldg(p.ckpt_scales + ((int64_t)(tc >> 2) * p.rows + r0 + j) * 4 + (tc & 3)) : 0u;
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[j][i] = gelu(v[j][i], p.tanh_form);   // of the zeros that pad: zero
-    } else if constexpr (OP == FP8_GELU_GRAD) {
-#pragma unroll
         for (int j = 0; j < 4; j++) {
-            if (in && r0 + j < p.rows) {
+            to_floats<TYPE>(raw[j], v[j]);
+            if constexpr (OP == FP8_GELU_GRAD) {
                 float h[8];
-                load_ckpt8(p, r0 + j, c, h);
+                ckpt_values(q[j], codes[j], h);
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[j][i] *= gelu_grad(h[i], p.tanh_form);
             }
         }
     }
+    auto store_rows = [&](uint8_t *data, int64_t ld, uint8_t *scales, int f8, uint32_t codes, uint32_t odd) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float inv = inverse_scale(byte_of(codes, j));
+            uint2 q = round8(v[j], inv, f8);
+            if (byte_of(odd, j)) q = mend8(q, v[j], f8);
+            if (in && r0 + j < p.rows) *reinterpret_cast<uint2 *>(data + (r0 + j) * ld + c) = q;
+        }
+        if ((lane & 3) == 0 && r0 + own_row < p.rows) store_scale(scales, p.rows, r0 + own_row, tc, cblocks, byte_of(codes, own_row));
+    };
+    if constexpr (OP == FP8_GELU) {
+        if (p.ckpt) {
+            uint32_t odd;
+            const uint32_t codes = codes_of4(v, F8_E4M3, &odd);
+            store_rows(p.ckpt, p.ldc, p.ckpt_scales, F8_E4M3, codes, odd);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[j][i] = gelu(v[j][i], p.tanh_form);   // of the zeros that pad: zero
+    }
 
     uint32_t tile_code = 0;
     bool tile_odd = false;
     if constexpr (SQUARE) {
-        uint32_t b = 0, f = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const uint32_t a = abs_bits(v[j][i]), g = finite_bits(v[j][i]);
-                b = a > b ? a : b;
-                f = g > f ? g : f;
-            }
-        b = __reduce_max_sync(0xffffffffu, b);
-        f = __reduce_max_sync(0xffffffffu, f);
-        if (lane == 0) { all[warp] = b; all_finite[warp] = f; }
+        float m = fmaxf(fmaxf(amax8(v[0]), amax8(v[1])), fmaxf(amax8(v[2]), amax8(v[3])));
+        m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));   // of values that are not negative: their bits' order
+        if (lane == 0) all[warp] = m;
         __syncthreads();
-        b = f = 0;
+        m = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 16; w++) { b = all[w] > b ? all[w] : b; f = all_finite[w] > f ? all_finite[w] : f; }
-        tile_odd = b >= INF_BITS;
-        tile_code = scale_code(f, p.f8);
+        for (int w = 0; w < 16; w++) m = fmaxf(m, all[w]);
+        tile_odd = !finite(m);
+        if (tile_odd) {
+            m = fmaxf(fmaxf(finite_amax8(v[0]), finite_amax8(v[1])), fmaxf(finite_amax8(v[2]), finite_amax8(v[3])));
+            m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+            __syncthreads();
+            if (lane == 0) all[warp] = m;
+            __syncthreads();
+            m = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 16; w++) m = fmaxf(m, all[w]);
+        }
+        tile_code = scale_code(m, p.f8);
     }
 
     if (p.data) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            bool odd = tile_odd;
-            uint32_t code = tile_code;
-            if constexpr (!SQUARE) code = scale_code(row_amax(v[j], &odd), p.f8);
-            if (in && r0 + j < p.rows) *reinterpret_cast<uint2 *>(p.data + (r0 + j) * p.ldd + c) = round8(v[j], inverse_scale(code), p.f8, odd);
-            if (group == 0 && r0 + j < p.rows) store_scale(p.scales, p.rows, r0 + j, tc, cblocks, code);
-        }
+        uint32_t odd = tile_odd ? 0x01010101u : 0u, codes = tile_code * 0x01010101u;
+        if constexpr (!SQUARE) codes = codes_of4(v, p.f8, &odd);
+        store_rows(p.data, p.ldd, p.scales, p.f8, codes, odd);
     }
 
     if (p.data_t) {
         float inv[8];
         if constexpr (!SQUARE) {
-#pragma unroll
-            for (int pass = 0; pass < 2; pass++) {   // the second one only for columns with values that are not finite: see below
+#pragma unroll 1
+            for (int pass = 0; pass < 2; pass++) {   // the second one only where a column has an infinity
                 if (pass == 1 && !__syncthreads_or(threadIdx.x < 128 && inv_of[threadIdx.x & 127] < 0.0f)) break;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    uint32_t b = 0;
+                    float m = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t a = pass ? finite_bits(v[j][i]) : abs_bits(v[j][i]);
-                        b = a > b ? a : b;
-                    }
-                    const uint32_t n = __shfl_xor_sync(0xffffffffu, b, 16);
-                    if (half == 0) amax_of[warp][group * 8 + i] = n > b ? n : b;
+                    for (int j = 0; j < 4; j++) m = pass && !finite(v[j][i]) ? m : fmaxf(m, fabsf(v[j][i]));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    if (half == 0) amax_of[warp][group * 8 + i] = m;
                 }
                 __syncthreads();
                 if (threadIdx.x < 128) {
-                    uint32_t b = 0;
+                    float m = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < 16; w++) b = amax_of[w][threadIdx.x] > b ? amax_of[w][threadIdx.x] : b;
-                    const bool odd = pass == 0 ? b >= INF_BITS : inv_of[threadIdx.x] < 0.0f;
-                    const uint32_t code = scale_code(b < INF_BITS ? b : 0u, p.f8);
-                    inv_of[threadIdx.x] = odd ? -inverse_scale(code) : inverse_scale(code);   // the sign says that some are not finite
+                    for (int w = 0; w < 16; w++) m = fmaxf(m, amax_of[w][threadIdx.x]);
+                    const bool odd = pass == 0 ? !finite(m) : inv_of[threadIdx.x] < 0.0f;
+                    const uint32_t code = scale_code(finite(m) ? m : 0.0f, p.f8);
+                    inv_of[threadIdx.x] = odd ? -inverse_scale(code) : inverse_scale(code);   // the sign says that it has one
                     const int col = tc * 128 + (int)threadIdx.x;
                     if (col < p.cols) store_scale(p.scales_t, p.cols, col, tr, rblocks, code);
                 }
@@ -411,9 +521,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) fp8_tiles_kernel(const Fp8Qua
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const bool odd = inv[i] < 0.0f;
-            const float s = fabsf(inv[i]);
-            image[(group * 8 + i) * 32 + ((warp * 2 + half) ^ (2 * group))] = round2(v[0][i], v[1][i], s, p.f8, odd) | (round2(v[2][i], v[3][i], s, p.f8, odd) << 16);
+            const float a = fabsf(inv[i]);
+            uint32_t w = __byte_perm(round2(v[0][i], v[1][i], a, p.f8), round2(v[2][i], v[3][i], a, p.f8), 0x5410);
+            if (inv[i] < 0.0f) w = mend4(w, v[0][i], v[1][i], v[2][i], v[3][i], p.f8);
+            image[(group * 8 + i) * 32 + ((warp * 2 + half) ^ (2 * group))] = w;
         }
         __syncthreads();
         const int64_t padded = ((int64_t)p.rows + 15) & ~(int64_t)15;
@@ -429,19 +540,18 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) fp8_tiles_kernel(const Fp8Qua
 
     if (p.partial) {
         __syncthreads();   // amax_of is read no more
-        float (*sum_of)[128] = reinterpret_cast<float (*)[128]>(amax_of);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             float s = (v[0][i] + v[1][i]) + (v[2][i] + v[3][i]);
             s += __shfl_xor_sync(0xffffffffu, s, 16);
-            if (half == 0) sum_of[warp][group * 8 + i] = s;
+            if (half == 0) amax_of[warp][group * 8 + i] = s;
         }
         __syncthreads();
         const int col = tc * 128 + (int)threadIdx.x;
         if (threadIdx.x < 128 && col < p.cols) {
             float s = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 16; w++) s += sum_of[w][threadIdx.x];
+            for (int w = 0; w < 16; w++) s += amax_of[w][threadIdx.x];
             p.partial[(int64_t)tr * p.cols + col] = s;
         }
     }
@@ -514,12 +624,9 @@ int device_sms()
 template <int TYPE>
 cudaError_t rows_of(const Fp8QuantParams &p, int op, cudaStream_t stream)
 {
-    const int64_t units = (int64_t)p.rows * (((int64_t)p.cols + 127) / 128), per_cta = ROWS_THREADS / 16;
-    // one pass of the loop where that fills the GPU, so that every load is on its way at once
-    int64_t ctas = (units + per_cta * ROWS_UNROLL - 1) / (per_cta * ROWS_UNROLL);
-    const int64_t wave = (int64_t)device_sms() * 8;
-    if (ctas < wave / 8) ctas = (units + per_cta - 1) / per_cta < wave / 8 ? (units + per_cta - 1) / per_cta : wave / 8;
-    if (ctas > wave) ctas = wave;
+    const int64_t units = (int64_t)p.rows * (((int64_t)p.cols + 511) / 512), per_cta = ROWS_THREADS / 16;
+    const int64_t wave = (int64_t)device_sms() * (TYPE == T_F32 || op != FP8_PLAIN ? 2 : 3);
+    const int64_t ctas = (units + per_cta - 1) / per_cta < wave ? (units + per_cta - 1) / per_cta : wave;
     const dim3 grid((unsigned)ctas);
     if (op == FP8_PLAIN) return launch(fp8_rows_kernel<TYPE, FP8_PLAIN>, grid, ROWS_THREADS, stream, p);
     if (op == FP8_GELU) return launch(fp8_rows_kernel<TYPE, FP8_GELU>, grid, ROWS_THREADS, stream, p);

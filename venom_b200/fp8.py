@@ -15,7 +15,6 @@ Everything runs on the CUDA device of its operands and on torch's current stream
 There is no CPU path.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import spatha_module
 from .capi import VenomError
@@ -95,71 +94,9 @@ def _flat(x):
     return x if x.dim() == 2 else x.reshape(x.numel() // max(1, x.shape[-1]), x.shape[-1])
 
 
-def _check_linear(x, weight, bias, what):
-    _check_input(x, what)
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.dtype not in _FLOATS or weight.device != x.device:
-        raise VenomError("%s: the weight must be a float16, bfloat16 or float32 matrix on the input's device" % what)
-    if x.shape[-1] != weight.shape[1] or weight.shape[1] < 1:
-        raise VenomError("%s: an input of %s does not match a weight of %s" % (what, tuple(x.shape), tuple(weight.shape)))
-    if bias is not None and (bias.shape != weight.shape[:1] or bias.dtype not in _FLOATS or bias.device != x.device):
-        raise VenomError("%s: the bias must be a vector of %d values on the input's device" % (what, weight.shape[0]))
-
-
 def _check_grad_dtype(grad_dtype, what):
     if grad_dtype not in (E4M3, E5M2):
         raise VenomError("%s: gradients are kept in float8_e4m3fn or float8_e5m2, not %s" % (what, grad_dtype))
-
-
-def _apply(function, tensors, *rest):
-    if torch.cuda.is_current_stream_capturing() and torch.is_grad_enabled():
-        _call("fp8_check_capture", list(tensors))
-    return function.apply(*tensors, *rest)
-
-
-def _weight_grad(dy_t, x_t, dtype):
-    """dy.T @ x from the transposes' 8 bits; zeros without any token."""
-    if dy_t[0].shape[1] == 0:
-        return torch.zeros((dy_t[0].shape[0], x_t[0].shape[0]), dtype=dtype, device=dy_t[0].device)
-    return _call("fp8_matmul", dy_t[0], dy_t[1], x_t[0], x_t[1], None, dtype)
-
-
-def _product(a, b, bias, dtype):
-    return _call("fp8_matmul", a[0], a[1], b[0], b[1], None if bias is None else bias.detach().contiguous(), dtype)
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, grad_dtype):
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        flat = _flat(x)
-        xa, xs, xt, xts, _ = _call("fp8_quantize", flat, E4M3, False, True, need_w, None)
-        wa, ws, wt, wts, _ = _call("fp8_quantize", weight, E4M3, True, True, need_x, None)
-        y = _product((xa, xs), (wa, ws), bias, x.dtype)
-        ctx.save_for_backward(xt, xts, wt, wts)
-        ctx.types = weight.dtype, None if bias is None else bias.dtype, grad_dtype, x.shape, x.dtype
-        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0])
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        xt, xts, wt, wts = ctx.saved_tensors
-        w_dtype, b_dtype, grad_dtype, shape, x_dtype = ctx.types
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        ga, gs, gt, gts, db = _call("fp8_quantize", _flat(dy), grad_dtype, False, need_x, need_w or need_b, b_dtype if need_b else None)
-        dx = _product((ga, gs), (wt, wts), None, x_dtype).reshape(shape) if need_x else None
-        dw = _weight_grad((gt, gts), (xt, xts), w_dtype) if need_w else None
-        return dx, dw, db, None
-
-
-def linear(x, weight, bias=None, grad_dtype=E4M3):
-    """x @ weight.T + bias for x [..., in], weight [out, in] and bias [out], differentiable in all three; the result has the type of x.
-
-    x is rounded in blocks of 128 along its features, the weight in blocks of 128 x 128, gradients in blocks of 128 of `grad_dtype` (float8_e4m3fn
-    or float8_e5m2) along whichever way they are summed.  Kept until the backward pass: the 8-bit transposes of x (where the weight wants a gradient)
-    and of the weight (where x does)."""
-    _check_linear(x, weight, bias, "fp8.linear")
-    _check_grad_dtype(grad_dtype, "fp8.linear")
-    return _apply(_Linear, (x, weight, bias), grad_dtype)
 
 
 def _tanh_form(approximate, what):
@@ -168,75 +105,28 @@ def _tanh_form(approximate, what):
     return approximate == "tanh"
 
 
-class _Gelu(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, tanh_form):
-        y, _, _, _, _, h, hs = _call("fp8_gelu", _flat(x), tanh_form, True, False, False, ctx.needs_input_grad[0])
-        ctx.save_for_backward(h, hs)
-        ctx.tanh_form, ctx.dtype = tanh_form, x.dtype
-        return y.reshape(x.shape)
+def linear(x, weight, bias=None, grad_dtype=E4M3):
+    """x @ weight.T + bias for x [..., in], weight [out, in] and bias [out], differentiable once in all three; the result has the type of x, gradients
+    have their inputs' types.
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        h, hs = ctx.saved_tensors
-        dx = _call("fp8_gelu_grad", _flat(dy), h, hs, ctx.tanh_form, True, E4M3, False, False, None)[0]
-        return dx.reshape(dy.shape), None
+    x is rounded in blocks of 128 along its features, the weight in blocks of 128 x 128, gradients in blocks of 128 of `grad_dtype` (float8_e4m3fn
+    or float8_e5m2) along whichever way they are summed; the bias's gradient is the sum of unrounded ones.  Kept until the backward pass: the 8-bit
+    transposes of x (where the weight wants a gradient) and of the weight (where x does)."""
+    return _call("fp8_linear", x, weight, bias, grad_dtype)
 
 
 def gelu(x, approximate="none"):
-    """GELU of x [..., features] like torch.nn.functional.gelu; what is kept for the backward pass is x in 8 bits."""
-    _check_input(x, "fp8.gelu")
-    return _apply(_Gelu, (x,), _tanh_form(approximate, "fp8.gelu"))
-
-
-class _Mlp(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w1, b1, w2, b2, tanh_form, grad_dtype):
-        need_x, need_w1, need_b1, need_w2, need_b2 = ctx.needs_input_grad[:5]
-        inner = need_x or need_w1 or need_b1            # whether the gradient goes back through the GELU
-        flat = _flat(x)
-        xa, xs, xt, xts, _ = _call("fp8_quantize", flat, E4M3, False, True, need_w1, None)
-        w1a, w1s, w1t, w1ts, _ = _call("fp8_quantize", w1, E4M3, True, True, need_x, None)
-        h = _product((xa, xs), (w1a, w1s), b1, x.dtype)
-        _, aa, as_, at, ats, hc, hcs = _call("fp8_gelu", h, tanh_form, False, True, need_w2, inner)
-        del h
-        w2a, w2s, w2t, w2ts, _ = _call("fp8_quantize", w2, E4M3, True, True, inner, None)
-        y = _product((aa, as_), (w2a, w2s), b2, x.dtype)
-        ctx.save_for_backward(xt, xts, w1t, w1ts, at, ats, hc, hcs, w2t, w2ts)
-        ctx.types = w1.dtype, None if b1 is None else b1.dtype, w2.dtype, None if b2 is None else b2.dtype, tanh_form, grad_dtype, x.shape, x.dtype
-        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], w2.shape[0])
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        xt, xts, w1t, w1ts, at, ats, hc, hcs, w2t, w2ts = ctx.saved_tensors
-        w1_dtype, b1_dtype, w2_dtype, b2_dtype, tanh_form, grad_dtype, shape, x_dtype = ctx.types
-        need_x, need_w1, need_b1, need_w2, need_b2 = ctx.needs_input_grad[:5]
-        inner = need_x or need_w1 or need_b1
-        ga, gs, gt, gts, db2 = _call("fp8_quantize", _flat(dy), grad_dtype, False, inner, need_w2 or need_b2, b2_dtype if need_b2 else None)
-        dw2 = _weight_grad((gt, gts), (at, ats), w2_dtype) if need_w2 else None
-        dx = dw1 = db1 = None
-        if inner:
-            da = _product((ga, gs), (w2t, w2ts), None, x_dtype)
-            _, ha, hs, ht, hts, db1 = _call("fp8_gelu_grad", da, hc, hcs, tanh_form, False, grad_dtype, need_x, need_w1 or need_b1, b1_dtype if need_b1 else None)
-            dx = _product((ha, hs), (w1t, w1ts), None, x_dtype).reshape(shape) if need_x else None
-            dw1 = _weight_grad((ht, hts), (xt, xts), w1_dtype) if need_w1 else None
-        return dx, dw1, db1, dw2, db2, None, None
+    """GELU of x [..., features] like torch.nn.functional.gelu, but 0 for -inf; what is kept for the backward pass is x in 8 bits, in blocks of 128
+    features."""
+    return _call("fp8_gelu8", x, _tanh_form(approximate, "fp8.gelu"))
 
 
 def mlp(x, w1, b1, w2, b2, approximate="none", grad_dtype=E4M3):
-    """linear(gelu(linear(x, w1, b1)), w2, b2) for x [..., in], w1 [hidden, in], w2 [out, hidden], differentiable in all five.
+    """linear(gelu(linear(x, w1, b1)), w2, b2) for x [..., in], w1 [hidden, in], w2 [out, hidden], differentiable once in all five.
 
     The GELU's result is rounded to 8 bits straight from 32 (there is no copy of it in the type of x), its gradient likewise.  Kept until the
     backward pass, all in 8 bits: the transposes of x, of the GELU's result and of the weights, and the GELU's input."""
-    _check_linear(x, w1, b1, "fp8.mlp")
-    if not isinstance(w2, torch.Tensor) or w2.dim() != 2 or w2.dtype not in _FLOATS or w2.device != x.device or w2.shape[1] != w1.shape[0] or w2.shape[1] < 1:
-        raise VenomError("fp8.mlp: the second weight must be a float16, bfloat16 or float32 matrix of %d columns on the input's device" % w1.shape[0])
-    if b2 is not None and (b2.shape != w2.shape[:1] or b2.dtype not in _FLOATS or b2.device != x.device):
-        raise VenomError("fp8.mlp: the second bias must be a vector of %d values on the input's device" % w2.shape[0])
-    _check_grad_dtype(grad_dtype, "fp8.mlp")
-    return _apply(_Mlp, (x, w1, b1, w2, b2), _tanh_form(approximate, "fp8.mlp"), grad_dtype)
+    return _call("fp8_mlp", x, w1, b1, w2, b2, _tanh_form(approximate, "fp8.mlp"), grad_dtype)
 
 
 class _Held(torch.nn.Module):
