@@ -12,6 +12,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 namespace vnm {
 
 namespace {
@@ -119,9 +121,10 @@ __device__ __forceinline__ void store8(void *y, int64_t at, int c, int cols, int
 
 // ---- scales ----
 // The scale's byte (its exponent + 127) for a block whose largest finite magnitude is amax.
-__device__ __forceinline__ uint32_t scale_code(float amax, int f8)
+template <int F8>
+__device__ __forceinline__ uint32_t scale_code(float amax)
 {
-    const int e = (int)((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - (f8 == F8_E4M3 ? 8 : 15);
+    const int e = (int)((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - (F8 == F8_E4M3 ? 8 : 15);
     return e > 0 ? (uint32_t)e : 0u;
 }
 __device__ __forceinline__ float inverse_scale(uint32_t code) { return __uint_as_float((254u - code) << 23); }
@@ -143,33 +146,35 @@ __device__ __forceinline__ float finite_amax8(const float (&v)[8])
 }
 
 // (a, b) / s in 8 bits, a in the low byte.
-__device__ __forceinline__ uint32_t round2(float a, float b, float inv, int f8)
+template <int F8>
+__device__ __forceinline__ uint32_t round2(float a, float b, float inv)
 {
-    const float2 v = make_float2(a * inv, b * inv);
-    if (f8 == F8_E4M3) return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
-    return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E5M2);
+    return __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, F8 == F8_E4M3 ? __NV_E4M3 : __NV_E5M2);
 }
-__device__ __forceinline__ uint2 round8(const float (&v)[8], float inv, int f8)
+template <int F8>
+__device__ __forceinline__ uint2 round8(const float (&v)[8], float inv)
 {
     uint2 r;
-    r.x = __byte_perm(round2(v[0], v[1], inv, f8), round2(v[2], v[3], inv, f8), 0x5410);
-    r.y = __byte_perm(round2(v[4], v[5], inv, f8), round2(v[6], v[7], inv, f8), 0x5410);
+    r.x = __byte_perm(round2<F8>(v[0], v[1], inv), round2<F8>(v[2], v[3], inv), 0x5410);
+    r.y = __byte_perm(round2<F8>(v[4], v[5], inv), round2<F8>(v[6], v[7], inv), 0x5410);
     return r;
 }
 // Four rounded values of a block with infinities, which the conversion has made the largest value: they stay infinities in e5m2 and become NaN in e4m3.
-__device__ __forceinline__ uint32_t mend4(uint32_t w, float a, float b, float c, float d, int f8)
+template <int F8>
+__device__ __forceinline__ uint32_t mend4(uint32_t w, float a, float b, float c, float d)
 {
     const float v[4] = {a, b, c, d};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint32_t bits = __float_as_uint(v[i]);
-        if ((bits & 0x7FFFFFFFu) == 0x7F800000u) w = (w & ~(0xFFu << (8 * i))) | ((((bits >> 24) & 0x80u) | (f8 == F8_E4M3 ? 0x7Fu : 0x7Cu)) << (8 * i));
+        if ((bits & 0x7FFFFFFFu) == 0x7F800000u) w = (w & ~(0xFFu << (8 * i))) | ((((bits >> 24) & 0x80u) | (F8 == F8_E4M3 ? 0x7Fu : 0x7Cu)) << (8 * i));
     }
     return w;
 }
-__device__ __forceinline__ uint2 mend8(uint2 r, const float (&v)[8], int f8)
+template <int F8>
+__device__ __forceinline__ uint2 mend8(uint2 r, const float (&v)[8])
 {
-    return make_uint2(mend4(r.x, v[0], v[1], v[2], v[3], f8), mend4(r.y, v[4], v[5], v[6], v[7], f8));
+    return make_uint2(mend4<F8>(r.x, v[0], v[1], v[2], v[3]), mend4<F8>(r.y, v[4], v[5], v[6], v[7]));
 }
 
 // Largest of sixteen lanes for four values at once: lanes exchange the values that they do not keep, so that five shuffles do, and each lane ends with
@@ -192,7 +197,8 @@ __device__ __forceinline__ uint32_t bytes_of4(uint32_t code)
     return w;
 }
 // Codes of four blocks of eight values a lane; bit i of *odd: block i has an infinity.
-__device__ __forceinline__ uint32_t codes_of4(const float (&v)[4][8], int f8, uint32_t *odd)
+template <int F8>
+__device__ __forceinline__ uint32_t codes_of4(const float (&v)[4][8], uint32_t *odd)
 {
     float m = max16_of4(amax8(v[0]), amax8(v[1]), amax8(v[2]), amax8(v[3]));
     *odd = 0;
@@ -200,7 +206,7 @@ __device__ __forceinline__ uint32_t codes_of4(const float (&v)[4][8], int f8, ui
         *odd = bytes_of4(finite(m) ? 0u : 1u);
         m = max16_of4(finite_amax8(v[0]), finite_amax8(v[1]), finite_amax8(v[2]), finite_amax8(v[3]));
     }
-    return bytes_of4(scale_code(m, f8));
+    return bytes_of4(scale_code<F8>(m));
 }
 __device__ __forceinline__ uint32_t byte_of(uint32_t w, int i) { return (w >> (8 * i)) & 0xFFu; }
 
@@ -260,16 +266,18 @@ __device__ __forceinline__ float min_nan(float a, float b)
 }
 // Beyond 64 either form is x or 0 and the derivative 1 or 0; the square of a far larger x would overflow beside a zero.  So -inf gives 0.
 __device__ __forceinline__ float near(float x) { return max_nan(min_nan(x, 64.0f), -64.0f); }
-__device__ __forceinline__ float gelu(float x, int tanh_form)
+template <bool TANH>
+__device__ __forceinline__ float gelu(float x)
 {
     float d;
-    if (tanh_form) return max_nan(x, -64.0f) * gelu_sigmoid(near(x), &d);
+    if (TANH) return max_nan(x, -64.0f) * gelu_sigmoid(near(x), &d);
     return fmaf(-min_nan(fabsf(x), 64.0f), half_erfc(x, &d), max_nan(x, 0.0f));
 }
-__device__ __forceinline__ float gelu_grad(float x, int tanh_form)
+template <bool TANH>
+__device__ __forceinline__ float gelu_grad(float x)
 {
     float d;
-    if (tanh_form) {
+    if (TANH) {
         x = near(x);
         const float s = gelu_sigmoid(x, &d);
         return fmaf(x * s * (1.0f - s), d, s);
@@ -297,7 +305,7 @@ __device__ __forceinline__ void ckpt_values(uint2 q, uint32_t code, float (&h)[8
 // are worked on.  Every value is read and written once; bound by HBM, and by launch and latency for few rows.
 constexpr int ROWS_THREADS = 256;
 
-template <int TYPE, int OP>
+template <int TYPE, int OP, int F8, bool TANH>
 __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN ? 2 : 3) fp8_rows_kernel(const Fp8QuantParams p)
 {
     grid_dependency_wait();
@@ -344,16 +352,17 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
         if (g >= groups) { g -= groups; row++; }
         fetch(u, row, g);
 
-        auto store = [&](uint8_t *data, int64_t ld, uint8_t *scales, int f8) {
+        auto store = [&](uint8_t *data, int64_t ld, uint8_t *scales, auto type) {
+            constexpr int T8 = decltype(type)::value;
             uint32_t odd;
-            const uint32_t codes = codes_of4(v, f8, &odd);
+            const uint32_t codes = codes_of4<T8>(v, &odd);
             if (on) {
                 uint8_t *dst = data + r * ld + c;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float inv = inverse_scale(byte_of(codes, i));
-                    uint2 q = round8(v[i], inv, f8);
-                    if (byte_of(odd, i)) q = mend8(q, v[i], f8);
+                    uint2 q = round8<T8>(v[i], inv);
+                    if (byte_of(odd, i)) q = mend8<T8>(q, v[i]);
                     if (c + 128 * i < p.cols) *reinterpret_cast<uint2 *>(dst + 128 * i) = q;
                 }
                 // blocks past the last one are zeros, whose code is 0
@@ -361,18 +370,18 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
             }
         };
         if constexpr (OP == FP8_GELU) {
-            if (p.ckpt) store(p.ckpt, p.ldc, p.ckpt_scales, F8_E4M3);
+            if (p.ckpt) store(p.ckpt, p.ldc, p.ckpt_scales, std::integral_constant<int, F8_E4M3>());
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[i][j] = gelu(v[i][j], p.tanh_form);
+                for (int j = 0; j < 8; j++) v[i][j] = gelu<TANH>(v[i][j]);
         } else if constexpr (OP == FP8_GELU_GRAD) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float x[8];
                 ckpt_values(h[i], byte_of(h_codes, i), x);
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[i][j] *= gelu_grad(x[j], p.tanh_form);
+                for (int j = 0; j < 8; j++) v[i][j] *= gelu_grad<TANH>(x[j]);
             }
         }
         if (OP != FP8_PLAIN && p.y && on) {
@@ -380,7 +389,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
             for (int i = 0; i < 4; i++)
                 if (c + 128 * i < p.cols) store8<TYPE>(p.y, r * p.ldy, c + 128 * i, p.cols, p.align_y, v[i]);
         }
-        if (p.data) store(p.data, p.ldd, p.scales, p.f8);
+        if (p.data) store(p.data, p.ldd, p.scales, std::integral_constant<int, F8>());
     }
 }
 
@@ -388,38 +397,42 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
 // A thread holds four rows x eight columns.  The transposed bytes pass through shared memory: column c's 32 words of four rows each, word w at
 // w ^ 2 (c / 8), so that the lanes of a warp (sixteen groups of eight columns, two of four rows) write to 32 banks, and read back whole columns.
 constexpr int TILE_THREADS = 512;
+constexpr int AMAX_PITCH = 136;    // four rows side by side lie in different banks
 
-template <int TYPE, int OP, bool SQUARE>
-__global__ void __launch_bounds__(TILE_THREADS, 2) fp8_tiles_kernel(const Fp8QuantParams p)
+struct TileShared {
+    uint32_t image[128 * 32];
+    float amax_of[32][AMAX_PITCH];   // of each four rows; later their sums
+    float inv_of[128];
+    float all[16];
+};
+
+// WHOLE: a tile of 128 x 128 values whose rows are 16-byte aligned; nothing is checked.
+template <int TYPE, int OP, int F8, bool SQUARE, bool TANH, bool WHOLE>
+__device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh, int tr, int tc)
 {
-    __shared__ uint32_t image[128 * 32];
-    __shared__ float amax_of[16][128];
-    __shared__ float inv_of[128];
-    __shared__ float all[16];
-    grid_dependency_wait();
-    grid_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = lane & 15, half = lane >> 4;
     const int cblocks = (int)(((int64_t)p.cols + 127) >> 7), rblocks = (int)(((int64_t)p.rows + 127) >> 7);
-    const int tr = (int)(blockIdx.x / (unsigned)cblocks), tc = (int)blockIdx.x - tr * cblocks;
     const int c = tc * 128 + group * 8;
     const int64_t r0 = (int64_t)tr * 128 + warp * 8 + half * 4;
-    const bool in = c < p.cols;
+    const bool in = WHOLE || c < p.cols;
+    const int left = WHOLE ? 4 : (int)(p.rows - r0 < 4 ? p.rows - r0 : 4);   // rows that there are, or fewer than one
     const int own_row = (lane >> 2) & 3;                       // the row whose code this lane stores (lanes 0, 4, 8, 12 of a half)
 
     float v[4][8];
     {
         Raw<TYPE> raw[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) raw[j] = load_raw<TYPE>(p.x, (r0 + j) * p.ldx, c, r0 + j < p.rows ? p.cols : 0, p.align_x);
+        for (int j = 0; j < 4; j++) raw[j] = load_raw<TYPE>(p.x, (r0 + j) * p.ldx, c, WHOLE ? c + 8 : j < left ? p.cols : 0, WHOLE ? 16 : p.align_x);
         uint2 q[4];
         uint32_t codes[4];
         if constexpr (OP == FP8_GELU_GRAD) {
+            const uint8_t *src = p.ckpt + r0 * p.ldc + c, *code = p.ckpt_scales + ((int64_t)(tc >> 2) * p.rows + r0) * 4 + (tc & 3);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const bool there = in && r0 + j < p.rows;
-                q[j] = there ? __ldg(reinterpret_cast<const uint2 *>(p.ckpt + (r0 + j) * p.ldc + c)) : make_uint2(0u, 0u);
-                codes[j] = there ? __ldg(p.ckpt_scales + ((int64_t)(tc >> 2) * p.rows + r0 + j) * 4 + (tc & 3)) : 0u;
+                const bool there = WHOLE || (in && j < left);
+                q[j] = there ? __ldg(reinterpret_cast<const uint2 *>(src + j * p.ldc)) : make_uint2(0u, 0u);
+                codes[j] = there ? __ldg(code + 4 * j) : 0u;
             }
         }
 #pragma unroll
@@ -429,91 +442,104 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) fp8_tiles_kernel(const Fp8Qua
                 float h[8];
                 ckpt_values(q[j], codes[j], h);
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[j][i] *= gelu_grad(h[i], p.tanh_form);
+                for (int i = 0; i < 8; i++) v[j][i] *= gelu_grad<TANH>(h[i]);
             }
         }
     }
-    auto store_rows = [&](uint8_t *data, int64_t ld, uint8_t *scales, int f8, uint32_t codes, uint32_t odd) {
+    auto store_rows = [&](uint8_t *data, int64_t ld, uint8_t *scales, auto type, uint32_t codes, uint32_t odd) {
+        constexpr int T8 = decltype(type)::value;
+        uint8_t *dst = data + r0 * ld + c;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const float inv = inverse_scale(byte_of(codes, j));
-            uint2 q = round8(v[j], inv, f8);
-            if (byte_of(odd, j)) q = mend8(q, v[j], f8);
-            if (in && r0 + j < p.rows) *reinterpret_cast<uint2 *>(data + (r0 + j) * ld + c) = q;
+            uint2 q = round8<T8>(v[j], inverse_scale(byte_of(codes, j)));
+            if (byte_of(odd, j)) q = mend8<T8>(q, v[j]);
+            if (in && (WHOLE || j < left)) *reinterpret_cast<uint2 *>(dst + j * ld) = q;
         }
-        if ((lane & 3) == 0 && r0 + own_row < p.rows) store_scale(scales, p.rows, r0 + own_row, tc, cblocks, byte_of(codes, own_row));
+        if ((lane & 3) == 0 && own_row < left) store_scale(scales, p.rows, r0 + own_row, tc, cblocks, byte_of(codes, own_row));
     };
     if constexpr (OP == FP8_GELU) {
         if (p.ckpt) {
             uint32_t odd;
-            const uint32_t codes = codes_of4(v, F8_E4M3, &odd);
-            store_rows(p.ckpt, p.ldc, p.ckpt_scales, F8_E4M3, codes, odd);
+            const uint32_t codes = codes_of4<F8_E4M3>(v, &odd);
+            store_rows(p.ckpt, p.ldc, p.ckpt_scales, std::integral_constant<int, F8_E4M3>(), codes, odd);
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[j][i] = gelu(v[j][i], p.tanh_form);   // of the zeros that pad: zero
+            for (int i = 0; i < 8; i++) v[j][i] = gelu<TANH>(v[j][i]);   // of the zeros that pad: zero
     }
 
     uint32_t tile_code = 0;
     bool tile_odd = false;
     if constexpr (SQUARE) {
-        float m = fmaxf(fmaxf(amax8(v[0]), amax8(v[1])), fmaxf(amax8(v[2]), amax8(v[3])));
-        m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));   // of values that are not negative: their bits' order
-        if (lane == 0) all[warp] = m;
-        __syncthreads();
-        m = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 16; w++) m = fmaxf(m, all[w]);
-        tile_odd = !finite(m);
-        if (tile_odd) {
-            m = fmaxf(fmaxf(finite_amax8(v[0]), finite_amax8(v[1])), fmaxf(finite_amax8(v[2]), finite_amax8(v[3])));
+        // values that are not negative are ordered like their bits
+        auto over_tile = [&](float m) {
             m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
-            __syncthreads();
-            if (lane == 0) all[warp] = m;
+            if (lane == 0) sh.all[warp] = m;
             __syncthreads();
             m = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 16; w++) m = fmaxf(m, all[w]);
+            for (int w = 0; w < 16; w++) m = fmaxf(m, sh.all[w]);
+            return m;
+        };
+        float m = over_tile(fmaxf(fmaxf(amax8(v[0]), amax8(v[1])), fmaxf(amax8(v[2]), amax8(v[3]))));
+        tile_odd = !finite(m);
+        if (tile_odd) {
+            __syncthreads();
+            m = over_tile(fmaxf(fmaxf(finite_amax8(v[0]), finite_amax8(v[1])), fmaxf(finite_amax8(v[2]), finite_amax8(v[3]))));
         }
-        tile_code = scale_code(m, p.f8);
+        tile_code = scale_code<F8>(m);
     }
 
     if (p.data) {
         uint32_t odd = tile_odd ? 0x01010101u : 0u, codes = tile_code * 0x01010101u;
-        if constexpr (!SQUARE) codes = codes_of4(v, p.f8, &odd);
-        store_rows(p.data, p.ldd, p.scales, p.f8, codes, odd);
+        if constexpr (!SQUARE) codes = codes_of4<F8>(v, &odd);
+        store_rows(p.data, p.ldd, p.scales, std::integral_constant<int, F8>(), codes, odd);
     }
 
+    // four threads a column: rows of sh.amax_of taken in turn
+    const int own_col = threadIdx.x >> 2, part = threadIdx.x & 3;
+    auto put8 = [&](const float (&m)[8]) {
+        float4 *at = reinterpret_cast<float4 *>(&sh.amax_of[warp * 2 + half][group * 8]);
+        at[0] = make_float4(m[0], m[1], m[2], m[3]);
+        at[1] = make_float4(m[4], m[5], m[6], m[7]);
+    };
     if (p.data_t) {
         float inv[8];
         if constexpr (!SQUARE) {
 #pragma unroll 1
             for (int pass = 0; pass < 2; pass++) {   // the second one only where a column has an infinity
-                if (pass == 1 && !__syncthreads_or(threadIdx.x < 128 && inv_of[threadIdx.x & 127] < 0.0f)) break;
+                if (pass == 1 && !__syncthreads_or(sh.inv_of[own_col] < 0.0f)) break;
+                float m[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    float m = 0.0f;
+                    if (pass == 0) {
+                        m[i] = fmaxf(fmaxf(fabsf(v[0][i]), fabsf(v[1][i])), fmaxf(fabsf(v[2][i]), fabsf(v[3][i])));
+                    } else {
+                        m[i] = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) m = pass && !finite(v[j][i]) ? m : fmaxf(m, fabsf(v[j][i]));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    if (half == 0) amax_of[warp][group * 8 + i] = m;
+                        for (int j = 0; j < 4; j++) m[i] = finite(v[j][i]) ? fmaxf(m[i], fabsf(v[j][i])) : m[i];
+                    }
                 }
+                put8(m);
                 __syncthreads();
-                if (threadIdx.x < 128) {
-                    float m = 0.0f;
+                float a = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < 16; w++) m = fmaxf(m, amax_of[w][threadIdx.x]);
-                    const bool odd = pass == 0 ? !finite(m) : inv_of[threadIdx.x] < 0.0f;
-                    const uint32_t code = scale_code(finite(m) ? m : 0.0f, p.f8);
-                    inv_of[threadIdx.x] = odd ? -inverse_scale(code) : inverse_scale(code);   // the sign says that it has one
-                    const int col = tc * 128 + (int)threadIdx.x;
-                    if (col < p.cols) store_scale(p.scales_t, p.cols, col, tr, rblocks, code);
+                for (int k = 0; k < 8; k++) a = fmaxf(a, sh.amax_of[4 * k + part][own_col]);
+                a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+                a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+                if (part == 0) {
+                    const bool odd = pass == 0 ? !finite(a) : sh.inv_of[own_col] < 0.0f;
+                    const uint32_t code = scale_code<F8>(finite(a) ? a : 0.0f);
+                    sh.inv_of[own_col] = odd ? -inverse_scale(code) : inverse_scale(code);   // the sign says that it has one
+                    const int col = tc * 128 + own_col;
+                    if (WHOLE || col < p.cols) store_scale(p.scales_t, p.cols, col, tr, rblocks, code);
                 }
                 __syncthreads();
             }
-#pragma unroll
-            for (int i = 0; i < 8; i++) inv[i] = inv_of[group * 8 + i];
+            const float4 lo = *reinterpret_cast<const float4 *>(&sh.inv_of[group * 8]), hi = *reinterpret_cast<const float4 *>(&sh.inv_of[group * 8 + 4]);
+            inv[0] = lo.x; inv[1] = lo.y; inv[2] = lo.z; inv[3] = lo.w;
+            inv[4] = hi.x; inv[5] = hi.y; inv[6] = hi.z; inv[7] = hi.w;
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) inv[i] = tile_odd ? -inverse_scale(tile_code) : inverse_scale(tile_code);
@@ -522,39 +548,50 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) fp8_tiles_kernel(const Fp8Qua
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const float a = fabsf(inv[i]);
-            uint32_t w = __byte_perm(round2(v[0][i], v[1][i], a, p.f8), round2(v[2][i], v[3][i], a, p.f8), 0x5410);
-            if (inv[i] < 0.0f) w = mend4(w, v[0][i], v[1][i], v[2][i], v[3][i], p.f8);
-            image[(group * 8 + i) * 32 + ((warp * 2 + half) ^ (2 * group))] = w;
+            uint32_t w = __byte_perm(round2<F8>(v[0][i], v[1][i], a), round2<F8>(v[2][i], v[3][i], a), 0x5410);
+            if (inv[i] < 0.0f) w = mend4<F8>(w, v[0][i], v[1][i], v[2][i], v[3][i]);
+            sh.image[(group * 8 + i) * 32 + ((warp * 2 + half) ^ (2 * group))] = w;
         }
         __syncthreads();
+        // sixteen lanes a column: eight rows each
         const int64_t padded = ((int64_t)p.rows + 15) & ~(int64_t)15;
+        const int piece = lane & 15, col0 = threadIdx.x >> 4;
+        const int64_t row = (int64_t)tr * 128 + piece * 8;
+        uint8_t *dst = p.data_t + ((int64_t)tc * 128 + col0) * p.ldt + row;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const int e = k * TILE_THREADS + threadIdx.x;
-            const int col = e >> 4, piece = e & 15;
-            const uint2 q = *reinterpret_cast<const uint2 *>(&image[col * 32 + 2 * (piece ^ (col >> 3))]);
-            const int64_t row = (int64_t)tr * 128 + piece * 8;
-            if (tc * 128 + col < p.cols && row < padded) *reinterpret_cast<uint2 *>(p.data_t + (int64_t)(tc * 128 + col) * p.ldt + row) = q;
+            const int col = col0 + 32 * k;
+            const uint2 q = *reinterpret_cast<const uint2 *>(&sh.image[col * 32 + 2 * (piece ^ (col >> 3))]);
+            if (WHOLE || (tc * 128 + col < p.cols && row < padded)) *reinterpret_cast<uint2 *>(dst + (int64_t)(32 * k) * p.ldt) = q;
         }
     }
 
-    if (p.partial) {
-        __syncthreads();   // amax_of is read no more
+    if (p.partial) {                       // amax_of has been read by all: the image is complete
+        float s[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            float s = (v[0][i] + v[1][i]) + (v[2][i] + v[3][i]);
-            s += __shfl_xor_sync(0xffffffffu, s, 16);
-            if (half == 0) amax_of[warp][group * 8 + i] = s;
-        }
+        for (int i = 0; i < 8; i++) s[i] = (v[0][i] + v[1][i]) + (v[2][i] + v[3][i]);
+        put8(s);
         __syncthreads();
-        const int col = tc * 128 + (int)threadIdx.x;
-        if (threadIdx.x < 128 && col < p.cols) {
-            float s = 0.0f;
+        float a = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 16; w++) s += amax_of[w][threadIdx.x];
-            p.partial[(int64_t)tr * p.cols + col] = s;
-        }
+        for (int k = 0; k < 8; k++) a += sh.amax_of[4 * k + part][own_col];
+        a += __shfl_xor_sync(0xffffffffu, a, 1);
+        a += __shfl_xor_sync(0xffffffffu, a, 2);
+        const int col = tc * 128 + own_col;
+        if (part == 0 && (WHOLE || col < p.cols)) p.partial[(int64_t)tr * p.cols + col] = a;
     }
+}
+
+template <int TYPE, int OP, int F8, bool SQUARE, bool TANH>
+__global__ void __launch_bounds__(TILE_THREADS, 2) fp8_tiles_kernel(const Fp8QuantParams p)
+{
+    __shared__ TileShared sh;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int cblocks = (int)(((int64_t)p.cols + 127) >> 7);
+    const int tr = (int)(blockIdx.x / (unsigned)cblocks), tc = (int)blockIdx.x - tr * cblocks;
+    if (p.align_x == 16 && (int64_t)tr * 128 + 128 <= p.rows && (int64_t)tc * 128 + 128 <= p.cols) fp8_tile<TYPE, OP, F8, SQUARE, TANH, true>(p, sh, tr, tc);
+    else fp8_tile<TYPE, OP, F8, SQUARE, TANH, false>(p, sh, tr, tc);
 }
 
 // Sums of the blocks' partial sums, always in the same order: eight threads a column, each every eighth block.
@@ -628,19 +665,29 @@ cudaError_t rows_of(const Fp8QuantParams &p, int op, cudaStream_t stream)
     const int64_t wave = (int64_t)device_sms() * (TYPE == T_F32 || op != FP8_PLAIN ? 2 : 3);
     const int64_t ctas = (units + per_cta - 1) / per_cta < wave ? (units + per_cta - 1) / per_cta : wave;
     const dim3 grid((unsigned)ctas);
-    if (op == FP8_PLAIN) return launch(fp8_rows_kernel<TYPE, FP8_PLAIN>, grid, ROWS_THREADS, stream, p);
-    if (op == FP8_GELU) return launch(fp8_rows_kernel<TYPE, FP8_GELU>, grid, ROWS_THREADS, stream, p);
-    return launch(fp8_rows_kernel<TYPE, FP8_GELU_GRAD>, grid, ROWS_THREADS, stream, p);
+    const bool e4 = p.f8 == F8_E4M3;
+#define VNM_ROWS(OP, F8, TANH) launch(fp8_rows_kernel<TYPE, OP, F8, TANH>, grid, ROWS_THREADS, stream, p)
+    if (op == FP8_PLAIN) return e4 ? VNM_ROWS(FP8_PLAIN, F8_E4M3, false) : VNM_ROWS(FP8_PLAIN, F8_E5M2, false);
+    if (op == FP8_GELU) return p.tanh_form ? VNM_ROWS(FP8_GELU, F8_E4M3, true) : VNM_ROWS(FP8_GELU, F8_E4M3, false);
+    if (e4) return p.tanh_form ? VNM_ROWS(FP8_GELU_GRAD, F8_E4M3, true) : VNM_ROWS(FP8_GELU_GRAD, F8_E4M3, false);
+    return p.tanh_form ? VNM_ROWS(FP8_GELU_GRAD, F8_E5M2, true) : VNM_ROWS(FP8_GELU_GRAD, F8_E5M2, false);
+#undef VNM_ROWS
 }
 
 template <int TYPE>
 cudaError_t tiles_of(const Fp8QuantParams &p, int op, bool square, cudaStream_t stream)
 {
     const dim3 grid((unsigned)((((int64_t)p.cols + 127) / 128) * (((int64_t)p.rows + 127) / 128)));
-    if (op == FP8_GELU) return launch(fp8_tiles_kernel<TYPE, FP8_GELU, false>, grid, TILE_THREADS, stream, p);
-    if (op == FP8_GELU_GRAD) return launch(fp8_tiles_kernel<TYPE, FP8_GELU_GRAD, false>, grid, TILE_THREADS, stream, p);
-    if (square) return launch(fp8_tiles_kernel<TYPE, FP8_PLAIN, true>, grid, TILE_THREADS, stream, p);
-    return launch(fp8_tiles_kernel<TYPE, FP8_PLAIN, false>, grid, TILE_THREADS, stream, p);
+    const bool e4 = p.f8 == F8_E4M3;
+#define VNM_TILES(OP, F8, SQUARE, TANH) launch(fp8_tiles_kernel<TYPE, OP, F8, SQUARE, TANH>, grid, TILE_THREADS, stream, p)
+    if (op == FP8_GELU) return p.tanh_form ? VNM_TILES(FP8_GELU, F8_E4M3, false, true) : VNM_TILES(FP8_GELU, F8_E4M3, false, false);
+    if (op == FP8_GELU_GRAD) {
+        if (e4) return p.tanh_form ? VNM_TILES(FP8_GELU_GRAD, F8_E4M3, false, true) : VNM_TILES(FP8_GELU_GRAD, F8_E4M3, false, false);
+        return p.tanh_form ? VNM_TILES(FP8_GELU_GRAD, F8_E5M2, false, true) : VNM_TILES(FP8_GELU_GRAD, F8_E5M2, false, false);
+    }
+    if (square) return e4 ? VNM_TILES(FP8_PLAIN, F8_E4M3, true, false) : VNM_TILES(FP8_PLAIN, F8_E5M2, true, false);
+    return e4 ? VNM_TILES(FP8_PLAIN, F8_E4M3, false, false) : VNM_TILES(FP8_PLAIN, F8_E5M2, false, false);
+#undef VNM_TILES
 }
 
 }  // namespace
