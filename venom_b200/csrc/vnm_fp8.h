@@ -41,6 +41,44 @@ cudaError_t launch_fp8_tiles(const Fp8QuantParams &p, int type, int op, bool squ
 cudaError_t launch_fp8_colsum(const float *partial, int blocks, int cols, void *out, int type, cudaStream_t stream);
 cudaError_t launch_fp8_dequantize(const uint8_t *data, int64_t ldd, const uint8_t *scales, int f8, int rows, int cols, void *out, int type, int64_t ldo, cudaStream_t stream);
 
+// n / d of 0 <= n < 2^31 by a multiplication: with 2^(s - 1) < d <= 2^s and m = floor(2^(31 + s) / d) + 1, m d - 2^(31 + s) is at most 2^s, so that
+// floor(n m / 2^(31 + s)) is the quotient (Granlund and Montgomery, 1994).
+struct FastDiv {
+    uint32_t d, m;
+    int s;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t divisor) : d(divisor), s(0)
+    {
+        while ((1ull << s) < d) s++;
+        m = (uint32_t)((1ull << (31 + s)) / d + 1);
+    }
+    __host__ __device__ uint32_t quotient(uint32_t n) const { return (uint32_t)(((uint64_t)n * m) >> (31 + s)); }
+};
+// The order of tile_coords() with its divisions prepared: a tile's place is on the way of every role of a kernel with short tiles (two divisions
+// took 600 of 5000 clocks a tile).
+struct TileOrder {
+    FastDiv band, full, last;   // tiles of a band, lines of a band and of the last one
+    int lines, other, rows;     // lines banded (row or column tiles), the other count, whether lines are row tiles
+    TileOrder() = default;
+    TileOrder(int mt, int nt, int group) : rows(group >= 0)
+    {
+        const int g = group >= 0 ? group : -group;
+        lines = rows ? mt : nt;
+        other = rows ? nt : mt;
+        band = FastDiv((uint32_t)g * (uint32_t)other);
+        full = FastDiv((uint32_t)g);
+        last = FastDiv((uint32_t)(lines % g ? lines % g : g));
+    }
+    __host__ __device__ void at(int tile, int *tm, int *tn) const
+    {
+        const uint32_t b = band.quotient((uint32_t)tile), within = (uint32_t)tile - b * band.d, first = b * full.d;
+        const FastDiv size = first + full.d <= (uint32_t)lines ? full : last;
+        const uint32_t across = size.quotient(within), line = first + within - across * size.d;
+        *tm = (int)(rows ? line : across);
+        *tn = (int)(rows ? across : line);
+    }
+};
+
 // out[m, n] = sum over k of A[m, k] B[n, k] (+ bias[n]), A [M, K] and B [N, K] in 8 bits with a scale for each 128 k of a row.
 struct Fp8MatmulParams {
     const uint32_t *sa, *sb;  // scale words [groups][M] and [groups][N]: byte j of word (g, r) is block 4 g + j of row r
@@ -49,10 +87,11 @@ struct Fp8MatmulParams {
     int64_t ldo;
     int M, N, K, ktiles;
     int out_type, bias_type;
+    int whole_pieces;         // pair kernel: rows of the result lie on 16-byte boundaries and are a multiple of 16 bytes long
     int a_f8, b_f8;
     int mt, nt;               // tiles along M and N
     int split;                // CTAs of a cluster that share one tile's k
-    int band;                 // pair kernel: order of the tiles (tile_coords)
+    TileOrder order;          // pair kernel
     int *status;
 };
 

@@ -122,7 +122,7 @@ CUresult encode_operand(EncodeTiledFn enc, CUtensorMap *map, const void *data, i
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
-// Band of the tile order of the pair kernel (tile_coords).  A band's operand stays in L2 while the other one streams past: row bands read A once and B once per
+// Band of the tile order of the pair kernel.  A band's operand stays in L2 while the other one streams past: row bands read A once and B once per
 // band, column bands the other way round.
 int tile_band(int M, int N, int K, int mt, int nt, int bn)
 {
@@ -255,6 +255,7 @@ extern "C" int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, 
     p.sa = static_cast<const uint32_t *>(a_scales); p.sb = static_cast<const uint32_t *>(b_scales);
     p.bias = bias; p.bias_type = bias_type;
     p.out = out; p.out_type = out_type; p.ldo = ldo;
+    p.whole_pieces = aligned(out, 16) && ldo * elem_size(out_type) % 16 == 0 && (int64_t)N * elem_size(out_type) % 16 == 0;
     p.M = M; p.N = N; p.K = K; p.ktiles = (K + 127) / 128;
     p.a_f8 = a_type; p.b_f8 = b_type;
     p.status = status;
@@ -270,7 +271,7 @@ extern "C" int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, 
     if (on_pairs) {
         p.mt = (M + 255) / 256;
         p.nt = (N + plan.bn - 1) / plan.bn;
-        p.band = tile_band(M, N, K, p.mt, p.nt, plan.bn);
+        p.order = TileOrder(p.mt, p.nt, tile_band(M, N, K, p.mt, p.nt, plan.bn));
         return done(launch_fp8_pair(plan, map_a, map_b, p, s), name);
     }
     p.mt = (M + plan.bn - 1) / plan.bn;

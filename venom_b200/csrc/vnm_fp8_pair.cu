@@ -25,7 +25,9 @@ constexpr int SCALE_WARP0 = 4, EPI_WARP0 = 8;
 constexpr int TMEM_COLS = 512;
 constexpr int SF_SETS = 2;
 
-template <int BN>
+constexpr int WINDOW = 11;       // epilogue: 16-byte pieces between the rows of a window (ten are used): an odd number, so that eight rows lie in different banks
+
+template <int BN, bool WHOLE>
 struct Fp8Pair {
     static_assert(BN % 16 == 0 && BN <= 256 && BN > 128, "accumulator columns");
     static constexpr bool ONE = BN > 240;                // one accumulator
@@ -33,14 +35,16 @@ struct Fp8Pair {
     static constexpr int B_BYTES = HALF_N * 128;
     static constexpr int B_SLOT = (B_BYTES + 1023) / 1024 * 1024;
     static constexpr int STAGE_BYTES = A_BYTES + B_SLOT;
-    static constexpr int STAGES = 7;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 512 + 1024;
+    static constexpr int WARP_BYTES = (WHOLE ? 4096 : 32 * WINDOW * 16) + 640;   // an epilogue warp's 32 rows, and the bias of its columns and 32 before
+    static constexpr int OUT_BYTES = 8 * WARP_BYTES;
+    static constexpr int STAGES = (227 * 1024 - OUT_BYTES - 512 - 1024) / STAGE_BYTES;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 512 + 1024;
     static_assert(SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
     static_assert((2 * STAGES + 2 * SF_SETS + 4) * 8 + 8 <= 512, "barriers");
 };
 __device__ __forceinline__ uint32_t acc_col(int a) { return (uint32_t)a * 256u; }
 template <int BN>
-__device__ __forceinline__ uint32_t sf_col(int set) { return Fp8Pair<BN>::ONE ? 256u + 16u * (uint32_t)set : 240u + 256u * (uint32_t)set; }
+__device__ __forceinline__ uint32_t sf_col(int set) { return Fp8Pair<BN, true>::ONE ? 256u + 16u * (uint32_t)set : 240u + 256u * (uint32_t)set; }
 
 __device__ __forceinline__ uint32_t cluster_ctarank()
 {
@@ -90,30 +94,14 @@ __device__ __forceinline__ void tc_mma2_mxf8(uint32_t d_tmem, uint64_t adesc, ui
         : "memory");
 }
 
-// ---- epilogue of one warp: 32 accumulator lanes (rows of the result) x up to 128 columns, straight from tensor memory ----
-// Read in fragment order: thread t holds columns 2 (t % 4), + 1 of every eight for lanes t / 4 and t / 4 + 8 of a 16-lane group.  Two 4 x 4 exchanges inside a
-// quad give each thread 16 neighbouring columns of a row in 16 bits, so that a store instruction writes 128 contiguous bytes of eight rows; 32-bit
-// results leave as pairs, a sector a quad.
-__device__ __forceinline__ void quad_swap(uint32_t &a, uint32_t &b, bool up, int mask)
-{
-    const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? a : b, mask);
-    if (up) a = got; else b = got;
-}
-__device__ __forceinline__ float2 bias_pair(const void *bias, int type, int n, int N)
-{
-    float2 r;
-    if (type == T_F32) {
-        const float *b = reinterpret_cast<const float *>(bias);
-        r.x = n < N ? __ldg(b + n) : 0.0f;
-        r.y = n + 1 < N ? __ldg(b + n + 1) : 0.0f;
-    } else {
-        const unsigned short *b = reinterpret_cast<const unsigned short *>(bias);
-        const unsigned short x = n < N ? __ldg(b + n) : (unsigned short)0, y = n + 1 < N ? __ldg(b + n + 1) : (unsigned short)0;
-        if (type == T_F16) r = make_float2(__half2float(__ushort_as_half(x)), __half2float(__ushort_as_half(y)));
-        else r = make_float2(__uint_as_float((uint32_t)x << 16), __uint_as_float((uint32_t)y << 16));
-    }
-    return r;
-}
+// ---- epilogue of one warp: 32 accumulator lanes (rows of the result), `cols` columns from n0 on ----
+// 128 bytes of each row at a time pass through shared memory and leave in pieces of 16 bytes, eight lanes a row.  Exchanging words between lanes instead, so
+// that nothing passes through shared memory, needs 2.4 times the instructions, and the epilogue's eight warps are what short tiles wait for: 16384 x 4096 x
+// 1024 with a bias 83 us.
+// Rows that begin anywhere (odd numbers of columns) leave in the same pieces, aligned where they go and not where they come from: a piece is cut out of two in
+// shared memory.  A row's window there is 32 bytes of the columns before and 128 new ones, so that a sector between two steps is written once and whole;
+// what costs is sectors written in parts (11844 x 15043, K = 116, bf16: 348 us with words of 4 bytes a lane and single values at the edges of each 128 bytes),
+// and only a tile's edges are.
 template <int TYPE>
 __device__ __forceinline__ uint32_t pack16(float a, float b)
 {
@@ -125,108 +113,180 @@ __device__ __forceinline__ uint32_t pack16(float a, float b)
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 }
-
-template <int TYPE, int COLS, typename Release>
-__device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n0, const Fp8MatmulParams &p, Release release)
+__device__ __forceinline__ uint32_t bias_bits(const void *bias, int type, int n)
 {
-    const int lane = threadIdx.x & 31, quad = lane & 3, w = lane >> 2;
-    const bool odd = (lane & 1) != 0, upper = (lane & 2) != 0;
-    const int64_t size = TYPE == T_F32 ? 4 : 2;
-    const uintptr_t base = reinterpret_cast<uintptr_t>(p.out);
-    const bool wide = ((base | (uintptr_t)(p.ldo * size)) & 31) == 0, half_wide = ((base | (uintptr_t)(p.ldo * size)) & 15) == 0, pairs = ((base | (uintptr_t)(p.ldo * size)) & (2 * size - 1)) == 0;
-    constexpr int CHUNKS = (COLS + 63) / 64;
+    return type == T_F32 ? __ldg(reinterpret_cast<const uint32_t *>(bias) + n) : (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(bias) + n);
+}
+__device__ __forceinline__ float bias_float(uint32_t bits, int type)
+{
+    return type == T_F32 ? __uint_as_float(bits) : type == T_F16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
+}
+
+// (a, b) += (x, y), both rounded to nearest
+__device__ __forceinline__ void add2(uint32_t &a, uint32_t &b, float x, float y)
+{
+    asm("{\n\t.reg .b64 p, q;\n\t"
+        "mov.b64 p, {%0, %1};\n\t"
+        "mov.b64 q, {%2, %3};\n\t"
+        "add.rn.f32x2 p, p, q;\n\t"
+        "mov.b64 {%0, %1}, p;\n\t}"
+        : "+r"(a), "+r"(b)
+        : "f"(x), "f"(y));
+}
+// What a load of tensor memory has brought is used behind its wait only.
+__device__ __forceinline__ void wait_for(uint32_t (&v)[32])
+{
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; i++) asm volatile("" : "+r"(v[i]));
+}
+
+// 32 columns from `v` on, rounded and packed.
+template <int TYPE, bool BIAS>
+__device__ __forceinline__ void round32(uint32_t (&v)[32], const float4 *bias, uint32_t (&word)[TYPE == T_F32 ? 32 : 16])
+{
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if constexpr (BIAS) {
+            const float4 b = bias[i];
+            add2(v[4 * i], v[4 * i + 1], b.x, b.y);
+            add2(v[4 * i + 2], v[4 * i + 3], b.z, b.w);
+        }
+        if constexpr (TYPE == T_F32) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) word[4 * i + k] = v[4 * i + k];
+        } else {
+            word[2 * i] = pack16<TYPE>(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]));
+            word[2 * i + 1] = pack16<TYPE>(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+        }
+    }
+}
+
+// Bytes [from, to) of a 16-byte piece at `dst`, both even: at most six stores, for the edges of a tile.
+__device__ __forceinline__ void store_part(uint8_t *dst, const uint32_t (&y)[4], int from, int to)
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const bool lo = from <= 4 * i && to >= 4 * i + 2, hi = from <= 4 * i + 2 && to >= 4 * i + 4;
+        if (lo && hi) *reinterpret_cast<uint32_t *>(dst + 4 * i) = y[i];
+        else if (lo) *reinterpret_cast<uint16_t *>(dst + 4 * i) = (uint16_t)y[i];
+        else if (hi) *reinterpret_cast<uint16_t *>(dst + 4 * i + 2) = (uint16_t)(y[i] >> 16);
+    }
+}
+
+// `part`: 0 the first 128 columns of a tile, 1 the rest; WHOLE: rows lie on 16-byte boundaries and have whole pieces.
+template <int TYPE, bool BIAS, bool WHOLE, typename Release>
+__device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n0, int cols, int part, uint4 *stage, const float4 *bias, const Fp8MatmulParams &p, Release release)
+{
+    constexpr int SIZE = TYPE == T_F32 ? 4 : 2, WIDTH = 128 / SIZE, PIECES = TYPE == T_F32 ? 8 : 4;   // pieces of 32 columns
+    const int lane = threadIdx.x & 31;
+    const int64_t pitch = p.ldo * SIZE;
+    uint8_t *out = reinterpret_cast<uint8_t *>(p.out) + row0 * pitch + (int64_t)n0 * SIZE;
+    const int rows = p.M - row0 < 32 ? (int)(p.M - row0) : 32;     // that there are; may be none
+    const int bytes = (p.N - n0 < cols ? p.N - n0 : cols) * SIZE;   // of a row to store; may be none
+    uint4 *const mine = stage + lane * (WHOLE ? 8 : WINDOW);
+    uint32_t before[8];                                            // !WHOLE: the 32 bytes ahead of these columns
+    if constexpr (!WHOLE) {
+        if (part == 1) {                                           // the first part leaves the sector between the two to this one
+            uint32_t u[32];
+            tc_ld_32x32b_x32(tacc - 32u, u);
+            wait_for(u);
+            uint32_t w[TYPE == T_F32 ? 32 : 16];
+            round32<TYPE, BIAS>(u, bias - 8, w);
+#pragma unroll
+            for (int i = 0; i < 8; i++) before[i] = w[(TYPE == T_F32 ? 24 : 8) + i];
+        }
+    }
+    uint32_t v[32];
+    tc_ld_32x32b_x32(tacc, v);
 #pragma unroll 1
-    for (int k = 0; k < CHUNKS; k++) {
-        const int cols = COLS - 64 * k;                     // a last chunk of fewer reads on into columns that it does not store
-        const int c0 = n0 + 64 * k;
+    for (int c0 = 0; c0 < cols; c0 += WIDTH, out += 128) {
+        // 32 columns at a time, the next ones on their way while these are rounded
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
-            uint32_t v[32];
-            tc_ld_16x256b(tacc + ((uint32_t)(16 * g) << 16) + (uint32_t)(64 * k), v);
-            tc_wait_ld();
-            if (k == CHUNKS - 1 && g == 1) release();
-            if (p.bias) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float2 b = bias_pair(p.bias, p.bias_type, c0 + 8 * j + 2 * quad, p.N);
-                    v[4 * j] = __float_as_uint(__uint_as_float(v[4 * j]) + b.x);
-                    v[4 * j + 1] = __float_as_uint(__uint_as_float(v[4 * j + 1]) + b.y);
-                    v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + b.x);
-                    v[4 * j + 3] = __float_as_uint(__uint_as_float(v[4 * j + 3]) + b.y);
+        for (int h = 0; h < WIDTH / 32; h++) {
+            wait_for(v);
+            uint32_t word[TYPE == T_F32 ? 32 : 16];
+            round32<TYPE, BIAS>(v, bias + c0 / 4 + 8 * h, word);
+            const int c1 = c0 + 32 * (h + 1);
+            if (c1 < cols) tc_ld_32x32b_x32(tacc + (uint32_t)c1, v);
+            else if (c1 - 32 < cols) release();                    // once: behind the last columns that belong to the tile
+            if (h == 0) {
+                __syncwarp();                                      // the columns before have been read
+                if constexpr (!WHOLE) {
+                    mine[0] = make_uint4(before[0], before[1], before[2], before[3]);
+                    mine[1] = make_uint4(before[4], before[5], before[6], before[7]);
                 }
             }
-            if constexpr (TYPE == T_F32) {
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const int64_t row = row0 + 16 * g + 8 * r + w;
-                    float *dst = reinterpret_cast<float *>(p.out) + row * p.ldo;
-                    if (row < p.M) {
+            for (int i = 0; i < PIECES; i++) {
+                const uint4 q = make_uint4(word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
+                if constexpr (WHOLE) mine[(PIECES * h + i) ^ (lane & 7)] = q;
+                else mine[2 + PIECES * h + i] = q;
+            }
+            if constexpr (!WHOLE) {
+                if (h == WIDTH / 32 - 1) {
 #pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const int n = c0 + 8 * j + 2 * quad;
-                            const float x = __uint_as_float(v[4 * j + 2 * r]), y = __uint_as_float(v[4 * j + 2 * r + 1]);
-                            if (8 * j >= cols) break;
-                            if (pairs && n + 1 < p.N) {
-                                *reinterpret_cast<float2 *>(dst + n) = make_float2(x, y);
-                            } else {
-                                if (n < p.N) dst[n] = x;
-                                if (n + 1 < p.N) dst[n + 1] = y;
-                            }
-                        }
-                    }
+                    for (int i = 0; i < 8; i++) before[i] = word[(TYPE == T_F32 ? 24 : 8) + i];
                 }
-            } else {
+            }
+        }
+        __syncwarp();
+        const int left = bytes - c0 * SIZE;                         // bytes of a row from here on
+        const int piece = lane & 7, first = lane >> 3;
+        if constexpr (WHOLE) {
+            uint8_t *dst = out + first * pitch + piece * 16;
+            const bool on = piece * 16 < left;
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    uint32_t x[8];
+            for (int i = 0; i < 8; i++, dst += 4 * pitch) {
+                const int r = 4 * i + first;
+                const uint4 q = stage[r * 8 + (piece ^ (r & 7))];
+                if (on && r < rows) *reinterpret_cast<uint4 *>(dst) = q;
+            }
+        } else if (left > 0) {
+            // piece q of row r, counted from the sector that these columns begin in
+            auto put = [&](int r, int q) {
+                uint8_t *row = out + r * pitch;
+                const int s = (int)(reinterpret_cast<uintptr_t>(row) & 31);
+                const int at = 32 + 16 * q - s, b = at & 15;        // where it begins in the window
+                const uint4 *w = stage + r * WINDOW + (at >> 4);
+                const uint4 lo = w[0], hi = w[1];
+                uint32_t x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] = pack16<TYPE>(__uint_as_float(v[4 * j + 2 * r]), __uint_as_float(v[4 * j + 2 * r + 1]));
+                for (int i = 0; i < 6; i++) x[i] = b & 8 ? x[i + 2] : x[i];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        quad_swap(x[0 + h], x[2 + h], odd, 1);
-                        quad_swap(x[4 + h], x[6 + h], odd, 1);
-                        quad_swap(x[0 + h], x[4 + h], upper, 2);
-                        quad_swap(x[2 + h], x[6 + h], upper, 2);
-                    }
-                    const uint32_t o[8] = {x[0], x[2], x[4], x[6], x[1], x[3], x[5], x[7]};
-                    const int64_t row = row0 + 16 * g + 8 * r + w;
-                    const int n = c0 + 16 * quad, rest = p.N - n;
-                    if (row >= p.M || rest <= 0 || 16 * quad >= cols) continue;
-                    uint16_t *dst = reinterpret_cast<uint16_t *>(p.out) + row * p.ldo + n;
-                    if (wide && rest >= 16) {
-                        st_global_v8(dst, o);
-                    } else if (half_wide && rest >= 16) {
-                        *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-                        *reinterpret_cast<uint4 *>(dst + 8) = make_uint4(o[4], o[5], o[6], o[7]);
-                    } else if (pairs) {
+                for (int i = 0; i < 5; i++) x[i] = b & 4 ? x[i + 1] : x[i];
+                uint32_t y[4];
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            if (2 * i + 1 < rest) *reinterpret_cast<uint32_t *>(dst + 2 * i) = o[i];
-                            else if (2 * i < rest) dst[2 * i] = (uint16_t)o[i];
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            if (2 * i < rest) dst[2 * i] = (uint16_t)o[i];
-                            if (2 * i + 1 < rest) dst[2 * i + 1] = (uint16_t)(o[i] >> 16);
-                        }
-                    }
+                for (int i = 0; i < 4; i++) y[i] = __byte_perm(x[i], x[i + 1], b & 2 ? 0x5432 : 0x3210);
+                const int end = s + left - 16 * q;                  // of the row, from this piece on
+                const int begin = c0 == 0 && part == 0 ? s - 16 * q : 0;
+                if (r < rows && end > 0 && begin < 16) {
+                    if (begin <= 0 && end >= 16) *reinterpret_cast<uint4 *>(row - s + 16 * q) = make_uint4(y[0], y[1], y[2], y[3]);
+                    else store_part(row - s + 16 * q, y, begin, end);
                 }
+            };
+            // the sector that ends with these columns or behind them is left to the next ones, or to the other part
+            const bool last = left <= 128 && !(part == 0 && p.N - n0 > 128);
+#pragma unroll 2
+            for (int i = 0; i < 8; i++) put(4 * i + first, piece);
+            if (last) {
+#pragma unroll 1
+                for (int i = 0; i < 2; i++) put(16 * i + (lane >> 1), 8 + (lane & 1));
             }
         }
     }
 }
 
 // Warps: 0 loads A, 1 loads B, 2 issues the MMAs (leader), 3 owns tensor memory, 4..7 scale words, 8..15 epilogue: columns 0..127 and the rest.
-template <int BN>
+template <int BN, bool WHOLE>
 __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Fp8MatmulParams p)
 {
-    using T = Fp8Pair<BN>;
+    using T = Fp8Pair<BN, WHOLE>;
     constexpr int S = T::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *a_ring = smem, *b_ring = smem + S * A_BYTES;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + S * T::STAGE_BYTES);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + S * T::STAGE_BYTES + T::OUT_BYTES);
     uint64_t *freed = full + S;
     uint64_t *sf_full = freed + S, *sf_free = sf_full + SF_SETS;
     uint64_t *acc_full = sf_free + SF_SETS, *acc_empty = acc_full + 2;
@@ -278,7 +338,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
             uint8_t *ring = is_a ? a_ring : b_ring;
             const int slot = is_a ? A_BYTES : T::B_SLOT;
             const uint32_t bytes = is_a ? A_BYTES : T::B_BYTES;
-            const uint64_t policy = (p.band >= 0) == is_a ? L2_EVICT_LAST : L2_EVICT_NORMAL;   // the banded operand is read again soon
+            const uint64_t policy = (p.order.rows != 0) == is_a ? L2_EVICT_LAST : L2_EVICT_NORMAL;   // the banded operand is read again soon
             const uint32_t report = mapa_shared(smem_u32(full), 0);
             tma_prefetch_desc(map);
             int s = 0, it = 0;
@@ -286,7 +346,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
             bool alive = true;
             for (int tile = pair; alive && tile < total; tile += npairs) {
                 int tm, tn;
-                tile_coords(tile, p.mt, p.nt, p.band, &tm, &tn);
+                p.order.at(tile, &tm, &tn);
                 const int row = is_a ? tm * 256 + (int)crank * 128 : tn * BN + (int)crank * T::HALF_N;
                 for (int kt = 0; kt < p.ktiles; ++kt, ++it) {
                     if (!wait_quiet(&freed[s], ph, abort_flag, p.status, DEV_TIMEOUT_PRODUCER)) { alive = false; break; }
@@ -344,7 +404,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
         uint32_t next[12];
         auto fetch = [&](int tile, int g) {
             int tm, tn;
-            tile_coords(tile, p.mt, p.nt, p.band, &tm, &tn);
+            p.order.at(tile, &tm, &tn);
             const int m0 = tm * 256 + (int)crank * 128 + lane, n0 = tn * BN + lane;
             const uint32_t *sa = p.sa + (int64_t)g * p.M, *sb = p.sb + (int64_t)g * p.N;
 #pragma unroll
@@ -374,11 +434,34 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
     } else if (warp >= EPI_WARP0) {
         // ---------------- epilogue ----------------
         const int q = warp & 3, part = (warp - EPI_WARP0) >> 2;
+        constexpr int REST = BN - 128;
+        const int cols = part == 0 ? 128 : REST;
+        uint8_t *own = smem + S * T::STAGE_BYTES + (warp - EPI_WARP0) * T::WARP_BYTES;
+        uint4 *stage = reinterpret_cast<uint4 *>(own);
+        float4 *bias = reinterpret_cast<float4 *>(own + T::WARP_BYTES - 512);      // 32 columns before: part 1, !WHOLE
+        // bias of four columns a lane (and of one of the 32 before), on its way while the tile before is stored: as it lies, for a conversion would wait for it
+        uint32_t next[5];
+        auto fetch = [&](int tile) {
+            int tm, tn;
+            p.order.at(tile, &tm, &tn);
+            const int n = tn * BN + part * 128 + 4 * lane;
+#pragma unroll
+            for (int i = 0; i < 4; i++) next[i] = n + i < p.N ? bias_bits(p.bias, p.bias_type, n + i) : 0u;
+            if (!WHOLE && part == 1) next[4] = n - 3 * lane - 32 < p.N ? bias_bits(p.bias, p.bias_type, n - 3 * lane - 32) : 0u;
+        };
+        if (p.bias && my_tiles > 0) fetch(pair);
         int ti = 0;
         for (int tile = pair; tile < total; tile += npairs, ++ti) {
             const int acc = T::ONE ? 0 : ti & 1;
             int tm, tn;
-            tile_coords(tile, p.mt, p.nt, p.band, &tm, &tn);
+            p.order.at(tile, &tm, &tn);
+            if (p.bias) {
+                __syncwarp();
+                bias[lane] = make_float4(bias_float(next[0], p.bias_type), bias_float(next[1], p.bias_type), bias_float(next[2], p.bias_type), bias_float(next[3], p.bias_type));
+                if (!WHOLE && part == 1) reinterpret_cast<float *>(bias)[lane - 32] = bias_float(next[4], p.bias_type);
+                __syncwarp();
+                if (tile + npairs < total) fetch(tile + npairs);
+            }
             if (!wait_warp(&acc_full[acc], T::ONE ? (uint32_t)ti & 1u : (uint32_t)(ti >> 1) & 1u, abort_flag, p.status, DEV_TIMEOUT_EPILOGUE)) break;
             tc_fence_after();
             const uint32_t empty = mapa_shared(smem_u32(&acc_empty[acc]), 0);
@@ -392,8 +475,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
             const int n0 = tn * BN + part * 128;
             auto store = [&](auto type) {
                 constexpr int TYPE = decltype(type)::value;
-                if (part == 0) store_columns<TYPE, 128>(tacc, row0, n0, p, release);
-                else store_columns<TYPE, BN - 128>(tacc, row0, n0, p, release);
+                if (p.bias) store_columns<TYPE, true, WHOLE>(tacc, row0, n0, cols, part, stage, bias, p, release);
+                else store_columns<TYPE, false, WHOLE>(tacc, row0, n0, cols, part, stage, bias, p, release);
             };
             if (p.out_type == T_F16) store(std::integral_constant<int, T_F16>());
             else if (p.out_type == T_BF16) store(std::integral_constant<int, T_BF16>());
@@ -414,13 +497,13 @@ int g_clusters = 0;          // co-resident clusters of two CTAs on this device 
 
 }  // namespace
 
-#define VNM_FP8_PAIR(X) X(192) X(224) X(240) X(256)
+#define VNM_FP8_PAIR(X) X(192, true) X(224, true) X(240, true) X(256, true) X(192, false) X(224, false) X(240, false) X(256, false)
 
 cudaError_t fp8_pair_init()
 {
     cudaError_t e;
-#define VNM_ATTR(BN) \
-    if ((e = cudaFuncSetAttribute(fp8_pair_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8Pair<BN>::SMEM_BYTES)) != cudaSuccess) return e;
+#define VNM_ATTR(BN, WHOLE) \
+    if ((e = cudaFuncSetAttribute(fp8_pair_kernel<BN, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8Pair<BN, WHOLE>::SMEM_BYTES)) != cudaSuccess) return e;
     VNM_FP8_PAIR(VNM_ATTR)
 #undef VNM_ATTR
     int dev = 0, sms = 0;
@@ -429,7 +512,7 @@ cudaError_t fp8_pair_init()
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)(sms & ~1));
     lc.blockDim = dim3(NUM_THREADS);
-    lc.dynamicSmemBytes = Fp8Pair<256>::SMEM_BYTES;
+    lc.dynamicSmemBytes = Fp8Pair<256, true>::SMEM_BYTES;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
@@ -438,7 +521,7 @@ cudaError_t fp8_pair_init()
     lc.attrs = attr;
     lc.numAttrs = 1;
     int clusters = 0;
-    e = cudaOccupancyMaxActiveClusters(&clusters, fp8_pair_kernel<256>, &lc);
+    e = cudaOccupancyMaxActiveClusters(&clusters, fp8_pair_kernel<256, true>, &lc);
     if (e != cudaSuccess) { (void)cudaGetLastError(); clusters = 0; }
     g_clusters = clusters;
     return cudaSuccess;
@@ -479,10 +562,10 @@ cudaError_t launch_fp8_pair(const Fp8Plan &plan, const CUtensorMap &map_a, const
     attr[1] = early_launch();
     lc.attrs = attr;
     lc.numAttrs = 2;
-#define VNM_LAUNCH(BN)                                   \
-    if (plan.bn == BN) {                                 \
-        lc.dynamicSmemBytes = Fp8Pair<BN>::SMEM_BYTES;   \
-        return cudaLaunchKernelEx(&lc, fp8_pair_kernel<BN>, map_a, map_b, p); \
+#define VNM_LAUNCH(BN, WHOLE)                                      \
+    if (plan.bn == BN && (p.whole_pieces != 0) == WHOLE) {         \
+        lc.dynamicSmemBytes = Fp8Pair<BN, WHOLE>::SMEM_BYTES;      \
+        return cudaLaunchKernelEx(&lc, fp8_pair_kernel<BN, WHOLE>, map_a, map_b, p); \
     }
     VNM_FP8_PAIR(VNM_LAUNCH)
 #undef VNM_LAUNCH
