@@ -243,35 +243,51 @@ __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n
                 if (on && r < rows) *reinterpret_cast<uint4 *>(dst) = q;
             }
         } else if (left > 0) {
-            // piece q of row r, counted from the sector that these columns begin in
-            auto put = [&](int r, int q) {
-                uint8_t *row = out + r * pitch;
-                const int s = (int)(reinterpret_cast<uintptr_t>(row) & 31);
-                const int at = 32 + 16 * q - s, b = at & 15;        // where it begins in the window
-                const uint4 *w = stage + r * WINDOW + (at >> 4);
-                const uint4 lo = w[0], hi = w[1];
-                uint32_t x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            // Piece q of a row, counted from the sector that these columns begin in (s bytes into it), out of the row's window: five words at a byte offset that
+            // is even.
+            auto cut = [&](const uint32_t *window, int s, int q, uint32_t (&y)[4]) {
+                const int at = 32 + 16 * q - s;
+                const uint32_t *w = window + (at >> 2);
+                const uint32_t half = at & 2 ? 0x5432u : 0x3210u;
+                uint32_t x[5];
 #pragma unroll
-                for (int i = 0; i < 6; i++) x[i] = b & 8 ? x[i + 2] : x[i];
+                for (int i = 0; i < 5; i++) x[i] = w[i];
 #pragma unroll
-                for (int i = 0; i < 5; i++) x[i] = b & 4 ? x[i + 1] : x[i];
-                uint32_t y[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) y[i] = __byte_perm(x[i], x[i + 1], b & 2 ? 0x5432 : 0x3210);
-                const int end = s + left - 16 * q;                  // of the row, from this piece on
-                const int begin = c0 == 0 && part == 0 ? s - 16 * q : 0;
-                if (r < rows && end > 0 && begin < 16) {
-                    if (begin <= 0 && end >= 16) *reinterpret_cast<uint4 *>(row - s + 16 * q) = make_uint4(y[0], y[1], y[2], y[3]);
-                    else store_part(row - s + 16 * q, y, begin, end);
-                }
+                for (int i = 0; i < 4; i++) y[i] = __byte_perm(x[i], x[i + 1], half);
             };
-            // the sector that ends with these columns or behind them is left to the next ones, or to the other part
-            const bool last = left <= 128 && !(part == 0 && p.N - n0 > 128);
-#pragma unroll 2
-            for (int i = 0; i < 8; i++) put(4 * i + first, piece);
-            if (last) {
-#pragma unroll 1
-                for (int i = 0; i < 2; i++) put(16 * i + (lane >> 1), 8 + (lane & 1));
+            const uint32_t *words = reinterpret_cast<const uint32_t *>(stage);
+            const bool head = c0 == 0 && part == 0;                                // the sector that the row begins in is another tile's as well
+            {
+                uint8_t *row = out + first * pitch;
+                const uint32_t *window = words + first * WINDOW * 4;
+#pragma unroll 4
+                for (int i = 0; i < 8; i++, row += 4 * pitch, window += 16 * WINDOW) {
+                    const int s = (int)(reinterpret_cast<uintptr_t>(row) & 31);
+                    uint32_t y[4];
+                    cut(window, s, piece, y);
+                    if (4 * i + first < rows && 16 * piece >= (head ? s : 0) && 16 * piece + 16 <= s + left)
+                        *reinterpret_cast<uint4 *>(row - s + 16 * piece) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+            }
+            // The last sector, where it is not left to the next columns or the other part; and pieces that begin or end inside: a lane a row.
+            const bool tail = left <= 128 && !(part == 0 && p.N - n0 > 128);
+            if ((head || tail) && lane < rows) {
+                uint8_t *row = out + lane * pitch;
+                const uint32_t *window = words + lane * WINDOW * 4;
+                const int s = (int)(reinterpret_cast<uintptr_t>(row) & 31), end = s + left;
+                uint32_t y[4];
+                if (head && (s & 15)) {
+                    cut(window, s, s >> 4, y);
+                    store_part(row - s + (s & 16), y, s & 15, end - (s & 16) < 16 ? end - (s & 16) : 16);
+                }
+                if (tail && end >= 144) {
+                    cut(window, s, 8, y);
+                    *reinterpret_cast<uint4 *>(row - s + 128) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+                if (tail && (end & 15) && !(head && end < ((s + 15) & ~15))) {      // not where head and tail are one piece
+                    cut(window, s, end >> 4, y);
+                    store_part(row - s + (end & ~15), y, 0, end & 15);
+                }
             }
         }
     }
