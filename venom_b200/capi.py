@@ -90,6 +90,7 @@ def lib():
                            ("gelu", [vp, i32, i64, i32, i32, i32, vp, i64, vp, i64, vp, vp, i64, vp, vp, i64, vp, vp]),
                            ("gelu_grad", [vp, i32, i64, i32, i32, i32, vp, i64, vp, vp, i64, i32, vp, i64, vp, vp, i64, vp, vp, i32, vp, vp]),
                            ("matmul", [vp, i64, vp, i32, vp, i64, vp, i32, i32, i32, i32, vp, i32, vp, i32, i64, vp]),
+                           ("matmul_config", [i32] * 6 + [C.POINTER(C.c_int)] * 4),
                            ("device_status", [C.POINTER(C.c_int), vp])):
             getattr(L, "vnm_fp8_" + name).argtypes = args
             getattr(L, "vnm_fp8_" + name).restype = i32

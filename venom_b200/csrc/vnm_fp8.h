@@ -103,11 +103,12 @@ struct Fp8Plan {
 
 // On pairs of SMs: tiles of 256 x (192 .. 256).
 cudaError_t fp8_pair_init();
-float fp8_pair_config(int M, int N, int K, Fp8Plan *plan);   // an estimate in microseconds, < 0: not for this problem
+// wide_out: results of 32 bits; whole: their rows are stored in whole pieces (see whole_pieces).  Both return an estimate in microseconds, < 0: not for this problem.
+float fp8_pair_config(int M, int N, int K, bool wide_out, bool whole, bool bias, Fp8Plan *plan);
 cudaError_t launch_fp8_pair(const Fp8Plan &plan, const CUtensorMap &map_a, const CUtensorMap &map_b, const Fp8MatmulParams &p, cudaStream_t stream);
 // One SM a tile: 128 rows of B x (16 .. 128) rows of A, k split over a cluster where tiles are few.
 cudaError_t fp8_small_init();
-float fp8_small_config(int M, int N, int ktiles, Fp8Plan *plan);
+float fp8_small_config(int M, int N, int ktiles, bool wide_out, Fp8Plan *plan);
 cudaError_t launch_fp8_small(const Fp8Plan &plan, const CUtensorMap &map_a, const CUtensorMap &map_b, const Fp8MatmulParams &p, cudaStream_t stream);
 
 #if defined(__CUDACC__)

@@ -122,6 +122,17 @@ CUresult encode_operand(EncodeTiledFn enc, CUtensorMap *map, const void *data, i
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
+// The kernel and tile with the smaller estimate.
+int choose_plan(int M, int N, int K, bool wide_out, bool whole, bool bias, Fp8Plan *plan, bool *on_pairs)
+{
+    Fp8Plan small = {}, pair = {};
+    const float small_us = fp8_small_config(M, N, (int)(((int64_t)K + 127) / 128), wide_out, &small), pair_us = fp8_pair_config(M, N, K, wide_out, whole, bias, &pair);
+    if (small_us < 0.0f && pair_us < 0.0f) return fail(VNM_ERR_UNSUPPORTED, "vnm_fp8_matmul: no kernel for %d x %d x %d", M, N, K);
+    *on_pairs = small_us < 0.0f || (pair_us >= 0.0f && pair_us < small_us);
+    *plan = *on_pairs ? pair : small;
+    return VNM_OK;
+}
+
 // Band of the tile order of the pair kernel.  A band's operand stays in L2 while the other one streams past: row bands read A once and B once per
 // band, column bands the other way round.
 int tile_band(int M, int N, int K, int mt, int nt, int bn)
@@ -260,10 +271,9 @@ extern "C" int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, 
     p.a_f8 = a_type; p.b_f8 = b_type;
     p.status = status;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    Fp8Plan small = {}, pair = {};
-    const float small_us = fp8_small_config(M, N, p.ktiles, &small), pair_us = fp8_pair_config(M, N, K, &pair);
-    const bool on_pairs = pair_us >= 0.0f && pair_us < small_us;
-    const Fp8Plan &plan = on_pairs ? pair : small;
+    Fp8Plan plan = {};
+    bool on_pairs = false;
+    VNM_TRY(choose_plan(M, N, K, out_type == VNM_F32, p.whole_pieces != 0, bias != nullptr, &plan, &on_pairs));
     CUtensorMap map_a, map_b;
     if (encode_operand(enc, &map_a, a, lda, M, K, on_pairs ? 128 : plan.bn) != CUDA_SUCCESS || encode_operand(enc, &map_b, b, ldb, N, K, on_pairs ? plan.bn / 2 : 128) != CUDA_SUCCESS)
         return fail(VNM_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", name);
@@ -277,6 +287,23 @@ extern "C" int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, 
     p.mt = (M + plan.bn - 1) / plan.bn;
     p.nt = (N + 127) / 128;
     return done(launch_fp8_small(plan, map_a, map_b, p, s), name);
+}
+
+extern "C" int vnm_fp8_matmul_config(int M, int N, int K, int out_type, int whole, int bias, int *tile_m, int *tile_n, int *split, int *grid)
+{
+    const char *name = "vnm_fp8_matmul_config";
+    if (M < 1 || N < 1 || K < 1) return fail(VNM_ERR_BAD_ARG, "%s: sizes must be positive (got %d, %d, %d)", name, M, N, K);
+    if (!known_type(out_type)) return fail(VNM_ERR_BAD_ARG, "%s: unknown type %d", name, out_type);
+    int *status = nullptr;
+    VNM_TRY(device_ready(&status));
+    Fp8Plan plan = {};
+    bool on_pairs = false;
+    VNM_TRY(choose_plan(M, N, K, out_type == VNM_F32, whole != 0, bias != 0, &plan, &on_pairs));
+    if (tile_m) *tile_m = on_pairs ? 256 : plan.bn;
+    if (tile_n) *tile_n = on_pairs ? plan.bn : 128;
+    if (split) *split = plan.split;
+    if (grid) *grid = plan.grid;
+    return VNM_OK;
 }
 
 extern "C" int vnm_fp8_device_status(int *status, void *stream)

@@ -13,6 +13,7 @@
 
 #include <cuda_bf16.h>
 
+#include <cmath>
 #include <type_traits>
 
 namespace vnm {
@@ -462,8 +463,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
             p.order.at(tile, &tm, &tn);
             const int n = tn * BN + part * 128 + 4 * lane;
 #pragma unroll
-            for (int i = 0; i < 4; i++) next[i] = n + i < p.N ? bias_bits(p.bias, p.bias_type, n + i) : 0u;
-            if (!WHOLE && part == 1) next[4] = n - 3 * lane - 32 < p.N ? bias_bits(p.bias, p.bias_type, n - 3 * lane - 32) : 0u;
+            for (int i = 0; i < 4; i++) next[i] = bias_bits(p.bias, p.bias_type, n + i < p.N ? n + i : p.N - 1);      // past the end: not stored
+            if (!WHOLE && part == 1) next[4] = bias_bits(p.bias, p.bias_type, n - 3 * lane - 32 < p.N ? n - 3 * lane - 32 : p.N - 1);
         };
         if (p.bias && my_tiles > 0) fetch(pair);
         int ti = 0;
@@ -543,17 +544,28 @@ cudaError_t fp8_pair_init()
     return cudaSuccess;
 }
 
-float fp8_pair_config(int M, int N, int K, Fp8Plan *plan)
+// The cost of a call, us: a start, waves of tiles (between the whole number that the last one makes and the fraction that the power limit sees), and the last
+// tile's epilogue.  A tile takes its k-tiles' time or its epilogue's, whichever is longer (a smooth maximum), or with one accumulator both.  Fitted
+// together with the costs of vnm_fp8_small.cu to steady calls on inputs that change, 431 shapes of 1 to 16384 x 8 to 36864 x 64 to 16384, odd ones and round ones, with and
+// without a bias, fp16 and fp32 results: ratio to the measured time 0.8 to 1.25; the plan chosen over both kernels takes 1.02 of the fastest one's time
+// on average, 1.6 at most (6687 x 40 x 3212).
+float fp8_pair_config(int M, int N, int K, bool wide_out, bool whole, bool bias, Fp8Plan *plan)
 {
     if (g_clusters <= 0) return -1.0f;
-    static const int widths[4] = {256, 240, 224, 192};
+    static const int widths[4] = {192, 224, 240, 256};
+    static const float ktile[4] = {0.333f, 0.364f, 0.379f, 0.406f};
     const int64_t mt = ((int64_t)M + 255) / 256;
+    const float kt = (float)(((int64_t)K + 127) / 128);
+    const float edge = 1.81f + (wide_out ? 1.28f : 0.0f) + (whole ? 0.0f : wide_out ? 3.16f : 1.88f) + (bias ? 0.62f : 0.0f);
     float best = -1.0f;
-    for (int w : widths) {
+    for (int i = 0; i < 4; i++) {
+        const int w = widths[i];
         const int64_t nt = ((int64_t)N + w - 1) / w, tiles = mt * nt;
         if (tiles > INT32_MAX / 2) continue;
-        const int64_t waves = (tiles + g_clusters - 1) / g_clusters;
-        const float us = (float)waves * ((float)((K + 127) / 128) * w / 900.0f + (w == 256 ? 0.4f : 0.2f));
+        const float waves = 0.72f * (float)((tiles + g_clusters - 1) / g_clusters) + 0.28f * (float)tiles / (float)g_clusters;
+        const float mma = kt * ktile[i], out = edge * (float)w / 240.0f;
+        const float one = w == 256 ? mma + 0.92f * out : powf(powf(mma, 1.233f) + powf(out, 1.233f), 1.0f / 1.233f);
+        const float us = 4.13f + waves * one + 0.21f * out;
         if (best < 0.0f || us < best) {
             best = us;
             plan->bn = w;

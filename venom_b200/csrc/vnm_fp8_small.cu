@@ -287,6 +287,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 2) fp8_small_kernel(const __gri
     }
 }
 
+int g_sms = 0;
+
 }  // namespace
 
 #define VNM_FP8_SMALL(X) X(16) X(32) X(64) X(128)
@@ -298,19 +300,44 @@ cudaError_t fp8_small_init()
     if ((e = cudaFuncSetAttribute(fp8_small_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8Small<BN>::SMEM_BYTES)) != cudaSuccess) return e;
     VNM_FP8_SMALL(VNM_ATTR)
 #undef VNM_ATTR
-    return cudaSuccess;
+    int dev = 0;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+    return cudaDeviceGetAttribute(&g_sms, cudaDevAttrMultiProcessorCount, dev);
 }
 
-float fp8_small_config(int M, int N, int ktiles, Fp8Plan *plan)
+// The cost of a call, us: a start, then a CTA's k-tiles (one CTA an SM, or two that share it) or the operands' bytes, whichever takes longer, its epilogue, and the exchange
+// of partial sums.  See fp8_pair_config for what they were fitted to.  (512 x 4096 x 4096: 128 x 64 24.7 us, pairs 14.0;  16 x 36864 x 12288: 128 x 16 71.1, of which
+// the weight's bytes 69.2;  128 x 4096 x 1024: 128 x 32 6.5, pairs 8.2;  8 x 1024 x 1024: 128 x 16 alone 5.0, split by eight 4.1.)
+float fp8_small_config(int M, int N, int ktiles, bool wide_out, Fp8Plan *plan)
 {
-    plan->bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const int64_t tiles = ((int64_t)M + plan->bn - 1) / plan->bn * (((int64_t)N + 127) / 128);
-    plan->split = 1;
-    while (plan->split < 8 && tiles * plan->split * 2 <= 296 && ktiles >= 4 * plan->split) plan->split *= 2;
-    plan->grid = (int)(tiles * plan->split);
-    if (M <= 128) return 0.0f;
-    const int64_t waves = ((int64_t)plan->grid + 295) / 296;
-    return (float)waves * ((float)(ktiles + plan->split - 1) / plan->split * 0.35f + 1.0f);
+    struct Cost { float start, kt1, kt2, out, split, bytes; };
+    static const Cost cost[4] = {{1.79f, 0.174f, 0.476f, 1.85f, 0.57f, 0.101f}, {1.92f, 0.173f, 0.477f, 2.79f, 0.65f, 0.091f}, {2.64f, 0.181f, 0.599f, 3.66f, 1.28f, 0.084f},
+                                 {5.27f, 0.253f, 0.911f, 4.00f, 2.91f, 0.106f}};
+    const int64_t nt = ((int64_t)N + 127) / 128;
+    const int sms = g_sms > 0 ? g_sms : 148;
+    float best = -1.0f;
+    for (int i = 0; i < 4; i++) {
+        const int bn = 16 << i;
+        if (i > 0 && bn >= 2 * (int64_t)M) break;
+        const int64_t tiles = ((int64_t)M + bn - 1) / bn * nt;
+        if (tiles > INT32_MAX / 8) continue;
+        const float mem = (float)tiles * (float)ktiles * (float)(128 + bn) * 128e-6f * cost[i].bytes;
+        for (int split = 1; split <= 8 && split <= ktiles; split *= 2) {
+            const int64_t ctas = tiles * split;
+            if (split > 1 && ctas > 8 * sms) break;
+            const int64_t waves = (ctas + 2 * sms - 1) / (2 * sms);
+            const float per = (float)((ktiles + split - 1) / split);
+            const float work = ctas <= sms ? per * cost[i].kt1 : (float)waves * per * cost[i].kt2;
+            const float us = cost[i].start + (work > mem ? work : mem) + (float)waves * cost[i].out * (wide_out ? 1.6f : 1.0f) + (split > 1 ? cost[i].split : 0.0f);
+            if (best < 0.0f || us < best) {
+                best = us;
+                plan->bn = bn;
+                plan->split = split;
+                plan->grid = (int)ctas;
+            }
+        }
+    }
+    return best;
 }
 
 cudaError_t launch_fp8_small(const Fp8Plan &plan, const CUtensorMap &map_a, const CUtensorMap &map_b, const Fp8MatmulParams &p, cudaStream_t stream)
