@@ -147,17 +147,33 @@ __device__ __forceinline__ float finite_amax8(const float (&v)[8])
 
 // (a, b) / s in 8 bits, a in the low byte.
 template <int F8>
-__device__ __forceinline__ uint32_t round2(float a, float b, float inv)
+__device__ __forceinline__ uint32_t round2(float a, float b)
 {
-    return __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, F8 == F8_E4M3 ? __NV_E4M3 : __NV_E5M2);
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, F8 == F8_E4M3 ? __NV_E4M3 : __NV_E5M2);
+}
+// (a x, b y), both rounded to nearest (exact here)
+__device__ __forceinline__ float2 mul2(float a, float b, float x, float y)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 p, q;\n\t"
+        "mov.b64 p, {%2, %3};\n\t"
+        "mov.b64 q, {%4, %5};\n\t"
+        "mul.rn.f32x2 p, p, q;\n\t"
+        "mov.b64 {%0, %1}, p;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a), "f"(b), "f"(x), "f"(y));
+    return r;
 }
 template <int F8>
 __device__ __forceinline__ uint2 round8(const float (&v)[8], float inv)
 {
-    uint2 r;
-    r.x = __byte_perm(round2<F8>(v[0], v[1], inv), round2<F8>(v[2], v[3], inv), 0x5410);
-    r.y = __byte_perm(round2<F8>(v[4], v[5], inv), round2<F8>(v[6], v[7], inv), 0x5410);
-    return r;
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 s = mul2(v[2 * i], v[2 * i + 1], inv, inv);
+        h[i] = round2<F8>(s.x, s.y);
+    }
+    return make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
 }
 // Four rounded values of a block with infinities, which the conversion has made the largest value: they stay infinities in e5m2 and become NaN in e4m3.
 template <int F8>
@@ -196,17 +212,19 @@ __device__ __forceinline__ uint32_t bytes_of4(uint32_t code)
     w |= __shfl_xor_sync(0xffffffffu, w, 8);
     return w;
 }
-// Codes of four blocks of eight values a lane; bit i of *odd: block i has an infinity.
+// Codes of four blocks of eight values a lane; byte i of *odd: block i has an infinity.  Returns whether any block of the warp has one: that way lies off the
+// usual one (selected by value instead, it took a third of all instructions).
 template <int F8>
-__device__ __forceinline__ uint32_t codes_of4(const float (&v)[4][8], uint32_t *odd)
+__device__ __forceinline__ bool codes_of4(const float (&v)[4][8], uint32_t *codes, uint32_t *odd)
 {
     float m = max16_of4(amax8(v[0]), amax8(v[1]), amax8(v[2]), amax8(v[3]));
-    *odd = 0;
-    if (__any_sync(0xffffffffu, !finite(m))) {
+    const bool any = __any_sync(0xffffffffu, !finite(m));
+    if (any) {
         *odd = bytes_of4(finite(m) ? 0u : 1u);
         m = max16_of4(finite_amax8(v[0]), finite_amax8(v[1]), finite_amax8(v[2]), finite_amax8(v[3]));
     }
-    return bytes_of4(scale_code<F8>(m));
+    *codes = bytes_of4(scale_code<F8>(m));
+    return any;
 }
 __device__ __forceinline__ uint32_t byte_of(uint32_t w, int i) { return (w >> (8 * i)) & 0xFFu; }
 
@@ -354,17 +372,21 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
 
         auto store = [&](uint8_t *data, int64_t ld, uint8_t *scales, auto type) {
             constexpr int T8 = decltype(type)::value;
-            uint32_t odd;
-            const uint32_t codes = codes_of4<T8>(v, &odd);
+            uint32_t codes, odd = 0;
+            const bool any = codes_of4<T8>(v, &codes, &odd);
+            uint2 q[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) q[i] = round8<T8>(v[i], inverse_scale(byte_of(codes, i)));
+            if (any) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (byte_of(odd, i)) q[i] = mend8<T8>(q[i], v[i]);
+            }
             if (on) {
                 uint8_t *dst = data + r * ld + c;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float inv = inverse_scale(byte_of(codes, i));
-                    uint2 q = round8<T8>(v[i], inv);
-                    if (byte_of(odd, i)) q = mend8<T8>(q, v[i]);
-                    if (c + 128 * i < p.cols) *reinterpret_cast<uint2 *>(dst + 128 * i) = q;
-                }
+                for (int i = 0; i < 4; i++)
+                    if (c + 128 * i < p.cols) *reinterpret_cast<uint2 *>(dst + 128 * i) = q[i];
                 // blocks past the last one are zeros, whose code is 0
                 if (sub == 0) reinterpret_cast<uint32_t *>(scales)[word] = codes;
             }
@@ -446,22 +468,27 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
             }
         }
     }
-    auto store_rows = [&](uint8_t *data, int64_t ld, uint8_t *scales, auto type, uint32_t codes, uint32_t odd) {
+    auto store_rows = [&](uint8_t *data, int64_t ld, uint8_t *scales, auto type, uint32_t codes, uint32_t odd, bool any) {
         constexpr int T8 = decltype(type)::value;
         uint8_t *dst = data + r0 * ld + c;
+        uint2 q[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            uint2 q = round8<T8>(v[j], inverse_scale(byte_of(codes, j)));
-            if (byte_of(odd, j)) q = mend8<T8>(q, v[j]);
-            if (in && (WHOLE || j < left)) *reinterpret_cast<uint2 *>(dst + j * ld) = q;
+        for (int j = 0; j < 4; j++) q[j] = round8<T8>(v[j], inverse_scale(byte_of(codes, j)));
+        if (any) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (byte_of(odd, j)) q[j] = mend8<T8>(q[j], v[j]);
         }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (in && (WHOLE || j < left)) *reinterpret_cast<uint2 *>(dst + j * ld) = q[j];
         if ((lane & 3) == 0 && own_row < left) store_scale(scales, p.rows, r0 + own_row, tc, cblocks, byte_of(codes, own_row));
     };
     if constexpr (OP == FP8_GELU) {
         if (p.ckpt) {
-            uint32_t odd;
-            const uint32_t codes = codes_of4<F8_E4M3>(v, &odd);
-            store_rows(p.ckpt, p.ldc, p.ckpt_scales, std::integral_constant<int, F8_E4M3>(), codes, odd);
+            uint32_t codes, odd = 0;
+            const bool any = codes_of4<F8_E4M3>(v, &codes, &odd);
+            store_rows(p.ckpt, p.ldc, p.ckpt_scales, std::integral_constant<int, F8_E4M3>(), codes, odd, any);
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -492,9 +519,10 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
     }
 
     if (p.data) {
-        uint32_t odd = tile_odd ? 0x01010101u : 0u, codes = tile_code * 0x01010101u;
-        if constexpr (!SQUARE) codes = codes_of4<F8>(v, &odd);
-        store_rows(p.data, p.ldd, p.scales, std::integral_constant<int, F8>(), codes, odd);
+        uint32_t odd = 0x01010101u, codes = tile_code * 0x01010101u;
+        bool any = tile_odd;
+        if constexpr (!SQUARE) any = codes_of4<F8>(v, &codes, &odd);
+        store_rows(p.data, p.ldd, p.scales, std::integral_constant<int, F8>(), codes, odd, any);
     }
 
     // four threads a column: rows of sh.amax_of taken in turn
@@ -506,36 +534,40 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
     };
     if (p.data_t) {
         float inv[8];
+        bool any = tile_odd;
         if constexpr (!SQUARE) {
-#pragma unroll 1
-            for (int pass = 0; pass < 2; pass++) {   // the second one only where a column has an infinity
-                if (pass == 1 && !__syncthreads_or(sh.inv_of[own_col] < 0.0f)) break;
-                float m[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (pass == 0) {
-                        m[i] = fmaxf(fmaxf(fabsf(v[0][i]), fabsf(v[1][i])), fmaxf(fabsf(v[2][i]), fabsf(v[3][i])));
-                    } else {
-                        m[i] = 0.0f;
-#pragma unroll
-                        for (int j = 0; j < 4; j++) m[i] = finite(v[j][i]) ? fmaxf(m[i], fabsf(v[j][i])) : m[i];
-                    }
-                }
-                put8(m);
+            // scales of the tile's columns from what put8() has laid out
+            auto column_scales = [&](bool finite_only) {
                 __syncthreads();
                 float a = 0.0f;
 #pragma unroll
                 for (int k = 0; k < 8; k++) a = fmaxf(a, sh.amax_of[4 * k + part][own_col]);
                 a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
                 a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+                const bool odd = finite_only ? sh.inv_of[own_col] < 0.0f : !finite(a);
+                __syncwarp();
                 if (part == 0) {
-                    const bool odd = pass == 0 ? !finite(a) : sh.inv_of[own_col] < 0.0f;
                     const uint32_t code = scale_code<F8>(finite(a) ? a : 0.0f);
-                    sh.inv_of[own_col] = odd ? -inverse_scale(code) : inverse_scale(code);   // the sign says that it has one
+                    sh.inv_of[own_col] = odd ? -inverse_scale(code) : inverse_scale(code);   // the sign says that it has an infinity
                     const int col = tc * 128 + own_col;
                     if (WHOLE || col < p.cols) store_scale(p.scales_t, p.cols, col, tr, rblocks, code);
                 }
-                __syncthreads();
+                return __syncthreads_or(odd) != 0;
+            };
+            float m[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) m[i] = fmaxf(fmaxf(fabsf(v[0][i]), fabsf(v[1][i])), fmaxf(fabsf(v[2][i]), fabsf(v[3][i])));
+            put8(m);
+            any = column_scales(false);
+            if (any) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    m[i] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) m[i] = finite(v[j][i]) ? fmaxf(m[i], fabsf(v[j][i])) : m[i];
+                }
+                put8(m);
+                (void)column_scales(true);
             }
             const float4 lo = *reinterpret_cast<const float4 *>(&sh.inv_of[group * 8]), hi = *reinterpret_cast<const float4 *>(&sh.inv_of[group * 8 + 4]);
             inv[0] = lo.x; inv[1] = lo.y; inv[2] = lo.z; inv[3] = lo.w;
@@ -545,12 +577,24 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
             for (int i = 0; i < 8; i++) inv[i] = tile_odd ? -inverse_scale(tile_code) : inverse_scale(tile_code);
             if (threadIdx.x < 128 && tc * 128 + (int)threadIdx.x < p.cols) store_scale(p.scales_t, p.cols, tc * 128 + threadIdx.x, tr, rblocks, tile_code);
         }
+        uint32_t *const image = &sh.image[group * 256 + ((warp * 2 + half) ^ (2 * group))];
+        if (!any) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float a = fabsf(inv[i]);
-            uint32_t w = __byte_perm(round2<F8>(v[0][i], v[1][i], a), round2<F8>(v[2][i], v[3][i], a), 0x5410);
-            if (inv[i] < 0.0f) w = mend4<F8>(w, v[0][i], v[1][i], v[2][i], v[3][i]);
-            sh.image[(group * 8 + i) * 32 + ((warp * 2 + half) ^ (2 * group))] = w;
+            for (int i = 0; i < 8; i += 2) {
+                float2 s[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[j] = mul2(v[j][i], v[j][i + 1], inv[i], inv[i + 1]);
+                image[i * 32] = __byte_perm(round2<F8>(s[0].x, s[1].x), round2<F8>(s[2].x, s[3].x), 0x5410);
+                image[i * 32 + 32] = __byte_perm(round2<F8>(s[0].y, s[1].y), round2<F8>(s[2].y, s[3].y), 0x5410);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float a = fabsf(inv[i]);
+                uint32_t w = __byte_perm(round2<F8>(v[0][i] * a, v[1][i] * a), round2<F8>(v[2][i] * a, v[3][i] * a), 0x5410);
+                if (inv[i] < 0.0f) w = mend4<F8>(w, v[0][i], v[1][i], v[2][i], v[3][i]);
+                image[i * 32] = w;
+            }
         }
         __syncthreads();
         // sixteen lanes a column: eight rows each
