@@ -119,6 +119,34 @@ __device__ __forceinline__ void store8(void *y, int64_t at, int c, int cols, int
     }
 }
 
+// ---- two 32-bit operations an instruction, each rounded to nearest ----
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 p, q;\n\t"
+        "mov.b64 p, {%2, %3};\n\t"
+        "mov.b64 q, {%4, %5};\n\t"
+        "mul.rn.f32x2 p, p, q;\n\t"
+        "mov.b64 {%0, %1}, p;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 p, q, s;\n\t"
+        "mov.b64 p, {%2, %3};\n\t"
+        "mov.b64 q, {%4, %5};\n\t"
+        "mov.b64 s, {%6, %7};\n\t"
+        "fma.rn.f32x2 p, p, q, s;\n\t"
+        "mov.b64 {%0, %1}, p;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // ---- scales ----
 // The scale's byte (its exponent + 127) for a block whose largest finite magnitude is amax.
 template <int F8>
@@ -151,26 +179,13 @@ __device__ __forceinline__ uint32_t round2(float a, float b)
 {
     return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, F8 == F8_E4M3 ? __NV_E4M3 : __NV_E5M2);
 }
-// (a x, b y), both rounded to nearest (exact here)
-__device__ __forceinline__ float2 mul2(float a, float b, float x, float y)
-{
-    float2 r;
-    asm("{\n\t.reg .b64 p, q;\n\t"
-        "mov.b64 p, {%2, %3};\n\t"
-        "mov.b64 q, {%4, %5};\n\t"
-        "mul.rn.f32x2 p, p, q;\n\t"
-        "mov.b64 {%0, %1}, p;\n\t}"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a), "f"(b), "f"(x), "f"(y));
-    return r;
-}
 template <int F8>
 __device__ __forceinline__ uint2 round8(const float (&v)[8], float inv)
 {
     uint32_t h[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float2 s = mul2(v[2 * i], v[2 * i + 1], inv, inv);
+        const float2 s = mul2(make_float2(v[2 * i], v[2 * i + 1]), both(inv));
         h[i] = round2<F8>(s.x, s.y);
     }
     return make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
@@ -250,26 +265,6 @@ __device__ __forceinline__ float fast_rcp(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// The exact form by a published approximation of erfc (Abramowitz and Stegun, 7.1.26, |error| <= 1.5e-7): with t = 1 / (1 + p |z|), z = x / sqrt 2,
-// erfc |z| = (a1 t + .. + a5 t^5) exp(-z^2).  The exponential is the density's as well, which the derivative needs, so one exponential and one reciprocal
-// give both.  With h = erfc |z| / 2, gelu(x) = max(x, 0) - |x| h: no cancellation in the tail of negative x.
-__device__ __forceinline__ float half_erfc(float x, float *e)
-{
-    const float t = fast_rcp(fmaf(0.3275911f * 0.70710678118654752f, fabsf(x), 1.0f));
-    *e = fast_exp2(x * (x * -0.72134752044448170f));
-    float poly = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-    poly = fmaf(poly, t, 0.5f * 1.421413741f);
-    poly = fmaf(poly, t, 0.5f * -0.284496736f);
-    poly = fmaf(poly, t, 0.5f * 0.254829592f);
-    return poly * t * *e;
-}
-// The tanh form: (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
-__device__ __forceinline__ float gelu_sigmoid(float x, float *du2)
-{
-    const float x2 = x * x;
-    *du2 = fmaf(0.214064448817801f, x2, 1.59576912160573f);
-    return fast_rcp(1.0f + fast_exp2(x * fmaf(0.0713548162726f * -1.4426950408889634f, x2, 1.59576912160573f * -1.4426950408889634f)));
-}
 __device__ __forceinline__ float max_nan(float a, float b)   // a NaN stays
 {
     float r;
@@ -282,26 +277,65 @@ __device__ __forceinline__ float min_nan(float a, float b)
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// Beyond 64 either form is x or 0 and the derivative 1 or 0; the square of a far larger x would overflow beside a zero.  So -inf gives 0.
+// Beyond 64 either form is x or 0 and the derivative 1 or 0: values are cut off there, ahead of squares that would overflow beside a zero.  So -inf gives 0.
 __device__ __forceinline__ float near(float x) { return max_nan(min_nan(x, 64.0f), -64.0f); }
-template <bool TANH>
-__device__ __forceinline__ float gelu(float x)
+
+// The exact form by a published approximation of erfc (Abramowitz and Stegun, 7.1.26, |error| <= 1.5e-7): with t = 1 / (1 + p |z|), z = x / sqrt 2,
+// erfc |z| = (a1 t + .. + a5 t^5) exp(-z^2).  The exponential is the density's as well, which the derivative needs, so one exponential and one reciprocal
+// give both.  With h = erfc |z| / 2, gelu(x) = max(x, 0) - |x| h: no cancellation in the tail of negative x.  a = |x|, cut off.
+__device__ __forceinline__ float2 half_erfc(float2 a, float2 *e)
 {
-    float d;
-    if (TANH) return max_nan(x, -64.0f) * gelu_sigmoid(near(x), &d);
-    return fmaf(-min_nan(fabsf(x), 64.0f), half_erfc(x, &d), max_nan(x, 0.0f));
+    const float2 d = fma2(both(0.3275911f * 0.70710678118654752f), a, both(1.0f));
+    const float2 t = make_float2(fast_rcp(d.x), fast_rcp(d.y));
+    const float2 q = mul2(mul2(a, a), both(-0.72134752044448170f));
+    *e = make_float2(fast_exp2(q.x), fast_exp2(q.y));
+    float2 poly = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
+    poly = fma2(poly, t, both(0.5f * 1.421413741f));
+    poly = fma2(poly, t, both(0.5f * -0.284496736f));
+    poly = fma2(poly, t, both(0.5f * 0.254829592f));
+    return mul2(mul2(poly, t), *e);
+}
+// The tanh form: (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3); x cut off.
+__device__ __forceinline__ float2 gelu_sigmoid(float2 x, float2 x2)
+{
+    const float2 q = mul2(x, fma2(both(0.0713548162726f * -1.4426950408889634f), x2, both(1.59576912160573f * -1.4426950408889634f)));
+    return make_float2(fast_rcp(1.0f + fast_exp2(q.x)), fast_rcp(1.0f + fast_exp2(q.y)));
 }
 template <bool TANH>
-__device__ __forceinline__ float gelu_grad(float x)
+__device__ __forceinline__ void gelu2(float &x, float &y)
 {
-    float d;
+    float2 r;
     if (TANH) {
-        x = near(x);
-        const float s = gelu_sigmoid(x, &d);
-        return fmaf(x * s * (1.0f - s), d, s);
+        const float2 lo = make_float2(max_nan(x, -64.0f), max_nan(y, -64.0f)), n = make_float2(min_nan(lo.x, 64.0f), min_nan(lo.y, 64.0f));
+        r = mul2(lo, gelu_sigmoid(n, mul2(n, n)));
+    } else {
+        const float2 a = make_float2(min_nan(fabsf(x), 64.0f), min_nan(fabsf(y), 64.0f));
+        float2 e;
+        const float2 h = half_erfc(a, &e);
+        r = fma2(make_float2(-a.x, -a.y), h, make_float2(max_nan(x, 0.0f), max_nan(y, 0.0f)));
     }
-    const float h = half_erfc(x, &d);
-    return fmaf(x, d * 0.39894228040143268f, x < 0.0f ? h : 1.0f - h);
+    x = r.x;
+    y = r.y;
+}
+// (x, y) times the derivative at (a, b)
+template <bool TANH>
+__device__ __forceinline__ void times_gelu_grad2(float &x, float &y, float a, float b)
+{
+    const float2 n = make_float2(near(a), near(b));
+    float2 g;
+    if (TANH) {
+        const float2 n2 = mul2(n, n), s = gelu_sigmoid(n, n2);
+        const float2 du = fma2(both(0.214064448817801f), n2, both(1.59576912160573f));
+        g = fma2(mul2(mul2(n, s), fma2(both(-1.0f), s, both(1.0f))), du, s);
+    } else {
+        float2 e;
+        const float2 h = half_erfc(make_float2(fabsf(n.x), fabsf(n.y)), &e);
+        const float2 far = make_float2(n.x < 0.0f ? h.x : 1.0f - h.x, n.y < 0.0f ? h.y : 1.0f - h.y);
+        g = fma2(n, mul2(e, both(0.39894228040143268f)), far);
+    }
+    const float2 r = mul2(make_float2(x, y), g);
+    x = r.x;
+    y = r.y;
 }
 
 // Eight values of an e4m3 checkpoint whose block has this code.
@@ -313,8 +347,9 @@ __device__ __forceinline__ void ckpt_values(uint2 q, uint32_t code, float (&h)[8
         const uint32_t w = (i < 2 ? q.x : q.y) >> (16 * (i & 1));
         const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3);
         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r));
-        h[2 * i] = f.x * s;
-        h[2 * i + 1] = f.y * s;
+        const float2 r2 = mul2(f, both(s));
+        h[2 * i] = r2.x;
+        h[2 * i + 1] = r2.y;
     }
 }
 
@@ -396,14 +431,14 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[i][j] = gelu<TANH>(v[i][j]);
+                for (int j = 0; j < 8; j += 2) gelu2<TANH>(v[i][j], v[i][j + 1]);
         } else if constexpr (OP == FP8_GELU_GRAD) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float x[8];
                 ckpt_values(h[i], byte_of(h_codes, i), x);
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[i][j] *= gelu_grad<TANH>(x[j]);
+                for (int j = 0; j < 8; j += 2) times_gelu_grad2<TANH>(v[i][j], v[i][j + 1], x[j], x[j + 1]);
             }
         }
         if (OP != FP8_PLAIN && p.y && on) {
@@ -464,7 +499,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
                 float h[8];
                 ckpt_values(q[j], codes[j], h);
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[j][i] *= gelu_grad<TANH>(h[i]);
+                for (int i = 0; i < 8; i += 2) times_gelu_grad2<TANH>(v[j][i], v[j][i + 1], h[i], h[i + 1]);
             }
         }
     }
@@ -493,7 +528,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[j][i] = gelu<TANH>(v[j][i]);   // of the zeros that pad: zero
+            for (int i = 0; i < 8; i += 2) gelu2<TANH>(v[j][i], v[j][i + 1]);   // of the zeros that pad: zero
     }
 
     uint32_t tile_code = 0;
@@ -583,7 +618,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
             for (int i = 0; i < 8; i += 2) {
                 float2 s[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[j] = mul2(v[j][i], v[j][i + 1], inv[i], inv[i + 1]);
+                for (int j = 0; j < 4; j++) s[j] = mul2(make_float2(v[j][i], v[j][i + 1]), make_float2(inv[i], inv[i + 1]));
                 image[i * 32] = __byte_perm(round2<F8>(s[0].x, s[1].x), round2<F8>(s[2].x, s[3].x), 0x5410);
                 image[i * 32 + 32] = __byte_perm(round2<F8>(s[0].y, s[1].y), round2<F8>(s[2].y, s[3].y), 0x5410);
             }
