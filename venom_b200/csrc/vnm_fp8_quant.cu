@@ -86,6 +86,77 @@ __device__ __forceinline__ void to_floats(const Raw<TYPE> &r, float (&v)[8])
     }
 }
 
+// The pair of words' values.
+template <int TYPE>
+__device__ __forceinline__ float2 pair_of(const Raw<TYPE> &r, int k)
+{
+    if constexpr (TYPE == T_F32) {
+        return make_float2(__uint_as_float(r.w[2 * k]), __uint_as_float(r.w[2 * k + 1]));
+    } else if constexpr (TYPE == T_F16) {
+        // volatile: converted anew for each use.  Kept between the uses, 32 values of a thread cost the tiles kernel its third CTA of an SM.
+        float2 f;
+        asm volatile("{\n\t.reg .b16 l, h;\n\t"
+                     "mov.b32 {l, h}, %2;\n\t"
+                     "cvt.f32.f16 %0, l;\n\t"
+                     "cvt.f32.f16 %1, h;\n\t}"
+                     : "=f"(f.x), "=f"(f.y)
+                     : "r"(r.w[k]));
+        return f;
+    } else return make_float2(__uint_as_float(r.w[k] << 16), __uint_as_float(r.w[k] & 0xFFFF0000u));
+}
+// Larger magnitudes of two words, passing over NaN.
+template <int TYPE>
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b)
+{
+    if constexpr (TYPE == T_F16) {
+        const __half2 m = __hmax2(__habs2(*reinterpret_cast<const __half2 *>(&a)), __habs2(*reinterpret_cast<const __half2 *>(&b)));
+        return *reinterpret_cast<const uint32_t *>(&m);
+    } else {
+        const __nv_bfloat162 m = __hmax2(__habs2(*reinterpret_cast<const __nv_bfloat162 *>(&a)), __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&b)));
+        return *reinterpret_cast<const uint32_t *>(&m);
+    }
+}
+template <int TYPE>
+__device__ __forceinline__ float2 word_values(uint32_t w)
+{
+    if constexpr (TYPE == T_F16) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+// Four rows x eight columns of a thread: as they were loaded (16-bit types whose values are only rounded: half of the registers, and maxima of two values an
+// instruction), or in 32 bits.
+template <int TYPE, bool AS_LOADED>
+struct Block4;
+template <int TYPE>
+struct Block4<TYPE, true> {
+    Raw<TYPE> raw[4];
+    __device__ __forceinline__ float2 at(int j, int k) const { return pair_of<TYPE>(raw[j], k); }
+    __device__ __forceinline__ float row_amax(int j) const
+    {
+        const uint32_t *w = raw[j].w;
+        const float2 m = word_values<TYPE>(max_word<TYPE>(max_word<TYPE>(w[0], w[1]), max_word<TYPE>(w[2], w[3])));
+        return fmaxf(m.x, m.y);
+    }
+    __device__ __forceinline__ float2 col_amax(int k) const
+    {
+        return word_values<TYPE>(max_word<TYPE>(max_word<TYPE>(raw[0].w[k], raw[1].w[k]), max_word<TYPE>(raw[2].w[k], raw[3].w[k])));
+    }
+};
+template <int TYPE>
+struct Block4<TYPE, false> {
+    float v[4][8];
+    __device__ __forceinline__ float2 at(int j, int k) const { return make_float2(v[j][2 * k], v[j][2 * k + 1]); }
+    __device__ __forceinline__ float row_amax(int j) const
+    {
+        const float a = fmaxf(fmaxf(fabsf(v[j][0]), fabsf(v[j][1])), fmaxf(fabsf(v[j][2]), fabsf(v[j][3])));
+        return fmaxf(a, fmaxf(fmaxf(fabsf(v[j][4]), fabsf(v[j][5])), fmaxf(fabsf(v[j][6]), fabsf(v[j][7]))));
+    }
+    __device__ __forceinline__ float2 col_amax(int k) const
+    {
+        return make_float2(fmaxf(fmaxf(fabsf(v[0][2 * k]), fabsf(v[1][2 * k])), fmaxf(fabsf(v[2][2 * k]), fabsf(v[3][2 * k]))),
+                           fmaxf(fmaxf(fabsf(v[0][2 * k + 1]), fabsf(v[1][2 * k + 1])), fmaxf(fabsf(v[2][2 * k + 1]), fabsf(v[3][2 * k + 1]))));
+    }
+};
+
 template <int TYPE>
 __device__ __forceinline__ void store8(void *y, int64_t at, int c, int cols, int align, const float (&v)[8])
 {
@@ -160,39 +231,35 @@ __device__ __forceinline__ float scale_value(uint32_t code) { return code ? __ui
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < __uint_as_float(0x7F800000u); }
 
 // The maximum passes over NaN; an infinity shows in it, and takes its block (`odd`) through the slow forms below.
-__device__ __forceinline__ float amax8(const float (&v)[8])
-{
-    const float a = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), b = fmaxf(fmaxf(fabsf(v[4]), fabsf(v[5])), fmaxf(fabsf(v[6]), fabsf(v[7])));
-    return fmaxf(a, b);
-}
-__device__ __forceinline__ float finite_amax8(const float (&v)[8])
+__device__ __forceinline__ float finite_max(float m, float x) { return finite(x) ? fmaxf(m, fabsf(x)) : m; }
+template <typename B>
+__device__ __forceinline__ float finite_row_amax(const B &v, int j)
 {
     float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = finite(v[i]) ? fmaxf(m, fabsf(v[i])) : m;
+    for (int k = 0; k < 4; k++) m = finite_max(finite_max(m, v.at(j, k).x), v.at(j, k).y);
     return m;
 }
 
-// (a, b) / s in 8 bits, a in the low byte.
 template <int F8>
 __device__ __forceinline__ uint32_t round2(float a, float b)
 {
     return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, F8 == F8_E4M3 ? __NV_E4M3 : __NV_E5M2);
 }
-template <int F8>
-__device__ __forceinline__ uint2 round8(const float (&v)[8], float inv)
+template <int F8, typename B>
+__device__ __forceinline__ uint2 round8(const B &v, int j, float inv)
 {
     uint32_t h[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 s = mul2(make_float2(v[2 * i], v[2 * i + 1]), both(inv));
-        h[i] = round2<F8>(s.x, s.y);
+    for (int k = 0; k < 4; k++) {
+        const float2 s = mul2(v.at(j, k), both(inv));
+        h[k] = round2<F8>(s.x, s.y);
     }
     return make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
 }
-// Four rounded values of a block with infinities, which the conversion has made the largest value: they stay infinities in e5m2 and become NaN in e4m3.
+// A call, so that the registers of this rare way are not taken from the usual one.  Four rounded values of a block with infinities, which the conversion has made the largest value: they stay infinities in e5m2 and become NaN in e4m3.
 template <int F8>
-__device__ __forceinline__ uint32_t mend4(uint32_t w, float a, float b, float c, float d)
+__device__ __noinline__ uint32_t mend4(uint32_t w, float a, float b, float c, float d)
 {
     const float v[4] = {a, b, c, d};
 #pragma unroll
@@ -202,10 +269,11 @@ __device__ __forceinline__ uint32_t mend4(uint32_t w, float a, float b, float c,
     }
     return w;
 }
-template <int F8>
-__device__ __forceinline__ uint2 mend8(uint2 r, const float (&v)[8])
+template <int F8, typename B>
+__device__ __forceinline__ uint2 mend8(uint2 r, const B &v, int j)
 {
-    return make_uint2(mend4<F8>(r.x, v[0], v[1], v[2], v[3]), mend4<F8>(r.y, v[4], v[5], v[6], v[7]));
+    const float2 a = v.at(j, 0), b = v.at(j, 1), c = v.at(j, 2), d = v.at(j, 3);
+    return make_uint2(mend4<F8>(r.x, a.x, a.y, b.x, b.y), mend4<F8>(r.y, c.x, c.y, d.x, d.y));
 }
 
 // Largest of sixteen lanes for four values at once: lanes exchange the values that they do not keep, so that five shuffles do, and each lane ends with
@@ -229,14 +297,14 @@ __device__ __forceinline__ uint32_t bytes_of4(uint32_t code)
 }
 // Codes of four blocks of eight values a lane; byte i of *odd: block i has an infinity.  Returns whether any block of the warp has one: that way lies off the
 // usual one (selected by value instead, it took a third of all instructions).
-template <int F8>
-__device__ __forceinline__ bool codes_of4(const float (&v)[4][8], uint32_t *codes, uint32_t *odd)
+template <int F8, typename B>
+__device__ __forceinline__ bool codes_of4(const B &v, uint32_t *codes, uint32_t *odd)
 {
-    float m = max16_of4(amax8(v[0]), amax8(v[1]), amax8(v[2]), amax8(v[3]));
+    float m = max16_of4(v.row_amax(0), v.row_amax(1), v.row_amax(2), v.row_amax(3));
     const bool any = __any_sync(0xffffffffu, !finite(m));
     if (any) {
         *odd = bytes_of4(finite(m) ? 0u : 1u);
-        m = max16_of4(finite_amax8(v[0]), finite_amax8(v[1]), finite_amax8(v[2]), finite_amax8(v[3]));
+        m = max16_of4(finite_row_amax(v, 0), finite_row_amax(v, 1), finite_row_amax(v, 2), finite_row_amax(v, 3));
     }
     *codes = bytes_of4(scale_code<F8>(m));
     return any;
@@ -389,9 +457,13 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
         const int64_t r = row;
         const int c = (int)g * 512 + sub;
         const int64_t word = (int64_t)g * p.rows + r;
-        float v[4][8];
+        constexpr bool AS_LOADED = OP == FP8_PLAIN && TYPE != T_F32;
+        Block4<TYPE, AS_LOADED> v;
 #pragma unroll
-        for (int i = 0; i < 4; i++) to_floats<TYPE>(next[i], v[i]);
+        for (int i = 0; i < 4; i++) {
+            if constexpr (AS_LOADED) v.raw[i] = next[i];
+            else to_floats<TYPE>(next[i], v.v[i]);
+        }
         uint2 h[4];
         uint32_t h_codes = 0;
         if constexpr (OP == FP8_GELU_GRAD) {
@@ -411,11 +483,11 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
             const bool any = codes_of4<T8>(v, &codes, &odd);
             uint2 q[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) q[i] = round8<T8>(v[i], inverse_scale(byte_of(codes, i)));
+            for (int i = 0; i < 4; i++) q[i] = round8<T8>(v, i, inverse_scale(byte_of(codes, i)));
             if (any) {
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (byte_of(odd, i)) q[i] = mend8<T8>(q[i], v[i]);
+                    if (byte_of(odd, i)) q[i] = mend8<T8>(q[i], v, i);
             }
             if (on) {
                 uint8_t *dst = data + r * ld + c;
@@ -431,20 +503,22 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) gelu2<TANH>(v[i][j], v[i][j + 1]);
+                for (int j = 0; j < 8; j += 2) gelu2<TANH>(v.v[i][j], v.v[i][j + 1]);
         } else if constexpr (OP == FP8_GELU_GRAD) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float x[8];
                 ckpt_values(h[i], byte_of(h_codes, i), x);
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) times_gelu_grad2<TANH>(v[i][j], v[i][j + 1], x[j], x[j + 1]);
+                for (int j = 0; j < 8; j += 2) times_gelu_grad2<TANH>(v.v[i][j], v.v[i][j + 1], x[j], x[j + 1]);
             }
         }
-        if (OP != FP8_PLAIN && p.y && on) {
+        if constexpr (OP != FP8_PLAIN) {
+            if (p.y && on) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (c + 128 * i < p.cols) store8<TYPE>(p.y, r * p.ldy, c + 128 * i, p.cols, p.align_y, v[i]);
+                for (int i = 0; i < 4; i++)
+                    if (c + 128 * i < p.cols) store8<TYPE>(p.y, r * p.ldy, c + 128 * i, p.cols, p.align_y, v.v[i]);
+            }
         }
         if (p.data) store(p.data, p.ldd, p.scales, std::integral_constant<int, F8>());
     }
@@ -476,7 +550,8 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
     const int left = WHOLE ? 4 : (int)(p.rows - r0 < 4 ? p.rows - r0 : 4);   // rows that there are, or fewer than one
     const int own_row = (lane >> 2) & 3;                       // the row whose code this lane stores (lanes 0, 4, 8, 12 of a half)
 
-    float v[4][8];
+    constexpr bool AS_LOADED = OP == FP8_PLAIN && TYPE != T_F32;
+    Block4<TYPE, AS_LOADED> v;
     {
         Raw<TYPE> raw[4];
 #pragma unroll
@@ -494,12 +569,13 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            to_floats<TYPE>(raw[j], v[j]);
+            if constexpr (AS_LOADED) v.raw[j] = raw[j];
+            else to_floats<TYPE>(raw[j], v.v[j]);
             if constexpr (OP == FP8_GELU_GRAD) {
                 float h[8];
                 ckpt_values(q[j], codes[j], h);
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) times_gelu_grad2<TANH>(v[j][i], v[j][i + 1], h[i], h[i + 1]);
+                for (int i = 0; i < 8; i += 2) times_gelu_grad2<TANH>(v.v[j][i], v.v[j][i + 1], h[i], h[i + 1]);
             }
         }
     }
@@ -508,11 +584,11 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
         uint8_t *dst = data + r0 * ld + c;
         uint2 q[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) q[j] = round8<T8>(v[j], inverse_scale(byte_of(codes, j)));
+        for (int j = 0; j < 4; j++) q[j] = round8<T8>(v, j, inverse_scale(byte_of(codes, j)));
         if (any) {
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (byte_of(odd, j)) q[j] = mend8<T8>(q[j], v[j]);
+                if (byte_of(odd, j)) q[j] = mend8<T8>(q[j], v, j);
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -528,7 +604,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) gelu2<TANH>(v[j][i], v[j][i + 1]);   // of the zeros that pad: zero
+            for (int i = 0; i < 8; i += 2) gelu2<TANH>(v.v[j][i], v.v[j][i + 1]);   // of the zeros that pad: zero
     }
 
     uint32_t tile_code = 0;
@@ -544,11 +620,11 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
             for (int w = 0; w < 16; w++) m = fmaxf(m, sh.all[w]);
             return m;
         };
-        float m = over_tile(fmaxf(fmaxf(amax8(v[0]), amax8(v[1])), fmaxf(amax8(v[2]), amax8(v[3]))));
+        float m = over_tile(fmaxf(fmaxf(v.row_amax(0), v.row_amax(1)), fmaxf(v.row_amax(2), v.row_amax(3))));
         tile_odd = !finite(m);
         if (tile_odd) {
             __syncthreads();
-            m = over_tile(fmaxf(fmaxf(finite_amax8(v[0]), finite_amax8(v[1])), fmaxf(finite_amax8(v[2]), finite_amax8(v[3]))));
+            m = over_tile(fmaxf(fmaxf(finite_row_amax(v, 0), finite_row_amax(v, 1)), fmaxf(finite_row_amax(v, 2), finite_row_amax(v, 3))));
         }
         tile_code = scale_code<F8>(m);
     }
@@ -591,15 +667,22 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
             };
             float m[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) m[i] = fmaxf(fmaxf(fabsf(v[0][i]), fabsf(v[1][i])), fmaxf(fabsf(v[2][i]), fabsf(v[3][i])));
+            for (int k = 0; k < 4; k++) {
+                const float2 a = v.col_amax(k);
+                m[2 * k] = a.x;
+                m[2 * k + 1] = a.y;
+            }
             put8(m);
             any = column_scales(false);
             if (any) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    m[i] = 0.0f;
+                for (int k = 0; k < 4; k++) {
+                    m[2 * k] = m[2 * k + 1] = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) m[i] = finite(v[j][i]) ? fmaxf(m[i], fabsf(v[j][i])) : m[i];
+                    for (int j = 0; j < 4; j++) {
+                        m[2 * k] = finite_max(m[2 * k], v.at(j, k).x);
+                        m[2 * k + 1] = finite_max(m[2 * k + 1], v.at(j, k).y);
+                    }
                 }
                 put8(m);
                 (void)column_scales(true);
@@ -618,7 +701,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
             for (int i = 0; i < 8; i += 2) {
                 float2 s[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[j] = mul2(make_float2(v[j][i], v[j][i + 1]), make_float2(inv[i], inv[i + 1]));
+                for (int j = 0; j < 4; j++) s[j] = mul2(v.at(j, i / 2), make_float2(inv[i], inv[i + 1]));
                 image[i * 32] = __byte_perm(round2<F8>(s[0].x, s[1].x), round2<F8>(s[2].x, s[3].x), 0x5410);
                 image[i * 32 + 32] = __byte_perm(round2<F8>(s[0].y, s[1].y), round2<F8>(s[2].y, s[3].y), 0x5410);
             }
@@ -626,8 +709,11 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float a = fabsf(inv[i]);
-                uint32_t w = __byte_perm(round2<F8>(v[0][i] * a, v[1][i] * a), round2<F8>(v[2][i] * a, v[3][i] * a), 0x5410);
-                if (inv[i] < 0.0f) w = mend4<F8>(w, v[0][i], v[1][i], v[2][i], v[3][i]);
+                float x[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[j] = i & 1 ? v.at(j, i / 2).y : v.at(j, i / 2).x;
+                uint32_t w = __byte_perm(round2<F8>(x[0] * a, x[1] * a), round2<F8>(x[2] * a, x[3] * a), 0x5410);
+                if (inv[i] < 0.0f) w = mend4<F8>(w, x[0], x[1], x[2], x[3]);
                 image[i * 32] = w;
             }
         }
@@ -648,7 +734,11 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
     if (p.partial) {                       // amax_of has been read by all: the image is complete
         float s[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) s[i] = (v[0][i] + v[1][i]) + (v[2][i] + v[3][i]);
+        for (int k = 0; k < 4; k++) {
+            const float2 a = v.at(0, k), b = v.at(1, k), c = v.at(2, k), d = v.at(3, k);
+            s[2 * k] = (a.x + b.x) + (c.x + d.x);
+            s[2 * k + 1] = (a.y + b.y) + (c.y + d.y);
+        }
         put8(s);
         __syncthreads();
         float a = 0.0f;
@@ -662,7 +752,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
 }
 
 template <int TYPE, int OP, int F8, bool SQUARE, bool TANH>
-__global__ void __launch_bounds__(TILE_THREADS, 2) fp8_tiles_kernel(const Fp8QuantParams p)
+__global__ void __launch_bounds__(TILE_THREADS, OP == FP8_PLAIN && TYPE != T_F32 ? 3 : 2) fp8_tiles_kernel(const Fp8QuantParams p)
 {
     __shared__ TileShared sh;
     grid_dependency_wait();
