@@ -58,13 +58,24 @@ struct Packed {
     void *scale() { return data.defined() ? scales.data_ptr() : nullptr; }
 };
 
+// A tensor on part of a storage, without the dispatcher (a view of a tensor takes 1.5 us).
+Tensor on_storage(const c10::Storage &storage, c10::ScalarType type, int64_t byte_offset, at::IntArrayRef shape, at::IntArrayRef strides)
+{
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(storage), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(byte_offset);      // of types of one byte
+    t.unsafeGetTensorImpl()->set_sizes_and_strides(shape, strides);
+    return t;
+}
+
+// Values and scales in one allocation.
 Packed pack(int64_t rows, int64_t cols, c10::ScalarType f8, const Tensor &like)
 {
     Packed p;
     p.ld = std::max<int64_t>(16, (cols + 15) / 16 * 16);
-    p.data = device_empty({rows, p.ld}, f8, like);
-    if (p.ld != cols) p.data = p.data.narrow(1, 0, cols);
-    p.scales = device_empty({(cols + 511) / 512, rows, 4}, torch::kFloat8_e8m0fnu, like);
+    const int64_t groups = (cols + 511) / 512;
+    const Tensor bytes = device_empty({rows * p.ld + groups * rows * 4}, torch::kUInt8, like);
+    p.data = on_storage(bytes.storage(), f8, 0, {rows, cols}, {p.ld, 1});
+    p.scales = on_storage(bytes.storage(), torch::kFloat8_e8m0fnu, rows * p.ld, {groups, rows, 4}, {rows * 4, 4, 1});
     return p;
 }
 
