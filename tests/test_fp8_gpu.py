@@ -553,6 +553,47 @@ def test_training_step_with_modules():
     assert net[0].weight is weight and not torch.equal(ff(net(x)), first)
 
 
+def decoder(layers=2):
+    from venom_b200 import e2e_gpt
+    torch.manual_seed(3)
+    with torch.device("cuda"):
+        return e2e_gpt.build_block(layers, 256, 4, 1024).half()
+
+
+def test_decoder_block_in_8_bits():
+    """The command's block as a user runs it: forward frozen and trainable, a training step's gradients against the dense block's."""
+    from venom_b200 import e2e_gpt
+    dense = decoder()
+    x, dy = matrix(2 * 96, 256, 1, torch.float16, 0.0).reshape(2, 96, 256), matrix(2 * 96, 256, 2, torch.float16, 0.0).reshape(2, 96, 256)
+    with torch.no_grad():
+        want = dense(x)
+        frozen, trainable = e2e_gpt.to_fp8(dense), e2e_gpt.to_fp8(dense, trainable=True)
+        got = frozen(x)
+        assert torch.equal(got, trainable(x))
+    # every linear's operands are off by 2^-4 at most and 2^-5.8 of a standard deviation on average (uniform over a step), two of them, in eight linears whose results
+    # are added to the residual stream: 2^-5.8 sqrt(2 8) = 2^-3.8 of it if they were all as large as the stream
+    assert (got.float() - want.float()).norm() <= 2.0 ** -3.8 * want.float().norm()
+    # gradients: three operands more on their way, so below 2^-3 of their norm by the same count; a cosine of 0.9 would take 0.43
+    g, w = e2e_gpt.train_step(trainable, x, dy), e2e_gpt.train_step(dense, x, dy)
+    names = [n for n, _ in trainable.named_parameters()]
+    assert len(g) == len(w) == len(names) + 1 and {id(p) for p in trainable.parameters()} == {id(p) for p in dense.parameters()}
+    order = {id(p): i for i, p in enumerate(dense.parameters())}
+    for p, got_p in zip(trainable.parameters(), g[1:]):
+        ref = w[1 + order[id(p)]].float()
+        assert got_p.isfinite().all() and torch.nn.functional.cosine_similarity(got_p.float().flatten(), ref.flatten(), dim=0) > 0.9
+    assert torch.nn.functional.cosine_similarity(g[0].float().flatten(), w[0].float().flatten(), dim=0) > 0.9
+
+
+def test_decoder_commands_run(capsys):
+    from venom_b200 import e2e_gpt
+    try:
+        e2e_gpt.main(["--layers", "1", "--hidden", "256", "--heads", "4", "--ffn", "1024", "--batch", "2", "--seq", "64", "--repeats", "2", "-v", "64", "-m", "8", "--fp8", "--train"])
+    finally:
+        torch.set_grad_enabled(True)
+    out = capsys.readouterr().out
+    assert "fp8 forward," in out and "fp8 training step," in out and "dense training step," in out
+
+
 # ---- streams, graphs, devices ----
 
 def test_calls_on_another_stream():

@@ -128,6 +128,7 @@ template <int TYPE, bool AS_LOADED>
 struct Block4;
 template <int TYPE>
 struct Block4<TYPE, true> {
+    static constexpr bool SHORT = true;        // of registers
     Raw<TYPE> raw[4];
     __device__ __forceinline__ float2 at(int j, int k) const { return pair_of<TYPE>(raw[j], k); }
     __device__ __forceinline__ float row_amax(int j) const
@@ -143,6 +144,7 @@ struct Block4<TYPE, true> {
 };
 template <int TYPE>
 struct Block4<TYPE, false> {
+    static constexpr bool SHORT = false;
     float v[4][8];
     __device__ __forceinline__ float2 at(int j, int k) const { return make_float2(v[j][2 * k], v[j][2 * k + 1]); }
     __device__ __forceinline__ float row_amax(int j) const
@@ -257,9 +259,9 @@ __device__ __forceinline__ uint2 round8(const B &v, int j, float inv)
     }
     return make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
 }
-// A call, so that the registers of this rare way are not taken from the usual one.  Four rounded values of a block with infinities, which the conversion has made the largest value: they stay infinities in e5m2 and become NaN in e4m3.
+// Four rounded values of a block with infinities, which the conversion has made the largest value: they stay infinities in e5m2 and become NaN in e4m3.
 template <int F8>
-__device__ __noinline__ uint32_t mend4(uint32_t w, float a, float b, float c, float d)
+__device__ __forceinline__ uint32_t mend4_here(uint32_t w, float a, float b, float c, float d)
 {
     const float v[4] = {a, b, c, d};
 #pragma unroll
@@ -269,11 +271,20 @@ __device__ __noinline__ uint32_t mend4(uint32_t w, float a, float b, float c, fl
     }
     return w;
 }
+// The same as a call: where registers are short (three CTAs an SM) this rare way shall take none from the usual one.
+template <int F8>
+__device__ __noinline__ uint32_t mend4_call(uint32_t w, float a, float b, float c, float d) { return mend4_here<F8>(w, a, b, c, d); }
+template <int F8, bool CALL>
+__device__ __forceinline__ uint32_t mend4(uint32_t w, float a, float b, float c, float d)
+{
+    if constexpr (CALL) return mend4_call<F8>(w, a, b, c, d);
+    else return mend4_here<F8>(w, a, b, c, d);
+}
 template <int F8, typename B>
 __device__ __forceinline__ uint2 mend8(uint2 r, const B &v, int j)
 {
     const float2 a = v.at(j, 0), b = v.at(j, 1), c = v.at(j, 2), d = v.at(j, 3);
-    return make_uint2(mend4<F8>(r.x, a.x, a.y, b.x, b.y), mend4<F8>(r.y, c.x, c.y, d.x, d.y));
+    return make_uint2(mend4<F8, B::SHORT>(r.x, a.x, a.y, b.x, b.y), mend4<F8, B::SHORT>(r.y, c.x, c.y, d.x, d.y));
 }
 
 // Largest of sixteen lanes for four values at once: lanes exchange the values that they do not keep, so that five shuffles do, and each lane ends with
@@ -350,17 +361,18 @@ __device__ __forceinline__ float near(float x) { return max_nan(min_nan(x, 64.0f
 
 // The exact form by a published approximation of erfc (Abramowitz and Stegun, 7.1.26, |error| <= 1.5e-7): with t = 1 / (1 + p |z|), z = x / sqrt 2,
 // erfc |z| = (a1 t + .. + a5 t^5) exp(-z^2).  The exponential is the density's as well, which the derivative needs, so one exponential and one reciprocal
-// give both.  With h = erfc |z| / 2, gelu(x) = max(x, 0) - |x| h: no cancellation in the tail of negative x.  a = |x|, cut off.
+// give both.  With h = erfc |z| / 2, gelu(x) = max(x, 0) - |x| h: no cancellation in the tail of negative x.  a = |x|, cut off; the result is S h, S = 1 or -1.
+template <int S>
 __device__ __forceinline__ float2 half_erfc(float2 a, float2 *e)
 {
     const float2 d = fma2(both(0.3275911f * 0.70710678118654752f), a, both(1.0f));
     const float2 t = make_float2(fast_rcp(d.x), fast_rcp(d.y));
     const float2 q = mul2(mul2(a, a), both(-0.72134752044448170f));
     *e = make_float2(fast_exp2(q.x), fast_exp2(q.y));
-    float2 poly = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
-    poly = fma2(poly, t, both(0.5f * 1.421413741f));
-    poly = fma2(poly, t, both(0.5f * -0.284496736f));
-    poly = fma2(poly, t, both(0.5f * 0.254829592f));
+    float2 poly = fma2(both(S * 0.5f * 1.061405429f), t, both(S * 0.5f * -1.453152027f));
+    poly = fma2(poly, t, both(S * 0.5f * 1.421413741f));
+    poly = fma2(poly, t, both(S * 0.5f * -0.284496736f));
+    poly = fma2(poly, t, both(S * 0.5f * 0.254829592f));
     return mul2(mul2(poly, t), *e);
 }
 // The tanh form: (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3); x cut off.
@@ -379,8 +391,8 @@ __device__ __forceinline__ void gelu2(float &x, float &y)
     } else {
         const float2 a = make_float2(min_nan(fabsf(x), 64.0f), min_nan(fabsf(y), 64.0f));
         float2 e;
-        const float2 h = half_erfc(a, &e);
-        r = fma2(make_float2(-a.x, -a.y), h, make_float2(max_nan(x, 0.0f), max_nan(y, 0.0f)));
+        const float2 h = half_erfc<-1>(a, &e);
+        r = fma2(a, h, make_float2(max_nan(x, 0.0f), max_nan(y, 0.0f)));
     }
     x = r.x;
     y = r.y;
@@ -397,7 +409,7 @@ __device__ __forceinline__ void times_gelu_grad2(float &x, float &y, float a, fl
         g = fma2(mul2(mul2(n, s), fma2(both(-1.0f), s, both(1.0f))), du, s);
     } else {
         float2 e;
-        const float2 h = half_erfc(make_float2(fabsf(n.x), fabsf(n.y)), &e);
+        const float2 h = half_erfc<1>(make_float2(fabsf(n.x), fabsf(n.y)), &e);
         const float2 far = make_float2(n.x < 0.0f ? h.x : 1.0f - h.x, n.y < 0.0f ? h.y : 1.0f - h.y);
         g = fma2(n, mul2(e, both(0.39894228040143268f)), far);
     }
@@ -713,7 +725,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
 #pragma unroll
                 for (int j = 0; j < 4; j++) x[j] = i & 1 ? v.at(j, i / 2).y : v.at(j, i / 2).x;
                 uint32_t w = __byte_perm(round2<F8>(x[0] * a, x[1] * a), round2<F8>(x[2] * a, x[3] * a), 0x5410);
-                if (inv[i] < 0.0f) w = mend4<F8>(w, x[0], x[1], x[2], x[3]);
+                if (inv[i] < 0.0f) w = mend4<F8, AS_LOADED>(w, x[0], x[1], x[2], x[3]);
                 image[i * 32] = w;
             }
         }

@@ -7,8 +7,9 @@ three differences that the missing network access and the missing `sten` depende
   * linears are pruned by magnitude on the GPU (the path the reference keeps commented out) unless
     --fixed-mask asks for the shipped fixed pattern;
   * timing uses CUDA events around each forward pass instead of timeit without synchronisation.
+--fp8 times the encoder with every linear kept whole in block-scaled 8 bits (venom_b200.fp8) as well, on a line of its own.
 
-    python -m venom_b200.e2e_bert -m 8 -n 2 -v 64 [--layers 24] [--batch 32] [--seq 512] [--repeats 10]
+    python -m venom_b200.e2e_bert -m 8 -n 2 -v 64 [--layers 24] [--batch 32] [--seq 512] [--repeats 10] [--fp8]
 """
 import argparse
 import statistics
@@ -68,6 +69,7 @@ def main(argv=None):
     ap.add_argument("--seq", type=int, default=512)
     ap.add_argument("--repeats", type=int, default=10)
     ap.add_argument("--fixed-mask", action="store_true")
+    ap.add_argument("--fp8", action="store_true", help="also time the encoder with its weights in 8 bits")
     args = ap.parse_args(argv)
     if not torch.cuda.is_available():
         raise SystemExit("needs a CUDA device (there is no CPU path)")
@@ -80,8 +82,15 @@ def main(argv=None):
     ids = torch.randint(0, 30522, (args.batch, args.seq), device="cuda")
     d_ms = time_forward(dense, ids, args.repeats)
     s_ms = time_forward(sparse, ids, args.repeats)
+    f_ms = None
+    if args.fp8:
+        from .fp8 import linear_to_fp8
+        linear_to_fp8(dense.encoder)
+        f_ms = time_forward(dense, ids, args.repeats)
     report_time("dense", d_ms, args.n, args.m, args.v)
     report_time("n:m", s_ms, args.n, args.m, args.v)
+    if f_ms:
+        print("fp8 forward,%s,%s,%d" % (statistics.mean(f_ms), statistics.median(f_ms), len(f_ms)))
     tokens = args.batch * args.seq
     print("# %d linears replaced; dense %.0f tokens/s, %d:%d:%d %.0f tokens/s, speed-up %.2fx" % (
         replaced, tokens / statistics.median(d_ms) * 1e3, args.v, args.n, args.m, tokens / statistics.median(s_ms) * 1e3,

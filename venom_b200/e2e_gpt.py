@@ -11,10 +11,12 @@ replaced by SrnmSpmm, output lines `0,n,m,v,mean,median,std,len` in milliseconds
     batch / world_size whole sequences through the same replicated sparse weights (no collective inside the
     layers: attention never crosses a sequence) and the final hidden states are all-gathered once, so that every
     rank ends with the full [batch, seq, hidden] output, as a following un-sharded layer would need;
-  * timing uses CUDA events, the maximum over ranks is reported.
+  * timing uses CUDA events, the maximum over ranks is reported;
+  * --fp8 times the block with every weight kept whole in block-scaled 8 bits (venom_b200.fp8) as well, --train a training step (forward and
+    backward) of the dense block and of the 8-bit one, whose kept activations are 8 bits too; lines of their own, the name first.
 
     python -m venom_b200.e2e_gpt -m 16 -n 2 -v 128 [--layers 4] [--hidden 12288] [--heads 96] [--ffn 49152]
-           [--batch 8] [--seq 2048] [--repeats 5] [--fixed-mask]
+           [--batch 8] [--seq 2048] [--repeats 5] [--fixed-mask] [--fp8] [--train]
     python -m torch.distributed.run --nproc-per-node 2 --master-addr 127.0.0.1 -m venom_b200.e2e_gpt ...
 """
 import argparse
@@ -45,11 +47,44 @@ class DecoderLayer(torch.nn.Module):
         q, k, v = (t.reshape(b, s, self.heads, h // self.heads).transpose(1, 2) for t in (q, k, v))
         a = F.scaled_dot_product_attention(q, k, v, is_causal=True).transpose(1, 2).reshape(b, s, h)
         x = x + self.c_proj(a)
-        return x + self.c_fc_proj(F.gelu(self.c_fc(self.ln_2(x))))
+        return x + self.feed_forward(self.ln_2(x))
+
+    def feed_forward(self, x):
+        return self.c_fc_proj(F.gelu(self.c_fc(x)))
+
+
+class Fp8DecoderLayer(DecoderLayer):
+    """A decoder layer with its linears in 8 bits; norms, and the parameters where `trainable`, are the original's."""
+
+    def __init__(self, layer, trainable=False):
+        from .fp8 import Fp8Linear, Fp8Mlp
+        torch.nn.Module.__init__(self)
+        self.heads, self.ln_1, self.ln_2 = layer.heads, layer.ln_1, layer.ln_2
+        self.c_attn, self.c_proj = Fp8Linear(layer.c_attn, trainable), Fp8Linear(layer.c_proj, trainable)
+        self.mlp = Fp8Mlp(layer.c_fc, layer.c_fc_proj, trainable=trainable)
+
+    def feed_forward(self, x):
+        return self.mlp(x)
 
 
 def build_block(layers, hidden, heads, ffn):
     return torch.nn.Sequential(*[DecoderLayer(hidden, heads, ffn) for _ in range(layers)]).eval()
+
+
+def to_fp8(block, trainable=False):
+    """The block with its linears in 8 bits; the dense one stays."""
+    return torch.nn.Sequential(*[Fp8DecoderLayer(layer, trainable) for layer in block]).train(block.training)
+
+
+def train_step(block, x, dy):
+    """Gradients of every parameter and of x for the gradient dy of the result."""
+    with torch.enable_grad():
+        x = x.detach().requires_grad_()
+        block(x).backward(dy)
+    grads = [x.grad] + [p.grad for p in block.parameters()]
+    for p in block.parameters():
+        p.grad = None
+    return grads
 
 
 def sparsify(block, n, m, v, magnitude):
@@ -100,9 +135,13 @@ def main(argv=None):
     ap.add_argument("--peer-store", action="store_true",
                     help="with --gather-every-layer: no exchange step, every sparse linear stores its output tiles into all ranks' buffers "
                          "(vnm_mgpu_spmm_gathered_p2p) instead of the chunked NCCL exchange")
+    ap.add_argument("--fp8", action="store_true", help="also time the block with its weights in 8 bits")
+    ap.add_argument("--train", action="store_true", help="also time a training step, dense and in 8 bits")
     args = ap.parse_args(argv)
     if not torch.cuda.is_available():
         raise SystemExit("needs a CUDA device (there is no CPU path)")
+    if (args.fp8 or args.train) and args.gather_every_layer:
+        raise SystemExit("--fp8 and --train do not go with --gather-every-layer")
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))
     local = int(os.environ.get("LOCAL_RANK", "0"))
@@ -185,7 +224,7 @@ def main(argv=None):
     if args.gather_every_layer and world > 1:
         install_gather_hooks()
 
-    def step():
+    def step(block=block):
         y = block(x)
         if world > 1:
             dist.all_gather_into_tensor(gathered, y.contiguous())   # shards are contiguous blocks of sequences
@@ -201,6 +240,18 @@ def main(argv=None):
     d_ms = None
     if not args.skip_dense:
         d_ms = max_over_ranks(time_forward(step, args.repeats))
+    f_ms = t_ms = tf_ms = None
+    if args.fp8:
+        eight = to_fp8(block)
+        f_ms = max_over_ranks(time_forward(lambda: step(eight), args.repeats))
+        del eight
+    if args.train:
+        dy = torch.randn(x.shape, device="cuda", generator=g).mul_(1e-3).half()
+        if not args.skip_dense:
+            t_ms = max_over_ranks(time_forward(lambda: train_step(block, x, dy), args.repeats))
+        eight = to_fp8(block, trainable=True)
+        tf_ms = max_over_ranks(time_forward(lambda: train_step(eight, x, dy), args.repeats))
+        del eight, dy
     replaced = sparsify(block, args.n, args.m, args.v, not args.fixed_mask)
     torch.cuda.empty_cache()
     if args.gather_every_layer and world > 1:
@@ -214,6 +265,9 @@ def main(argv=None):
         if d_ms:
             line("0,0,", d_ms)
         line("%d,%d," % (args.n, args.m), s_ms)
+        for name, ms in (("fp8 forward", f_ms), ("dense training step", t_ms), ("fp8 training step", tf_ms)):
+            if ms:
+                print("%s,%s,%s,%d" % (name, statistics.mean(ms), statistics.median(ms), len(ms)))
         msg = "# %d GPUs%s, %d linears replaced (%s mask); %d:%d:%d %.0f tokens/s" % (
             world, (", every linear's output replicated by peer stores" if args.peer_store else ", all-gather after every linear") if args.gather_every_layer and world > 1 else "", replaced,
             "fixed" if args.fixed_mask else "magnitude", args.v, args.n, args.m, tokens / statistics.median(s_ms) * 1e3)
