@@ -4,7 +4,11 @@ Bounds: a value rounded to 8 bits is compared bit for bit (its scale is a power 
 is off by at most K 2^-23 of the sum of magnitudes (a unit in the last place for each addition, whatever the order), and rounding to the result's type adds half
 a step, eps / 2."""
 import copy
+import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -199,6 +203,80 @@ def test_matmul(M, N, K, types, bias):
     check_product(got, value64(a.dequantize().double(), types[0]), value64(b.dequantize().double(), types[1]), bias)
     assert torch.equal(got, fp8.matmul(a, b, bias, TYPES[types[2]])), "two calls differ"
     assert fp8.device_status() == 0
+
+
+# (columns of a pair tile, rows in whole pieces, at least two tiles for every pair of SMs, 32-bit results, bias): a shape that takes that instance
+INSTANCES = {
+    (192, False, False, False, False): (5054, 129, 628), (192, False, False, True, False): (4787, 135, 626), (192, False, True, False, False): (2324, 3678, 602),
+    (192, False, True, True, False): (5406, 1562, 611), (192, True, False, False, False): (2656, 136, 730), (192, True, False, True, True): (2651, 140, 640),
+    (192, True, True, False, False): (2361, 3632, 628), (192, True, True, True, True): (1555, 5552, 619), (224, False, False, False, True): (525, 4729, 652),
+    (224, False, False, True, True): (521, 4630, 615), (224, False, True, False, False): (1580, 5980, 610), (224, False, True, True, True): (2049, 4681, 604),
+    (224, True, False, False, False): (524, 4968, 644), (224, True, False, True, True): (559, 4964, 614), (224, True, True, False, True): (1797, 5424, 615),
+    (224, True, True, True, True): (1794, 5396, 601), (240, False, False, False, False): (4657, 674, 605), (240, False, False, True, False): (576, 5386, 620),
+    (240, False, True, False, True): (3358, 3439, 602), (240, False, True, True, True): (2060, 5487, 600), (240, True, False, False, False): (519, 5680, 632),
+    (240, True, False, True, True): (563, 5508, 613), (240, True, True, False, False): (2909, 4072, 619), (240, True, True, True, True): (2113, 5428, 604),
+    (256, False, False, False, False): (513, 5783, 660), (256, False, False, True, True): (544, 5938, 622), (256, False, True, False, True): (2627, 5026, 602),
+    (256, False, True, True, False): (2617, 5119, 613), (256, True, False, False, False): (807, 4472, 630), (256, True, False, True, False): (542, 5996, 645),
+    (256, True, True, False, False): (2306, 5576, 603), (256, True, True, True, True): (2338, 5576, 604)}
+
+
+def plan_of(M, N, K, dtype, bias):
+    v = [ctypes.c_int() for _ in range(4)]
+    whole = N * torch.finfo(dtype).bits // 8 % 16 == 0
+    assert capi.lib().vnm_fp8_matmul_config(M, N, K, 0 if dtype == torch.float32 else 1, whole, bias, *[ctypes.byref(x) for x in v]) == 0
+    return [x.value for x in v]
+
+
+@pytest.mark.parametrize("instance", list(INSTANCES), ids=lambda i: "-".join(map(str, i)))
+def test_matmul_pair_instances(instance):
+    width, _, _, wide, with_bias = instance
+    M, N, K = INSTANCES[instance]
+    for dtype in (torch.float32,) if wide else (torch.float16, torch.bfloat16):
+        assert plan_of(M, N, K, dtype, with_bias)[:2] == [256, width]
+        a, b = fp8.quantize(matrix(M, K, M, spread=0.5)), fp8.quantize(matrix(N, K, N, spread=0.3), E5M2)
+        bias = vector(N, 5, dtype) if with_bias else None
+        got = fp8.matmul(a, b, bias, dtype)
+        check_product(got, a.dequantize().double(), b.dequantize().double(), bias)
+        assert torch.equal(got, fp8.matmul(a, b, bias, dtype)), "two calls differ"
+    assert fp8.device_status() == 0
+
+
+@pytest.mark.parametrize("M,N,K,want", [(62, 10, 25, (16, 1)), (623, 8, 1252, (16, 2)), (1, 855, 720, (16, 4)), (1, 115, 1123, (16, 8)), (2496, 171, 16, (32, 1)), (1631, 8, 2666, (32, 2)),
+                                        (762, 9, 4578, (32, 4)), (399, 11, 6782, (32, 8)), (1912, 523, 20, (64, 1)), (2386, 8, 6084, (64, 2)), (1857, 8, 6344, (64, 4)), (2653, 1699, 17, (128, 1))])
+def test_matmul_one_sm_instances(M, N, K, want):
+    dtype = torch.float32 if want == (128, 1) else torch.float16
+    tile_m, tile_n, split, _ = plan_of(M, N, K, dtype, False)
+    assert (tile_m, split) == want and tile_n == 128
+    a, b = fp8.quantize(matrix(M, K, M, spread=0.5)), fp8.quantize(matrix(N, K, N, spread=0.3), E5M2)
+    check_product(fp8.matmul(a, b, None, dtype), a.dequantize().double(), b.dequantize().double())
+    assert fp8.device_status() == 0
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [(70000, 40008, 136, torch.float16), (40007, 33001, 40, torch.float32)])
+def test_matmul_results_past_32_bits(M, N, K, dtype):
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    a, b = fp8.quantize(matrix(M, K, 1, spread=0.3)), fp8.quantize(matrix(N, K, 2, spread=0.3))
+    got = fp8.matmul(a, b, None, dtype)
+    rows = torch.tensor([0, 1, 255, 256, M // 2, M - 257, M - 2, M - 1], device="cuda")
+    check_product(got[rows], a.dequantize()[rows].double(), b.dequantize().double())
+
+
+def test_matmul_operands_past_32_bits():
+    """A weight of 4.4 GB."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    N, K = 70000, 62992
+    data = torch.zeros((N, K), dtype=torch.uint8, device="cuda")
+    scales = torch.full((-(-K // 512), N, 4), 127, dtype=torch.uint8, device="cuda")
+    last = matrix(300, K, 3, spread=0.3)
+    q = fp8.quantize(last)
+    data[-300:] = q.data.view(torch.uint8)
+    scales[:, -300:] = q.scales.view(torch.uint8)
+    x = fp8.quantize(matrix(5, K, 4))
+    got = fp8.matmul(x, fp8.BlockFp8(data.view(E4M3), scales.view(torch.float8_e8m0fnu)), dtype=torch.float32)
+    assert bool((got[:, :-300] == 0).all())
+    check_product(got[:, -300:], x.dequantize().double(), q.dequantize().double())
 
 
 def test_matmul_scales_of_every_size():
@@ -521,8 +599,7 @@ def test_frozen_layers():
         other.load_state_dict({k: v.clone() for k, v in q.state_dict().items()}, assign=True)
         assert torch.equal(other(x), y)
         assert torch.equal(q.half()(x), y)
-    with pytest.raises(capi.VenomError, match="trainable"):
-        q(x)          # the bias wants a gradient
+    assert torch.equal(q(x), y) and not q(x).requires_grad      # the bias is as frozen as the weight
     with pytest.raises(capi.VenomError, match="trainable"):
         q(leaf(x))
 
@@ -653,3 +730,44 @@ def test_captured_training_step():
     torch.cuda.synchronize()
     for out in outs:
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first 8-bit calls are captured: what a device needs once is set up then."""
+    code = """
+import torch
+from venom_b200 import fp8
+x, w = torch.randn(300, 512, device="cuda").half(), torch.randn(700, 512, device="cuda").half()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = fp8.linear(x, w)
+    t = fp8.quantize(x, both=True)[1]
+g.replay()
+assert torch.equal(y, fp8.linear(x, w)) and torch.equal(t.dequantize(), fp8.quantize(x, both=True)[1].dequantize())
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
+def test_calls_from_two_threads():
+    import threading
+    x, w = matrix(260, 1024, 1, torch.float16), matrix(520, 1024, 2, torch.float16)
+    want = fp8.linear(x, w)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(50):
+                if not torch.equal(fp8.linear(x, w), want):
+                    bad.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

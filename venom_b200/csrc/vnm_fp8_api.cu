@@ -103,6 +103,12 @@ int device_ready(int **status)
     std::lock_guard<std::mutex> lock(g_mutex);
     Device &d = g_devices[dev];
     if (!d.ready) {
+        // settings of the kernels are not work that a capture on this thread must not miss
+        struct Relaxed {
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            Relaxed() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
+            ~Relaxed() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
+        } relaxed;
         if ((e = fp8_small_init()) != cudaSuccess || (e = fp8_pair_init()) != cudaSuccess) return done(e, "cudaFuncSetAttribute(max dynamic shared memory)");
         void *at = nullptr;
         if ((e = cudaGetSymbolAddress(&at, g_status)) != cudaSuccess) return done(e, "cudaGetSymbolAddress");

@@ -150,15 +150,20 @@ class _Held(torch.nn.Module):
             self._views[name] = (cols, data, q)
         return q
 
-    def _refuse_gradients(self, x, *others):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x,) + others):
+    def _refuse_gradients(self, x):
+        if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
             raise VenomError("%s holds a frozen weight: build it with trainable=True for gradients" % type(self).__name__)
+
+
+def _frozen(bias):
+    """The same values as a parameter that wants no gradient."""
+    return None if bias is None else torch.nn.Parameter(bias.detach(), requires_grad=False)
 
 
 class Fp8Linear(_Held):
     """Drop-in replacement of torch.nn.Linear whose products run in 8 bits.
 
-    trainable=False: the weight is quantised once and held in 8 bits only, like SrnmSpmm's, for inference.  trainable=True: the layer keeps the parameters
+    trainable=False: the weight is quantised once and held in 8 bits only, like SrnmSpmm's, for inference; an input that wants a gradient is refused.  trainable=True: the layer keeps the parameters
     of `original`, quantises the weight in every call and is differentiable (see linear)."""
 
     def __init__(self, original, trainable=False, grad_dtype=E4M3):
@@ -167,7 +172,7 @@ class Fp8Linear(_Held):
         _check_grad_dtype(grad_dtype, "Fp8Linear")
         self.in_features, self.out_features = original.in_features, original.out_features
         self.trainable, self.grad_dtype = bool(trainable), grad_dtype
-        self.bias = original.bias
+        self.bias = original.bias if self.trainable else _frozen(original.bias)
         if self.trainable:
             self.weight = original.weight
         else:
@@ -177,7 +182,7 @@ class Fp8Linear(_Held):
     def forward(self, input):
         if self.trainable:
             return linear(input, self.weight, self.bias, self.grad_dtype)
-        self._refuse_gradients(input, self.bias)
+        self._refuse_gradients(input)
         _check_input(input, "Fp8Linear")
         flat = _flat(input)
         q = quantize(flat)
@@ -200,7 +205,7 @@ class Fp8Mlp(_Held):
         self.tanh_form, self.approximate = _tanh_form(approximate, "Fp8Mlp"), approximate
         self.trainable, self.grad_dtype = bool(trainable), grad_dtype
         self.out_features = proj.out_features
-        self.fc_bias, self.proj_bias = fc.bias, proj.bias
+        self.fc_bias, self.proj_bias = (fc.bias, proj.bias) if self.trainable else (_frozen(fc.bias), _frozen(proj.bias))
         if self.trainable:
             self.fc_weight, self.proj_weight = fc.weight, proj.weight
         else:
@@ -212,7 +217,7 @@ class Fp8Mlp(_Held):
     def forward(self, input):
         if self.trainable:
             return mlp(input, self.fc_weight, self.fc_bias, self.proj_weight, self.proj_bias, self.approximate, self.grad_dtype)
-        self._refuse_gradients(input, self.fc_bias, self.proj_bias)
+        self._refuse_gradients(input)
         _check_input(input, "Fp8Mlp")
         h = matmul(quantize(_flat(input)), self._weight("fc"), self.fc_bias, input.dtype)
         _, a, sa, _, _, _, _ = _call("fp8_gelu", h, self.tanh_form, False, True, False, False)
