@@ -5,8 +5,11 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include "../../include/venom_b200.h"
@@ -426,16 +429,74 @@ int64_t device_status()
     return status;
 }
 
+// fp8.quantize() and fp8.matmul() as plain C functions of the module: at decoding sizes they take as long as the host takes to queue them, and pybind11's conversions of
+// arguments and results were 1 us of 5.4.
+const Tensor &tensor_of(PyObject *o)
+{
+    TORCH_CHECK_TYPE(THPVariable_Check(o), "expected a tensor");
+    return THPVariable_Unpack(o);
+}
+c10::ScalarType dtype_of(PyObject *o)
+{
+    TORCH_CHECK_TYPE(THPDtype_Check(o), "expected a dtype");
+    return reinterpret_cast<THPDtype *>(o)->scalar_type;
+}
+
+// (x, dtype, square, both) -> (data, scales) or (data, scales, data_t, scales_t)
+PyObject *py_quantize(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 4, "quantize(x, dtype, square, both)");
+    const Tensor &x = tensor_of(args[0]);
+    const c10::ScalarType f8 = dtype_of(args[1]);
+    const bool square = args[2] == Py_True, both = args[3] == Py_True;
+    Quantized q;
+    {
+        pybind11::gil_scoped_release no_gil;
+        q = quantize(x, f8, square, true, both, c10::nullopt);
+    }
+    PyObject *out = PyTuple_New(both ? 4 : 2);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(*std::get<0>(q))));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(*std::get<1>(q))));
+    if (both) {
+        PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::move(*std::get<2>(q))));
+        PyTuple_SET_ITEM(out, 3, THPVariable_Wrap(std::move(*std::get<3>(q))));
+    }
+    return out;
+    END_HANDLE_TH_ERRORS
+}
+
+// (a, a's scales, b, b's scales, bias or None, dtype) -> a b^T (+ bias)
+PyObject *py_matmul(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 6, "matmul(a, a_scales, b, b_scales, bias, dtype)");
+    const Tensor &a = tensor_of(args[0]), &sa = tensor_of(args[1]), &b = tensor_of(args[2]), &sb = tensor_of(args[3]);
+    const OptTensor bias = args[4] == Py_None ? c10::nullopt : OptTensor(tensor_of(args[4]));
+    const c10::ScalarType type = dtype_of(args[5]);
+    Tensor out;
+    {
+        pybind11::gil_scoped_release no_gil;
+        out = matmul(a, sa, b, sb, bias, type);
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef fast_calls[] = {
+    {"fp8_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&py_quantize)), METH_FASTCALL, "vnm_fp8_quantize with its allocations"},
+    {"fp8_matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&py_matmul)), METH_FASTCALL, "vnm_fp8_matmul with its allocation"},
+    {nullptr, nullptr, 0, nullptr}};
+
 }  // namespace
 
 void define_fp8(pybind11::module &mod)
 {
     using release = pybind11::call_guard<pybind11::gil_scoped_release>;
-    mod.def("fp8_quantize", &quantize, "vnm_fp8_quantize with its allocations", release());
+    if (PyModule_AddFunctions(mod.ptr(), fast_calls) != 0) throw pybind11::error_already_set();
     mod.def("fp8_dequantize", &dequantize, "vnm_fp8_dequantize with its allocation", release());
-    mod.def("fp8_matmul", &matmul, "vnm_fp8_matmul with its allocation", release());
     mod.def("fp8_gelu", &gelu, "vnm_fp8_gelu with its allocations", release());
-    mod.def("fp8_gelu_grad", &gelu_grad, "vnm_fp8_gelu_grad with its allocations", release());
     mod.def("fp8_linear", &linear, "A differentiable linear layer in 8 bits", release());
     mod.def("fp8_gelu8", &gelu8, "GELU with an 8-bit checkpoint for its gradient", release());
     mod.def("fp8_mlp", &mlp, "A differentiable feed-forward block in 8 bits", release());

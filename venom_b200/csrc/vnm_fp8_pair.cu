@@ -175,8 +175,9 @@ __device__ __forceinline__ void store_part(uint8_t *dst, const uint32_t (&y)[4],
     }
 }
 
-// `part`: 0 the first 128 columns of a tile, 1 the rest; WHOLE: rows lie on 16-byte boundaries and have whole pieces.
-template <int TYPE, bool BIAS, bool WHOLE, typename Release>
+// `part`: 0 the first 128 columns of a tile, 1 the rest; WHOLE: rows lie on 16-byte boundaries and have whole pieces.  HOLD (128 columns of 16 bits): all of them are
+// rounded into registers before the first is stored, where the next tile's MMAs wait for this accumulator.
+template <int TYPE, bool BIAS, bool WHOLE, bool HOLD, typename Release>
 __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n0, int cols, int part, uint4 *stage, const float4 *bias, const Fp8MatmulParams &p, Release release)
 {
     constexpr int SIZE = TYPE == T_F32 ? 4 : 2, WIDTH = 128 / SIZE, PIECES = TYPE == T_F32 ? 8 : 4;   // pieces of 32 columns
@@ -200,17 +201,35 @@ __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n
     }
     uint32_t v[32];
     tc_ld_32x32b_x32(tacc, v);
-#pragma unroll 1
-    for (int c0 = 0; c0 < cols; c0 += WIDTH, out += 128) {
+    uint32_t held[HOLD ? 64 : 1];
+    if constexpr (HOLD) {
+#pragma unroll
+        for (int h = 0; h < 4; h++) {
+            wait_for(v);
+            uint32_t word[16];
+            round32<TYPE, BIAS>(v, bias + 8 * h, word);
+            if (h < 3) tc_ld_32x32b_x32(tacc + (uint32_t)(32 * (h + 1)), v);
+            else release();
+#pragma unroll
+            for (int i = 0; i < 16; i++) held[16 * h + i] = word[i];
+        }
+    }
+#pragma unroll(HOLD ? 2 : 1)
+    for (int c0 = 0; c0 < (HOLD ? 128 : cols); c0 += WIDTH, out += 128) {
         // 32 columns at a time, the next ones on their way while these are rounded
 #pragma unroll
         for (int h = 0; h < WIDTH / 32; h++) {
-            wait_for(v);
             uint32_t word[TYPE == T_F32 ? 32 : 16];
-            round32<TYPE, BIAS>(v, bias + c0 / 4 + 8 * h, word);
-            const int c1 = c0 + 32 * (h + 1);
-            if (c1 < cols) tc_ld_32x32b_x32(tacc + (uint32_t)c1, v);
-            else if (c1 - 32 < cols) release();                    // once: behind the last columns that belong to the tile
+            if constexpr (HOLD) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) word[i] = held[c0 / 2 + 16 * h + i];
+            } else {
+                wait_for(v);
+                round32<TYPE, BIAS>(v, bias + c0 / 4 + 8 * h, word);
+                const int c1 = c0 + 32 * (h + 1);
+                if (c1 < cols) tc_ld_32x32b_x32(tacc + (uint32_t)c1, v);
+                else if (c1 - 32 < cols) release();                // once: behind the last columns that belong to the tile
+            }
             if (h == 0) {
                 __syncwarp();                                      // the columns before have been read
                 if constexpr (!WHOLE) {
@@ -492,8 +511,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
             const int n0 = tn * BN + part * 128;
             auto store = [&](auto type) {
                 constexpr int TYPE = decltype(type)::value;
-                if (p.bias) store_columns<TYPE, true, WHOLE>(tacc, row0, n0, cols, part, stage, bias, p, release);
-                else store_columns<TYPE, false, WHOLE>(tacc, row0, n0, cols, part, stage, bias, p, release);
+                constexpr bool HOLD = T::ONE && TYPE != T_F32;
+                if (p.bias) store_columns<TYPE, true, WHOLE, HOLD>(tacc, row0, n0, cols, part, stage, bias, p, release);
+                else store_columns<TYPE, false, WHOLE, HOLD>(tacc, row0, n0, cols, part, stage, bias, p, release);
             };
             if (p.out_type == T_F16) store(std::integral_constant<int, T_F16>());
             else if (p.out_type == T_BF16) store(std::integral_constant<int, T_BF16>());
@@ -547,8 +567,8 @@ cudaError_t fp8_pair_init()
 // The cost of a call, us: a start, waves of tiles (between the whole number that the last one makes and the fraction that the power limit sees), and the last
 // tile's epilogue.  A tile takes its k-tiles' time or its epilogue's, whichever is longer (a smooth maximum), or with one accumulator both.  Fitted
 // together with the costs of vnm_fp8_small.cu to steady calls on inputs that change, 431 shapes of 1 to 16384 x 8 to 36864 x 64 to 16384, odd ones and round ones, with and
-// without a bias, fp16 and fp32 results: ratio to the measured time 0.8 to 1.25; the plan chosen over both kernels takes 1.02 of the fastest one's time
-// on average, 1.6 at most (6687 x 40 x 3212).
+// without a bias, fp16 and fp32 results: ratio to the measured time 0.8 to 1.25; over 351 others, in runs long enough for the power limit, the plan chosen from both
+// kernels takes 1.012 of the fastest one's time on average, 1.4 at most (results of 8 to 40 columns).
 float fp8_pair_config(int M, int N, int K, bool wide_out, bool whole, bool bias, Fp8Plan *plan)
 {
     if (g_clusters <= 0) return -1.0f;

@@ -25,14 +25,21 @@ _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
 _ext = None
 
 
-def _call(name, *args):
+def _load():
     global _ext
-    if _ext is None:
-        _ext = spatha_module()
+    _ext = spatha_module()
+    return _ext
+
+
+def _error(e):
+    return VenomError(str(e).split("\nException raised from")[0])
+
+
+def _call(name, *args):
     try:
-        return getattr(_ext, name)(*args)
-    except RuntimeError as e:
-        raise VenomError(str(e).split("\nException raised from")[0]) from None
+        return getattr(_ext or _load(), name)(*args)
+    except (RuntimeError, TypeError) as e:
+        raise _error(e) from None
 
 
 class BlockFp8:
@@ -70,14 +77,20 @@ def quantize(x, dtype=E4M3, square=False, both=False):
     A block's scale is the smallest power of two that brings its largest finite magnitude to at most 448 (e4m3) or 57344 (e5m2); values are
     rounded to nearest even.  NaN stays NaN, infinities become NaN in e4m3 and stay in e5m2.  Blocks are 128 values of a row, or with `square` 128 x 128,
     so that a matrix and its transpose hold the same values.  both: also the transpose, as (BlockFp8 of x, BlockFp8 of x.T), from one read of x."""
-    a, sa, t, st, _ = _call("fp8_quantize", x, dtype, square, True, both, None)
-    return (BlockFp8(a, sa), BlockFp8(t, st)) if both else BlockFp8(a, sa)
+    try:
+        q = (_ext or _load()).fp8_quantize(x, dtype, bool(square), bool(both))
+    except (RuntimeError, TypeError) as e:
+        raise _error(e) from None
+    return (BlockFp8(q[0], q[1]), BlockFp8(q[2], q[3])) if both else BlockFp8(*q)
 
 
 def matmul(a, b, bias=None, dtype=torch.float16):
     """a @ b.T (+ bias): BlockFp8 [M, K] and [N, K] -> [M, N] of `dtype` (float16, bfloat16 or float32).  The 8-bit types of a and b may differ.
     bias: N values, added in 32 bits."""
-    return _call("fp8_matmul", a.data, a.scales, b.data, b.scales, bias, dtype)
+    try:
+        return (_ext or _load()).fp8_matmul(a.data, a.scales, b.data, b.scales, bias, dtype)
+    except (RuntimeError, TypeError) as e:
+        raise _error(e) from None
 
 
 def _check_input(x, what):
