@@ -301,7 +301,7 @@ int vnm_fp8_gelu_grad(const void *dy, int dy_type, int64_t ldy, int rows, int co
 int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, int a_type, const void *b, int64_t ldb, const void *b_scales, int b_type, int M, int N, int K,
                    const void *bias, int bias_type, void *out, int out_type, int64_t ldo, void *stream);
 /* The plan that vnm_fp8_matmul takes on the current device (for reporting): rows of A and of B a tile, CTAs that share a tile's k, CTAs in all.  whole: rows
- * of the result are 16-byte aligned and a multiple of 16 bytes long; bias: there is one.  tile_m = 256: pairs of SMs.  Any output pointer may be NULL. */
+ * of the result are 16-byte aligned; bias: there is one.  tile_m = 256: pairs of SMs.  Any output pointer may be NULL. */
 int vnm_fp8_matmul_config(int M, int N, int K, int out_type, int whole, int bias, int *tile_m, int *tile_n, int *split, int *grid);
 /* Reads and clears the sticky device-side status word of the 8-bit products on the current device, as vnm_device_status does for a handle.
  * Synchronises `stream`. */

@@ -168,6 +168,36 @@ def test_quantize_writes_its_own_rows_only(rows, cols):
     check_held(fp8.BlockFp8(data[:rows, :cols].view(E4M3), s[: sizes[0]].view(-1, rows, 4).view(torch.float8_e8m0fnu)), x, E4M3)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("cols", [1, 5, 7, 8, 9, 15, 17, 120, 127, 129, 505, 511, 513, 1031])
+def test_rows_that_begin_anywhere(dtype, cols):
+    """Every offset of a row inside 16 bytes, for what is read (values) and written (GELU and its gradient), and nothing written beside the rows."""
+    t = TYPES[dtype]
+    for start in range(0, 16 // t.itemsize):
+        x = matrix(11, cols, cols + start, t)
+        base = torch.zeros(11 * cols + 64, dtype=t, device="cuda")
+        moved = base[start:start + 11 * cols].view(11, cols)
+        moved.copy_(x)
+        base[:start], base[start + 11 * cols:] = math.nan, math.inf            # neighbours that must not get in
+        for both in (False, True):
+            q = fp8.quantize(moved, both=both)
+            check_held(q[0] if both else q, x, E4M3)
+            if both:
+                check_held(q[1], x.t(), E4M3)
+        lib, stream, tcode = capi.lib(), torch.cuda.current_stream().cuda_stream, {"fp32": 0, "fp16": 1, "bf16": 2}[dtype]
+        h = fp8.quantize(x)
+        y = torch.full((11 * cols + 64,), 7.0, dtype=t, device="cuda")
+        at = y.data_ptr() + start * t.itemsize
+        assert lib.vnm_fp8_gelu(moved.data_ptr(), tcode, cols, 11, cols, 0, at, cols, None, 16, None, None, 16, None, None, 16, None, stream) == 0
+        check_gelu(y[start:start + 11 * cols].view(11, cols), gelu64(x, False)[0], x)
+        assert bool((y[:start] == 7).all()) and bool((y[start + 11 * cols:] == 7).all())
+        y.fill_(7.0)
+        assert lib.vnm_fp8_gelu_grad(moved.data_ptr(), tcode, cols, 11, cols, 1, h.data.data_ptr(), h.data.stride(0), h.scales.data_ptr(), at, cols, 0, None, 16, None, None, 16, None,
+                                     None, 0, None, stream) == 0
+        check_gelu(y[start:start + 11 * cols].view(11, cols), x.double() * gelu64(value64(x), True)[1], value64(x), x)
+        assert bool((y[:start] == 7).all()) and bool((y[start + 11 * cols:] == 7).all())
+
+
 def test_quantize_long_rows_and_many_rows():
     """Offsets past 32 bits in the input and the result."""
     free, _ = torch.cuda.mem_get_info()
@@ -222,7 +252,7 @@ INSTANCES = {
 
 def plan_of(M, N, K, dtype, bias):
     v = [ctypes.c_int() for _ in range(4)]
-    whole = N * torch.finfo(dtype).bits // 8 % 16 == 0
+    whole = N * torch.finfo(dtype).bits // 8 % 16 == 0     # rows of a contiguous result
     assert capi.lib().vnm_fp8_matmul_config(M, N, K, 0 if dtype == torch.float32 else 1, whole, bias, *[ctypes.byref(x) for x in v]) == 0
     return [x.value for x in v]
 
@@ -318,7 +348,7 @@ def test_matmul_reads_operands_as_they_lie():
         fp8.matmul(fp8.BlockFp8(big.view(E4M3)[2:2 + M, 17:17 + K], a.scales), b)
 
 
-@pytest.mark.parametrize("M,N,ldo", [(33, 130, 161), (300, 257, 300), (5, 64, 64), (257, 520, 528)])
+@pytest.mark.parametrize("M,N,ldo", [(33, 130, 161), (300, 257, 300), (5, 64, 64), (257, 520, 528), (2051, 1999, 2000), (2050, 1999, 2008), (2050, 1993, 1999), (1500, 2053, 2056)])
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_matmul_writes_its_own_rows_only(M, N, ldo, dtype):
     K = 520

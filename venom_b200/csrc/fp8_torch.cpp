@@ -134,7 +134,8 @@ Tensor dequantize(const Tensor &data, const Tensor &scales, c10::ScalarType type
     return out;
 }
 
-Tensor matmul(const Tensor &a, const Tensor &sa, const Tensor &b, const Tensor &sb, const OptTensor &bias, c10::ScalarType type)
+// aligned_rows: the result's rows begin on 16-byte boundaries, for what stays inside an operator (the quantiser reads such rows faster).
+Tensor matmul(const Tensor &a, const Tensor &sa, const Tensor &b, const Tensor &sb, const OptTensor &bias, c10::ScalarType type, bool aligned_rows = false)
 {
     check_packed(a, sa, "fp8.matmul");
     check_packed(b, sb, "fp8.matmul");
@@ -146,10 +147,12 @@ Tensor matmul(const Tensor &a, const Tensor &sa, const Tensor &b, const Tensor &
                     " values on the operands' device");
     c10::cuda::CUDAGuard guard(a.device());
     const int M = to_int(a.size(0), "fp8.matmul"), N = to_int(b.size(0), "fp8.matmul"), K = to_int(a.size(1), "fp8.matmul");
-    Tensor out = device_empty({M, N}, type, a);
+    const int64_t ld = aligned_rows ? ((int64_t)N + 7) / 8 * 8 : N;
+    Tensor out = device_empty({M, ld}, type, a);
+    if (ld != N) out = out.narrow(1, 0, N);
     check(vnm_fp8_matmul(a.data_ptr(), packed_ld(a), sa.data_ptr(), f8_code(a.scalar_type(), "fp8.matmul"), b.data_ptr(), packed_ld(b), sb.data_ptr(),
                          f8_code(b.scalar_type(), "fp8.matmul"), M, N, K, with_bias ? bias->data_ptr() : nullptr, with_bias ? type_code(bias->scalar_type(), "fp8.matmul: bias") : VNM_F32,
-                         out.data_ptr(), type_code(type, "fp8.matmul"), std::max(1, N), c10::cuda::getCurrentCUDAStream().stream()),
+                         out.data_ptr(), type_code(type, "fp8.matmul"), std::max<int64_t>(1, ld), c10::cuda::getCurrentCUDAStream().stream()),
           "vnm_fp8_matmul");
     return out;
 }
@@ -287,9 +290,9 @@ Both quantized(const Tensor &x, c10::ScalarType f8, bool square, bool rows, bool
     const Quantized q = quantize(x, f8, square, rows, cols, sums);
     return {{or_undefined(std::get<0>(q)), or_undefined(std::get<1>(q))}, {or_undefined(std::get<2>(q)), or_undefined(std::get<3>(q))}, or_undefined(std::get<4>(q))};
 }
-Tensor product(const Operand &a, const Operand &b, const Tensor &bias, c10::ScalarType type)
+Tensor product(const Operand &a, const Operand &b, const Tensor &bias, c10::ScalarType type, bool aligned_rows = false)
 {
-    return matmul(a.data, a.scales, b.data, b.scales, bias.defined() ? OptTensor(bias.detach().contiguous()) : c10::nullopt, type);
+    return matmul(a.data, a.scales, b.data, b.scales, bias.defined() ? OptTensor(bias.detach().contiguous()) : c10::nullopt, type, aligned_rows);
 }
 // dy^T x from the transposes; zeros without any token
 Tensor weight_grad(const Operand &dy_t, const Operand &x_t, c10::ScalarType type)
@@ -372,7 +375,7 @@ struct Mlp : torch::autograd::Function<Mlp> {
         const bool inner = need_x || need_w1 || need_b1;      // whether the gradient goes back through the GELU
         Both xs = quantized(flat(x), torch::kFloat8_e4m3fn, false, true, need_w1, c10::nullopt);
         Both w1s = quantized(w1, torch::kFloat8_e4m3fn, true, true, need_x, c10::nullopt);
-        Gelu a = gelu(product(xs.rows, w1s.rows, b1, x.scalar_type()), tanh_form, false, true, need_w2, inner);
+        Gelu a = gelu(product(xs.rows, w1s.rows, b1, x.scalar_type(), true), tanh_form, false, true, need_w2, inner);
         Both w2s = quantized(w2, torch::kFloat8_e4m3fn, true, true, inner, c10::nullopt);
         const Tensor y = product({*std::get<1>(a), *std::get<2>(a)}, w2s.rows, b2, x.scalar_type());
         ctx->save_for_backward({xs.cols.data, xs.cols.scales, w1s.cols.data, w1s.cols.scales, or_undefined(std::get<3>(a)), or_undefined(std::get<4>(a)),
@@ -401,7 +404,7 @@ struct Mlp : torch::autograd::Function<Mlp> {
         Tensor dx, dw1, db1, dw2;
         if (need_w2) dw2 = weight_grad(g.cols, {s[4], s[5]}, type("w2"));
         if (inner) {
-            const Tensor da = product(g.rows, {s[8], s[9]}, Tensor(), type("x"));
+            const Tensor da = product(g.rows, {s[8], s[9]}, Tensor(), type("x"), true);
             const GeluGrad h = gelu_grad(da, s[6], s[7], ctx->saved_data["tanh"].toBool(), false, type("grad"), need_x, need_w1 || need_b1, type_of(need_b1, type("b1")));
             db1 = or_undefined(std::get<5>(h));
             if (need_x) dx = product({*std::get<1>(h), *std::get<2>(h)}, {s[2], s[3]}, Tensor(), type("x")).view(ctx->saved_data["shape"].toIntVector());

@@ -21,7 +21,7 @@ struct Fp8QuantParams {
     int rows, cols;
     int f8;                  // type of data and data_t
     int tanh_form;           // GELU by tanh
-    int align_x, align_y;    // what the addresses of the rows of x and y are a multiple of: 16, 4 or fewer bytes
+    int align_x, align_y;    // what the addresses of the rows of x and y are a multiple of: 16, 4 or 2 bytes
     uint8_t *data;           // [rows, ldd] or null
     int64_t ldd;
     uint8_t *scales;         // [groups][rows][4]
@@ -87,7 +87,7 @@ struct Fp8MatmulParams {
     int64_t ldo;
     int M, N, K, ktiles;
     int out_type, bias_type;
-    int whole_pieces;         // pair kernel: rows of the result lie on 16-byte boundaries and are a multiple of 16 bytes long
+    int whole_pieces;         // pair kernel: rows of the result lie on 16-byte boundaries
     int a_f8, b_f8;
     int mt, nt;               // tiles along M and N
     int split;                // CTAs of a cluster that share one tile's k

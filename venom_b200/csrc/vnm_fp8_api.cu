@@ -66,10 +66,18 @@ int check_sums(const char *name, const void *colsum, int type, const void *works
     return VNM_OK;
 }
 
+bool pieces(const void *x, int type, int64_t ld) { return aligned(x, 16) && ld * elem_size(type) % 16 == 0; }
+
 int row_alignment(const void *x, int type, int64_t ld)
 {
     const uintptr_t both = reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ld * elem_size(type));
     return (both & 15) == 0 ? 16 : (both & 3) == 0 ? 4 : 2;
+}
+
+void set_input(Fp8QuantParams *p, const void *x, int type, int64_t ldx, int rows, int cols)
+{
+    p->x = x; p->ldx = ldx; p->rows = rows; p->cols = cols;
+    p->align_x = row_alignment(x, type, ldx);
 }
 
 #define VNM_TRY(call)               \
@@ -172,8 +180,8 @@ extern "C" int vnm_fp8_quantize(const void *x, int x_type, int64_t ldx, int rows
     if (rows == 0 || cols == 0) return empty_sums(colsum, colsum_type, cols, s);
     if (!data && !data_t) return fail(VNM_ERR_BAD_ARG, "%s: nothing is wanted", name);
     Fp8QuantParams p = {};
-    p.x = x; p.ldx = ldx; p.rows = rows; p.cols = cols; p.f8 = f8_type;
-    p.align_x = row_alignment(x, x_type, ldx);
+    set_input(&p, x, x_type, ldx, rows, cols);
+    p.f8 = f8_type;
     p.data = static_cast<uint8_t *>(data); p.ldd = ldd; p.scales = static_cast<uint8_t *>(scales);
     p.data_t = static_cast<uint8_t *>(data_t); p.ldt = ldt; p.scales_t = static_cast<uint8_t *>(scales_t);
     p.partial = colsum ? static_cast<float *>(workspace) : nullptr;
@@ -209,8 +217,8 @@ extern "C" int vnm_fp8_gelu(const void *x, int x_type, int64_t ldx, int rows, in
     if (y && data_t) return fail(VNM_ERR_UNSUPPORTED, "%s: the result in its own type together with a transpose", name);
     if (!y && !data && !data_t) return fail(VNM_ERR_BAD_ARG, "%s: nothing is wanted", name);
     Fp8QuantParams p = {};
-    p.x = x; p.ldx = ldx; p.rows = rows; p.cols = cols; p.f8 = VNM_E4M3; p.tanh_form = tanh_form != 0;
-    p.align_x = row_alignment(x, x_type, ldx);
+    set_input(&p, x, x_type, ldx, rows, cols);
+    p.f8 = VNM_E4M3; p.tanh_form = tanh_form != 0;
     p.y = y; p.ldy = ldy; p.align_y = row_alignment(y, x_type, ldy);
     p.data = static_cast<uint8_t *>(data); p.ldd = ldd; p.scales = static_cast<uint8_t *>(scales);
     p.data_t = static_cast<uint8_t *>(data_t); p.ldt = ldt; p.scales_t = static_cast<uint8_t *>(scales_t);
@@ -237,8 +245,8 @@ extern "C" int vnm_fp8_gelu_grad(const void *dy, int dy_type, int64_t ldy, int r
     if (dx && data_t) return fail(VNM_ERR_UNSUPPORTED, "%s: the result in its own type together with a transpose", name);
     if (!dx && !data && !data_t) return fail(VNM_ERR_BAD_ARG, "%s: nothing is wanted", name);
     Fp8QuantParams p = {};
-    p.x = dy; p.ldx = ldy; p.rows = rows; p.cols = cols; p.f8 = f8_type; p.tanh_form = tanh_form != 0;
-    p.align_x = row_alignment(dy, dy_type, ldy);
+    set_input(&p, dy, dy_type, ldy, rows, cols);
+    p.f8 = f8_type; p.tanh_form = tanh_form != 0;
     p.y = dx; p.ldy = lddx; p.align_y = row_alignment(dx, dy_type, lddx);
     p.data = static_cast<uint8_t *>(data); p.ldd = ldd; p.scales = static_cast<uint8_t *>(scales);
     p.data_t = static_cast<uint8_t *>(data_t); p.ldt = ldt; p.scales_t = static_cast<uint8_t *>(scales_t);
@@ -272,7 +280,7 @@ extern "C" int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, 
     p.sa = static_cast<const uint32_t *>(a_scales); p.sb = static_cast<const uint32_t *>(b_scales);
     p.bias = bias; p.bias_type = bias_type;
     p.out = out; p.out_type = out_type; p.ldo = ldo;
-    p.whole_pieces = aligned(out, 16) && ldo * elem_size(out_type) % 16 == 0 && (int64_t)N * elem_size(out_type) % 16 == 0;
+    p.whole_pieces = pieces(out, out_type, ldo);
     p.M = M; p.N = N; p.K = K; p.ktiles = (K + 127) / 128;
     p.a_f8 = a_type; p.b_f8 = b_type;
     p.status = status;

@@ -175,7 +175,7 @@ __device__ __forceinline__ void store_part(uint8_t *dst, const uint32_t (&y)[4],
     }
 }
 
-// `part`: 0 the first 128 columns of a tile, 1 the rest; WHOLE: rows lie on 16-byte boundaries and have whole pieces.  HOLD (128 columns of 16 bits): all of them are
+// `part`: 0 the first 128 columns of a tile, 1 the rest; WHOLE: rows lie on 16-byte boundaries.  HOLD (128 columns of 16 bits): all of them are
 // rounded into registers before the first is stored, where the next tile's MMAs wait for this accumulator.
 template <int TYPE, bool BIAS, bool WHOLE, bool HOLD, typename Release>
 __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n0, int cols, int part, uint4 *stage, const float4 *bias, const Fp8MatmulParams &p, Release release)
@@ -255,12 +255,28 @@ __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n
         const int piece = lane & 7, first = lane >> 3;
         if constexpr (WHOLE) {
             uint8_t *dst = out + first * pitch + piece * 16;
-            const bool on = piece * 16 < left;
+            const int end = left - piece * 16;                      // bytes of a row from this piece on
+            if (left >= 128 || (left & 15) == 0) {
+                const bool on = end > 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++, dst += 4 * pitch) {
-                const int r = 4 * i + first;
-                const uint4 q = stage[r * 8 + (piece ^ (r & 7))];
-                if (on && r < rows) *reinterpret_cast<uint4 *>(dst) = q;
+                for (int i = 0; i < 8; i++, dst += 4 * pitch) {
+                    const int r = 4 * i + first;
+                    const uint4 q = stage[r * 8 + (piece ^ (r & 7))];
+                    if (on && r < rows) *reinterpret_cast<uint4 *>(dst) = q;
+                }
+            } else if (end > 0) {                                   // the matrix ends inside a piece
+#pragma unroll 1
+                for (int i = 0; i < 8; i++, dst += 4 * pitch) {
+                    const int r = 4 * i + first;
+                    const uint4 q = stage[r * 8 + (piece ^ (r & 7))];
+                    if (r >= rows) break;
+                    if (end >= 16) {
+                        *reinterpret_cast<uint4 *>(dst) = q;
+                    } else {
+                        const uint32_t y[4] = {q.x, q.y, q.z, q.w};
+                        store_part(dst, y, 0, end);
+                    }
+                }
             }
         } else if (left > 0) {
             // Piece q of a row, counted from the sector that these columns begin in (s bytes into it), out of the row's window: five words at a byte offset that

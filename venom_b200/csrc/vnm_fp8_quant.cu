@@ -37,9 +37,12 @@ struct Raw {
     static constexpr int WORDS = TYPE == T_F32 ? 8 : 4;
     uint32_t w[WORDS];
 };
-// `align`: what the rows' addresses are a multiple of, 16 or 4 bytes or the type's size.  What lies past `cols` is zero.
+// `align`: what the rows' addresses are a multiple of, 16, 4 or 2 bytes.  What lies past `cols` is zero.  inner: rows lie ahead of this one and behind it, so that a row
+// which begins inside a word may be read in whole words, with two bytes too many at either end: five of them, the last in `extra`, out of which settle() takes the
+// values when they are wanted (taken here, they would be waited for).  8191 x 4095 fp16: value by value 35 us.
+// Loading whole pieces of 16 bytes and exchanging words between lanes instead is slower for such rows, and its registers slow the others down.
 template <int TYPE>
-__device__ __forceinline__ Raw<TYPE> load_raw(const void *x, int64_t at, int c, int cols, int align)
+__device__ __forceinline__ Raw<TYPE> load_raw(const void *x, int64_t at, int c, int cols, int align, bool inner, uint32_t &extra)
 {
     using E = typename Elem<TYPE>::type;
     Raw<TYPE> r;
@@ -58,6 +61,12 @@ __device__ __forceinline__ Raw<TYPE> load_raw(const void *x, int64_t at, int c, 
     } else if constexpr (TYPE == T_F32) {
 #pragma unroll
         for (int i = 0; i < 8; i++) r.w[i] = c + i < cols ? __ldg(reinterpret_cast<const uint32_t *>(src) + i) : 0u;
+    } else if (c + 8 <= cols && inner) {
+        const uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 2);
+        const uint32_t *word = reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint8_t *>(src) - odd);
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.w[i] = __ldg(word + i);
+        extra = __ldg(word + (odd ? 4 : 3));
     } else {
         const unsigned short *h = reinterpret_cast<const unsigned short *>(src);
 #pragma unroll
@@ -67,6 +76,16 @@ __device__ __forceinline__ Raw<TYPE> load_raw(const void *x, int64_t at, int c, 
         }
     }
     return r;
+}
+template <int TYPE>
+__device__ __forceinline__ void settle(Raw<TYPE> &r, uint32_t extra, const void *x, int64_t at, int c, int cols, int align, bool inner)
+{
+    if constexpr (TYPE != T_F32) {
+        if (align < 4 && inner && c + 8 <= cols && ((reinterpret_cast<uintptr_t>(x) + 2 * (uintptr_t)(at + c)) & 2)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) r.w[i] = __byte_perm(r.w[i], i < 3 ? r.w[i < 3 ? i + 1 : 3] : extra, 0x5432);
+        }
+    }
 }
 template <int TYPE>
 __device__ __forceinline__ void to_floats(const Raw<TYPE> &r, float (&v)[8])
@@ -185,6 +204,22 @@ __device__ __forceinline__ void store8(void *y, int64_t at, int c, int cols, int
 #pragma unroll
             for (int i = 0; i < Raw<TYPE>::WORDS; i++) reinterpret_cast<uint32_t *>(dst)[i] = w[i];
         }
+    } else if (TYPE != T_F32 && c + 8 <= cols && (reinterpret_cast<uintptr_t>(dst) & 2)) {
+        // inside a word: the first and the last value alone, three words between them
+        dst[0] = from_float<TYPE>(v[0]);
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            uint32_t w;
+            if constexpr (TYPE == T_F16) {
+                const __half2 h = __floats2half2_rn(v[2 * i + 1], v[2 * i + 2]);
+                w = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i + 1], v[2 * i + 2]);
+                w = *reinterpret_cast<const uint32_t *>(&h);
+            }
+            *reinterpret_cast<uint32_t *>(dst + 2 * i + 1) = w;
+        }
+        dst[7] = from_float<TYPE>(v[7]);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
@@ -450,12 +485,13 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
     uint32_t u = first, row = first / groups, g = first - row * groups;
 
     Raw<TYPE> next[4];
+    uint32_t extra[4];
     uint2 next_h[4];
     uint32_t next_codes = 0;
     auto fetch = [&](uint32_t unit, uint32_t r, uint32_t gr) {
         const int c = (int)gr * 512 + sub;
 #pragma unroll
-        for (int i = 0; i < 4; i++) next[i] = load_raw<TYPE>(p.x, (int64_t)r * p.ldx, c + 128 * i, unit < total ? p.cols : 0, p.align_x);
+        for (int i = 0; i < 4; i++) next[i] = load_raw<TYPE>(p.x, (int64_t)r * p.ldx, c + 128 * i, unit < total ? p.cols : 0, p.align_x, r > 0 && r + 1 < (uint32_t)p.rows, extra[i]);
         if constexpr (OP == FP8_GELU_GRAD) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -471,6 +507,10 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
         const int64_t word = (int64_t)g * p.rows + r;
         constexpr bool AS_LOADED = OP == FP8_PLAIN && TYPE != T_F32;
         Block4<TYPE, AS_LOADED> v;
+        if (TYPE != T_F32 && p.align_x < 4 && on) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) settle<TYPE>(next[i], extra[i], p.x, r * p.ldx, c + 128 * i, p.cols, p.align_x, r > 0 && r + 1 < p.rows);
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if constexpr (AS_LOADED) v.raw[i] = next[i];
@@ -566,8 +606,20 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
     Block4<TYPE, AS_LOADED> v;
     {
         Raw<TYPE> raw[4];
+        if (WHOLE || p.align_x >= 4) {
+            uint32_t extra;
 #pragma unroll
-        for (int j = 0; j < 4; j++) raw[j] = load_raw<TYPE>(p.x, (r0 + j) * p.ldx, c, WHOLE ? c + 8 : j < left ? p.cols : 0, WHOLE ? 16 : p.align_x);
+            for (int j = 0; j < 4; j++) raw[j] = load_raw<TYPE>(p.x, (r0 + j) * p.ldx, c, WHOLE ? c + 8 : j < left ? p.cols : 0, WHOLE ? 16 : p.align_x, false, extra);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t extra;
+                const bool inner = r0 + j > 0 && r0 + j + 1 < p.rows;
+                const int cols = j < left ? p.cols : 0;
+                raw[j] = load_raw<TYPE>(p.x, (r0 + j) * p.ldx, c, cols, 2, inner, extra);
+                settle<TYPE>(raw[j], extra, p.x, (r0 + j) * p.ldx, c, cols, 2, inner);
+            }
+        }
         uint2 q[4];
         uint32_t codes[4];
         if constexpr (OP == FP8_GELU_GRAD) {
