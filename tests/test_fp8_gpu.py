@@ -12,6 +12,7 @@ import sys
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from venom_b200 import capi, fp8
 
@@ -610,6 +611,54 @@ def test_mlp_without_biases_and_tokens():
     assert y.shape == (0, 64) and grads[0].shape == (0, 64) and bool((grads[1] == 0).all()) and bool((grads[2] == 0).all())
 
 
+def test_gradients_without_any_output():
+    """A weight without rows: nothing to sum, so the gradients behind it are zeros."""
+    x, w, b = leaf(matrix(5, 64, 1, torch.float16)), leaf(torch.empty(0, 64, dtype=torch.float16, device="cuda")), leaf(torch.empty(0, dtype=torch.float16, device="cuda"))
+    y = fp8.linear(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+    assert y.shape == (5, 0) and dx.shape == x.shape and not dx.any() and dw.shape == (0, 64) and db.shape == (0,)
+    w1 = leaf(matrix(96, 64, 2, torch.float16))
+    y = fp8.mlp(x, w1, None, leaf(torch.empty(0, 96, dtype=torch.float16, device="cuda")), None)
+    grads = torch.autograd.grad(y, (x, w1), torch.empty_like(y))
+    assert y.shape == (5, 0) and not any(g.any() for g in grads)
+
+
+def offloaded():
+    """Saved tensors go to the host and come back."""
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda())
+
+
+@pytest.mark.parametrize("tokens,cin,hidden,cout", [(1, 64, 128, 64), (37, 100, 203, 70), (130, 256, 512, 128)])
+def test_saved_tensors_that_went_elsewhere(tokens, cin, hidden, cout):
+    leaves = block(tokens, cin, hidden, cout, torch.float16)
+    x, w1, b1 = leaves[:3]
+    calls = ((lambda: fp8.linear(x, w1, b1), (x, w1, b1)), (lambda: fp8.gelu(x), (x,)), (lambda: fp8.mlp(*leaves), leaves))
+    for call, of in calls:
+        y = call()
+        dy = matrix(*y.shape, 9, torch.float16)
+        want = torch.autograd.grad(y, of, dy)
+        with offloaded():
+            y = call()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, of, dy), want))
+        for reentrant in (False, True):
+            y = torch.utils.checkpoint.checkpoint(lambda *_: call(), *of, use_reentrant=reentrant)
+            if reentrant:
+                for t in of:
+                    t.grad = None
+                y.backward(dy)
+                assert all(torch.equal(t.grad, b) for t, b in zip(of, want))
+            else:
+                assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, of, dy), want))
+
+
+def test_saved_tensors_in_another_form_are_refused():
+    x, w = leaf(matrix(37, 100, 1, torch.float16)), leaf(matrix(70, 100, 2, torch.float16))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:-1]):
+        y = fp8.linear(x, w)
+    with pytest.raises(RuntimeError, match="another form"):
+        y.backward(torch.ones_like(y))
+
+
 # ---- modules ----
 
 def test_frozen_layers():
@@ -643,6 +692,30 @@ def test_frozen_mlp_and_conversion():
     conv = fp8.linear_to_fp8(copy.deepcopy(net))
     a = fp8.linear(x, net[0].weight, net[0].bias)
     assert torch.equal(conv[0](x), a) and torch.equal(conv(x), fp8.linear(torch.nn.functional.gelu(a), net[2].weight, net[2].bias))
+
+
+def test_layers_in_inference_mode():
+    lin, x = torch.nn.Linear(200, 131).half().cuda(), matrix(30, 200, 1, torch.float16)
+    want = fp8.Fp8Linear(lin)(x)
+    with torch.inference_mode():
+        made = fp8.Fp8Linear(lin)
+        assert torch.equal(made(x), want) and torch.equal(fp8.linear(x, lin.weight, lin.bias), want)
+        assert torch.equal(fp8.quantize(x).dequantize(), value64(x).float())
+    with torch.no_grad():
+        assert torch.equal(made(x), want)
+
+
+def test_gradients_accumulate_and_repeat():
+    """Two calls of one layer in one graph, backward twice: gradients add up, and saved tensors are as they were."""
+    x, w, b = leaf(matrix(50, 96, 1, torch.float16)), leaf(matrix(72, 96, 2, torch.float16)), leaf(matrix(1, 72, 3, torch.float16)[0].clone())
+    dy = matrix(50, 72, 9, torch.float16)
+    want = torch.autograd.grad(fp8.linear(x, w, b), (x, w, b), dy)
+    y = fp8.linear(x, w, b)
+    first = torch.autograd.grad(y, (x, w, b), dy, retain_graph=True)
+    assert all(torch.equal(a, c) for a, c in zip(first, want))
+    assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(y, (x, w, b), dy), want))
+    (fp8.linear(x, w, b) + fp8.linear(x, w, b)).backward(dy)
+    assert all(torch.equal(t.grad, c + c) for t, c in zip((x, w, b), want))
 
 
 def test_training_step_with_modules():

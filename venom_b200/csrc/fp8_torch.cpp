@@ -12,6 +12,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
+#include <array>
+
 #include "../../include/venom_b200.h"
 
 namespace {
@@ -54,13 +56,6 @@ Tensor as_rows(const Tensor &x, const char *what)
 }
 int64_t row_stride(const Tensor &x) { return x.size(0) > 1 ? x.stride(0) : x.size(1) > 1 ? x.size(1) : 1; }
 
-struct Packed {
-    Tensor data, scales;
-    int64_t ld = 16;
-    void *values() { return data.defined() ? data.data_ptr() : nullptr; }
-    void *scale() { return data.defined() ? scales.data_ptr() : nullptr; }
-};
-
 // A tensor on part of a storage, without the dispatcher (a view of a tensor takes 1.5 us).
 Tensor on_storage(const c10::Storage &storage, c10::ScalarType type, int64_t byte_offset, at::IntArrayRef shape, at::IntArrayRef strides)
 {
@@ -70,15 +65,31 @@ Tensor on_storage(const c10::Storage &storage, c10::ScalarType type, int64_t byt
     return t;
 }
 
-// Values and scales in one allocation.
-Packed pack(int64_t rows, int64_t cols, c10::ScalarType f8, const Tensor &like)
+// A matrix in 8 bits: values and scales in one allocation.
+struct Packed {
+    Tensor bytes;                // undefined: not wanted
+    c10::ScalarType f8 = torch::kFloat8_e4m3fn;
+    int64_t rows = 0, cols = 0, ld = 16;
+    bool wanted() const { return bytes.defined(); }
+    void *values() const { return wanted() ? bytes.data_ptr() : nullptr; }
+    void *scale() const { return wanted() ? static_cast<char *>(bytes.data_ptr()) + rows * ld : nullptr; }
+    Tensor data() const { return on_storage(bytes.storage(), f8, 0, {rows, cols}, {ld, 1}); }
+    Tensor scales() const { return on_storage(bytes.storage(), torch::kFloat8_e8m0fnu, rows * ld, {(cols + 511) / 512, rows, 4}, {rows * 4, 4, 1}); }
+};
+Packed packed(const Tensor &bytes, int64_t rows, int64_t cols, c10::ScalarType f8) { return {bytes, f8, rows, cols, std::max<int64_t>(16, (cols + 15) / 16 * 16)}; }
+int64_t packed_bytes(const Packed &p) { return p.rows * p.ld + (p.cols + 511) / 512 * p.rows * 4; }
+Packed pack(bool wanted, int64_t rows, int64_t cols, c10::ScalarType f8, const Tensor &like)
 {
-    Packed p;
-    p.ld = std::max<int64_t>(16, (cols + 15) / 16 * 16);
-    const int64_t groups = (cols + 511) / 512;
-    const Tensor bytes = device_empty({rows * p.ld + groups * rows * 4}, torch::kUInt8, like);
-    p.data = on_storage(bytes.storage(), f8, 0, {rows, cols}, {p.ld, 1});
-    p.scales = on_storage(bytes.storage(), torch::kFloat8_e8m0fnu, rows * p.ld, {groups, rows, 4}, {rows * 4, 4, 1});
+    Packed p = packed(Tensor(), rows, cols, f8);
+    if (wanted) p.bytes = device_empty({packed_bytes(p)}, torch::kUInt8, like);
+    return p;
+}
+// What a backward pass gets back of one: the bytes may have been elsewhere meanwhile (hooks on saved tensors).
+Packed unpacked(const Tensor &bytes, int64_t rows, int64_t cols)
+{
+    const Packed p = packed(bytes, rows, cols, torch::kFloat8_e4m3fn);
+    TORCH_CHECK(bytes.defined() && bytes.is_cuda() && bytes.scalar_type() == torch::kUInt8 && bytes.is_contiguous() && bytes.numel() == packed_bytes(p),
+                "a saved tensor came back from its hooks in another form");
     return p;
 }
 
@@ -100,26 +111,25 @@ Tensor sums_workspace(const Tensor &sums, int64_t rows, int64_t cols, const Tens
     return sums.defined() ? device_empty({(rows + 127) / 128 * cols}, torch::kFloat32, like) : Tensor();
 }
 void *ptr(const Tensor &t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
-OptTensor opt(const Tensor &t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 
-using Quantized = std::tuple<OptTensor, OptTensor, OptTensor, OptTensor, OptTensor>;
+struct Both {
+    Packed rows, cols;           // of a matrix and of its transpose
+    Tensor sums;                 // of its columns
+};
 
-// (data, scales, data_t, scales_t, column sums), None for what is not wanted
-Quantized quantize(const Tensor &x_in, c10::ScalarType f8, bool square, bool rows_wanted, bool cols_wanted, c10::optional<c10::ScalarType> sums_type)
+Both quantize(const Tensor &x_in, c10::ScalarType f8, bool square, bool rows_wanted, bool cols_wanted, c10::optional<c10::ScalarType> sums_type)
 {
     const Tensor x = as_rows(x_in, "fp8.quantize");
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t rows = x.size(0), cols = x.size(1);
     const int code = f8_code(f8, "fp8.quantize"), type = type_code(x.scalar_type(), "fp8.quantize");
     const int r = to_int(rows, "fp8.quantize"), c = to_int(cols, "fp8.quantize");
-    Packed a, t;
-    if (rows_wanted) a = pack(rows, cols, f8, x);
-    if (cols_wanted) t = pack(cols, rows, f8, x);
-    const Tensor sums = undefined_or_sums(sums_type, cols, x), ws = sums_workspace(sums, rows, cols, x);
-    check(vnm_fp8_quantize(x.data_ptr(), type, row_stride(x), r, c, code, square, a.values(), a.ld, a.scale(), t.values(), t.ld, t.scale(), ptr(sums),
+    Both q = {pack(rows_wanted, rows, cols, f8, x), pack(cols_wanted, cols, rows, f8, x), undefined_or_sums(sums_type, cols, x)};
+    const Tensor ws = sums_workspace(q.sums, rows, cols, x);
+    check(vnm_fp8_quantize(x.data_ptr(), type, row_stride(x), r, c, code, square, q.rows.values(), q.rows.ld, q.rows.scale(), q.cols.values(), q.cols.ld, q.cols.scale(), ptr(q.sums),
                            sums_type.has_value() ? type_code(*sums_type, "fp8.quantize") : VNM_F32, ptr(ws), c10::cuda::getCurrentCUDAStream().stream()),
           "vnm_fp8_quantize");
-    return Quantized(opt(a.data), opt(a.scales), opt(t.data), opt(t.scales), opt(sums));
+    return q;
 }
 
 Tensor dequantize(const Tensor &data, const Tensor &scales, c10::ScalarType type)
@@ -134,74 +144,83 @@ Tensor dequantize(const Tensor &data, const Tensor &scales, c10::ScalarType type
     return out;
 }
 
-// aligned_rows: the result's rows begin on 16-byte boundaries, for what stays inside an operator (the quantiser reads such rows faster).
-Tensor matmul(const Tensor &a, const Tensor &sa, const Tensor &b, const Tensor &sb, const OptTensor &bias, c10::ScalarType type, bool aligned_rows = false)
+struct Operand {
+    const void *data;
+    int64_t ld;
+    const void *scales;
+    c10::ScalarType f8;
+    int64_t rows, cols;
+    Operand(const Packed &p) : data(p.values()), ld(p.ld), scales(p.scale()), f8(p.f8), rows(p.rows), cols(p.cols) {}
+    Operand(const Tensor &d, const Tensor &s) : data(d.data_ptr()), ld(packed_ld(d)), scales(s.data_ptr()), f8(d.scalar_type()), rows(d.size(0)), cols(d.size(1)) {}
+};
+
+// On the current device.  aligned_rows: the result's rows begin on 16-byte boundaries, for what stays inside an operator (the quantiser reads such rows faster).
+Tensor multiply(const Operand &a, const Operand &b, const Tensor &bias, c10::ScalarType type, const Tensor &like, bool aligned_rows = false)
+{
+    const int M = to_int(a.rows, "fp8.matmul"), N = to_int(b.rows, "fp8.matmul"), K = to_int(a.cols, "fp8.matmul");
+    const int64_t ld = aligned_rows ? ((int64_t)N + 7) / 8 * 8 : N;
+    Tensor out = device_empty({M, ld}, type, like);
+    if (ld != N) out = out.narrow(1, 0, N);
+    check(vnm_fp8_matmul(a.data, a.ld, a.scales, f8_code(a.f8, "fp8.matmul"), b.data, b.ld, b.scales, f8_code(b.f8, "fp8.matmul"), M, N, K, ptr(bias),
+                         bias.defined() ? type_code(bias.scalar_type(), "fp8.matmul: bias") : VNM_F32, out.data_ptr(), type_code(type, "fp8.matmul"), std::max<int64_t>(1, ld),
+                         c10::cuda::getCurrentCUDAStream().stream()),
+          "vnm_fp8_matmul");
+    return out;
+}
+
+Tensor matmul(const Tensor &a, const Tensor &sa, const Tensor &b, const Tensor &sb, const Tensor &bias, c10::ScalarType type)
 {
     check_packed(a, sa, "fp8.matmul");
     check_packed(b, sb, "fp8.matmul");
     TORCH_CHECK(a.device() == b.device(), "fp8.matmul: operands on one device expected");
     TORCH_CHECK(a.size(1) == b.size(1), "fp8.matmul: ", a.size(1), " and ", b.size(1), " columns do not match");
-    const bool with_bias = bias.has_value() && bias->defined();
-    if (with_bias)
-        TORCH_CHECK(bias->device() == a.device() && bias->dim() == 1 && bias->numel() == b.size(0) && bias->is_contiguous(), "fp8.matmul: bias must be a contiguous vector of ", b.size(0),
+    if (bias.defined())
+        TORCH_CHECK(bias.device() == a.device() && bias.dim() == 1 && bias.numel() == b.size(0) && bias.is_contiguous(), "fp8.matmul: bias must be a contiguous vector of ", b.size(0),
                     " values on the operands' device");
     c10::cuda::CUDAGuard guard(a.device());
-    const int M = to_int(a.size(0), "fp8.matmul"), N = to_int(b.size(0), "fp8.matmul"), K = to_int(a.size(1), "fp8.matmul");
-    const int64_t ld = aligned_rows ? ((int64_t)N + 7) / 8 * 8 : N;
-    Tensor out = device_empty({M, ld}, type, a);
-    if (ld != N) out = out.narrow(1, 0, N);
-    check(vnm_fp8_matmul(a.data_ptr(), packed_ld(a), sa.data_ptr(), f8_code(a.scalar_type(), "fp8.matmul"), b.data_ptr(), packed_ld(b), sb.data_ptr(),
-                         f8_code(b.scalar_type(), "fp8.matmul"), M, N, K, with_bias ? bias->data_ptr() : nullptr, with_bias ? type_code(bias->scalar_type(), "fp8.matmul: bias") : VNM_F32,
-                         out.data_ptr(), type_code(type, "fp8.matmul"), std::max<int64_t>(1, ld), c10::cuda::getCurrentCUDAStream().stream()),
-          "vnm_fp8_matmul");
-    return out;
+    return multiply({a, sa}, {b, sb}, bias, type, a);
 }
 
-using Gelu = std::tuple<OptTensor, OptTensor, OptTensor, OptTensor, OptTensor, OptTensor, OptTensor>;
+struct Gelu {
+    Tensor y;
+    Packed rows, cols, ckpt;
+};
 
-// (y, data, scales, data_t, scales_t, checkpoint, its scales), None for what is not wanted
 Gelu gelu(const Tensor &x_in, bool tanh_form, bool y_wanted, bool rows_wanted, bool cols_wanted, bool ckpt_wanted)
 {
     const Tensor x = as_rows(x_in, "fp8.gelu");
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t rows = x.size(0), cols = x.size(1);
     const int type = type_code(x.scalar_type(), "fp8.gelu"), r = to_int(rows, "fp8.gelu"), c = to_int(cols, "fp8.gelu");
-    Packed a, t, k;
-    Tensor y;
-    if (y_wanted) y = device_empty({rows, cols}, x.scalar_type(), x);
-    if (rows_wanted) a = pack(rows, cols, torch::kFloat8_e4m3fn, x);
-    if (cols_wanted) t = pack(cols, rows, torch::kFloat8_e4m3fn, x);
-    if (ckpt_wanted) k = pack(rows, cols, torch::kFloat8_e4m3fn, x);
-    check(vnm_fp8_gelu(x.data_ptr(), type, row_stride(x), r, c, tanh_form, ptr(y), std::max<int64_t>(1, cols), a.values(), a.ld, a.scale(), t.values(), t.ld, t.scale(), k.values(), k.ld,
-                       k.scale(), c10::cuda::getCurrentCUDAStream().stream()),
+    Gelu g = {Tensor(), pack(rows_wanted, rows, cols, torch::kFloat8_e4m3fn, x), pack(cols_wanted, cols, rows, torch::kFloat8_e4m3fn, x),
+              pack(ckpt_wanted, rows, cols, torch::kFloat8_e4m3fn, x)};
+    if (y_wanted) g.y = device_empty({rows, cols}, x.scalar_type(), x);
+    check(vnm_fp8_gelu(x.data_ptr(), type, row_stride(x), r, c, tanh_form, ptr(g.y), std::max<int64_t>(1, cols), g.rows.values(), g.rows.ld, g.rows.scale(), g.cols.values(), g.cols.ld,
+                       g.cols.scale(), g.ckpt.values(), g.ckpt.ld, g.ckpt.scale(), c10::cuda::getCurrentCUDAStream().stream()),
           "vnm_fp8_gelu");
-    return Gelu(opt(y), opt(a.data), opt(a.scales), opt(t.data), opt(t.scales), opt(k.data), opt(k.scales));
+    return g;
 }
 
-using GeluGrad = std::tuple<OptTensor, OptTensor, OptTensor, OptTensor, OptTensor, OptTensor>;
+struct GeluGrad {
+    Tensor dx;
+    Both both;                   // of dx in 8 bits
+};
 
-// (dx, data, scales, data_t, scales_t, column sums), None for what is not wanted
-GeluGrad gelu_grad(const Tensor &dy_in, const Tensor &ckpt, const Tensor &ckpt_scales, bool tanh_form, bool dx_wanted, c10::ScalarType f8, bool rows_wanted, bool cols_wanted,
-                   c10::optional<c10::ScalarType> sums_type)
+GeluGrad gelu_grad(const Tensor &dy_in, const Packed &ckpt, bool tanh_form, bool dx_wanted, c10::ScalarType f8, bool rows_wanted, bool cols_wanted, c10::optional<c10::ScalarType> sums_type)
 {
     const Tensor dy = as_rows(dy_in, "fp8.gelu");
-    check_packed(ckpt, ckpt_scales, "fp8.gelu: checkpoint");
-    TORCH_CHECK(ckpt.scalar_type() == torch::kFloat8_e4m3fn && ckpt.size(0) == dy.size(0) && ckpt.size(1) == dy.size(1) && ckpt.device() == dy.device(),
-                "fp8.gelu: the checkpoint does not belong to this gradient");
+    TORCH_CHECK(ckpt.rows == dy.size(0) && ckpt.cols == dy.size(1) && ckpt.bytes.device() == dy.device(), "fp8.gelu: the checkpoint does not belong to this gradient");
     c10::cuda::CUDAGuard guard(dy.device());
     const int64_t rows = dy.size(0), cols = dy.size(1);
     const int type = type_code(dy.scalar_type(), "fp8.gelu"), r = to_int(rows, "fp8.gelu"), c = to_int(cols, "fp8.gelu"), code = f8_code(f8, "fp8.gelu");
-    Packed a, t;
-    Tensor dx;
-    if (dx_wanted) dx = device_empty({rows, cols}, dy.scalar_type(), dy);
-    if (rows_wanted) a = pack(rows, cols, f8, dy);
-    if (cols_wanted) t = pack(cols, rows, f8, dy);
-    const Tensor sums = undefined_or_sums(sums_type, cols, dy), ws = sums_workspace(sums, rows, cols, dy);
-    check(vnm_fp8_gelu_grad(dy.data_ptr(), type, row_stride(dy), r, c, tanh_form, ckpt.data_ptr(), packed_ld(ckpt), ckpt_scales.data_ptr(), ptr(dx), std::max<int64_t>(1, cols), code,
-                            a.values(), a.ld, a.scale(), t.values(), t.ld, t.scale(), ptr(sums), sums_type.has_value() ? type_code(*sums_type, "fp8.gelu") : VNM_F32, ptr(ws),
-                            c10::cuda::getCurrentCUDAStream().stream()),
+    GeluGrad g = {Tensor(), {pack(rows_wanted, rows, cols, f8, dy), pack(cols_wanted, cols, rows, f8, dy), undefined_or_sums(sums_type, cols, dy)}};
+    if (dx_wanted) g.dx = device_empty({rows, cols}, dy.scalar_type(), dy);
+    const Tensor ws = sums_workspace(g.both.sums, rows, cols, dy);
+    check(vnm_fp8_gelu_grad(dy.data_ptr(), type, row_stride(dy), r, c, tanh_form, ckpt.values(), ckpt.ld, ckpt.scale(), ptr(g.dx), std::max<int64_t>(1, cols), code, g.both.rows.values(),
+                            g.both.rows.ld, g.both.rows.scale(), g.both.cols.values(), g.both.cols.ld, g.both.cols.scale(), ptr(g.both.sums),
+                            sums_type.has_value() ? type_code(*sums_type, "fp8.gelu") : VNM_F32, ptr(ws), c10::cuda::getCurrentCUDAStream().stream()),
           "vnm_fp8_gelu_grad");
-    return GeluGrad(opt(dx), opt(a.data), opt(a.scales), opt(t.data), opt(t.scales), opt(sums));
+    return g;
 }
 
 // ---- differentiable operators ----
@@ -274,60 +293,64 @@ Tensor shaped(const Tensor &y, at::IntArrayRef shape)
     return y.view(s);
 }
 
-struct Operand {
-    Tensor data, scales;
-};
-struct Both {
-    Operand rows, cols;
-    Tensor sums;
-};
 Tensor or_undefined(const OptTensor &t) { return t.has_value() ? *t : Tensor(); }
 c10::optional<c10::ScalarType> type_of(bool wanted, c10::ScalarType t) { return wanted ? c10::optional<c10::ScalarType>(t) : c10::nullopt; }
 
 Both quantized(const Tensor &x, c10::ScalarType f8, bool square, bool rows, bool cols, c10::optional<c10::ScalarType> sums)
 {
     if (!rows && !cols) return {};
-    const Quantized q = quantize(x, f8, square, rows, cols, sums);
-    return {{or_undefined(std::get<0>(q)), or_undefined(std::get<1>(q))}, {or_undefined(std::get<2>(q)), or_undefined(std::get<3>(q))}, or_undefined(std::get<4>(q))};
+    return quantize(x, f8, square, rows, cols, sums);
 }
-Tensor product(const Operand &a, const Operand &b, const Tensor &bias, c10::ScalarType type, bool aligned_rows = false)
+// a b^T (+ bias); zeros where there is nothing to sum (a gradient without any token or output)
+Tensor product(const Packed &a, const Packed &b, const Tensor &bias, c10::ScalarType type, bool aligned_rows = false)
 {
-    return matmul(a.data, a.scales, b.data, b.scales, bias.defined() ? OptTensor(bias.detach().contiguous()) : c10::nullopt, type, aligned_rows);
-}
-// dy^T x from the transposes; zeros without any token
-Tensor weight_grad(const Operand &dy_t, const Operand &x_t, c10::ScalarType type)
-{
-    if (dy_t.data.size(1) == 0) return torch::zeros({dy_t.data.size(0), x_t.data.size(0)}, dy_t.data.options().dtype(type));
-    return product(dy_t, x_t, Tensor(), type);
+    c10::cuda::CUDAGuard guard(a.bytes.device());
+    if (a.cols == 0) return torch::zeros({a.rows, b.rows}, a.bytes.options().dtype(type));
+    return multiply(a, b, bias.defined() ? bias.detach().contiguous() : bias, type, a.bytes, aligned_rows);
 }
 
+// What a node keeps besides tensors, as one list: a shape behind N numbers.
+template <size_t N>
+void keep(AutogradContext *ctx, const std::array<int64_t, N> &numbers, at::IntArrayRef shape)
+{
+    std::vector<int64_t> v(numbers.begin(), numbers.end());
+    v.insert(v.end(), shape.begin(), shape.end());
+    ctx->saved_data["kept"] = std::move(v);
+}
+struct Kept {
+    std::vector<int64_t> v;
+    size_t n;
+    Kept(AutogradContext *ctx, size_t numbers) : v(ctx->saved_data["kept"].toIntVector()), n(numbers) {}
+    int64_t operator[](size_t i) const { return v[i]; }
+    c10::ScalarType type(size_t i) const { return (c10::ScalarType)v[i]; }
+    at::IntArrayRef shape() const { return at::IntArrayRef(v).slice(n); }
+};
+Tensor viewed(const Tensor &t, at::IntArrayRef shape) { return t.sizes() == shape ? t : t.view(shape); }
+
 struct Linear : torch::autograd::Function<Linear> {
+    enum { X_TYPE, W_TYPE, BIAS_TYPE, GRAD_TYPE, HAS_BIAS, TOKENS, IN, OUT, NUMBERS };
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &opt_bias, c10::ScalarType grad_type, bool record)
     {
         const Tensor bias = or_undefined(opt_bias);
         const bool need_x = record && wants_grad(x), need_w = record && wants_grad(w);
-        Both xs = quantized(flat(x), torch::kFloat8_e4m3fn, false, true, need_w, c10::nullopt);
-        Both ws = quantized(w, torch::kFloat8_e4m3fn, true, true, need_x, c10::nullopt);
+        const Both xs = quantized(flat(x), torch::kFloat8_e4m3fn, false, true, need_w, c10::nullopt);
+        const Both ws = quantized(w, torch::kFloat8_e4m3fn, true, true, need_x, c10::nullopt);
         const Tensor y = product(xs.rows, ws.rows, bias, x.scalar_type());
-        ctx->save_for_backward({xs.cols.data, xs.cols.scales, ws.cols.data, ws.cols.scales});
-        ctx->saved_data["shape"] = x.sizes().vec();
-        ctx->saved_data["x"] = (int64_t)x.scalar_type();
-        ctx->saved_data["w"] = (int64_t)w.scalar_type();
-        ctx->saved_data["b"] = (int64_t)(bias.defined() ? bias.scalar_type() : x.scalar_type());
-        ctx->saved_data["grad"] = (int64_t)grad_type;
-        ctx->saved_data["bias"] = bias.defined();
+        ctx->save_for_backward({xs.cols.bytes, ws.cols.bytes});
+        keep<NUMBERS>(ctx, {(int64_t)x.scalar_type(), (int64_t)w.scalar_type(), (int64_t)(bias.defined() ? bias.scalar_type() : x.scalar_type()), (int64_t)grad_type, bias.defined(),
+                            xs.rows.rows, w.size(1), w.size(0)}, x.sizes());
         return shaped(y, x.sizes());
     }
     static variable_list backward(AutogradContext *ctx, variable_list dys)
     {
         const variable_list saved = ctx->get_saved_variables();
+        const Kept kept(ctx, NUMBERS);
         // counted over the tensors that there are
-        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
-        auto type = [&](const char *k) { return (c10::ScalarType)ctx->saved_data[k].toInt(); };
-        const Both g = quantized(flat(dys[0]), type("grad"), false, need_x, need_w || need_b, type_of(need_b, type("b")));
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = kept[HAS_BIAS] && ctx->needs_input_grad(2);
+        const Both g = quantized(flat(dys[0]), kept.type(GRAD_TYPE), false, need_x, need_w || need_b, type_of(need_b, kept.type(BIAS_TYPE)));
         Tensor dx, dw;
-        if (need_x) dx = product(g.rows, {saved[2], saved[3]}, Tensor(), type("x")).view(ctx->saved_data["shape"].toIntVector());
-        if (need_w) dw = weight_grad(g.cols, {saved[0], saved[1]}, type("w"));
+        if (need_x) dx = viewed(product(g.rows, unpacked(saved[1], kept[IN], kept[OUT]), Tensor(), kept.type(X_TYPE)), kept.shape());
+        if (need_w) dw = product(g.cols, unpacked(saved[0], kept[IN], kept[TOKENS]), Tensor(), kept.type(W_TYPE));
         return once({dx, dw, g.sums, Tensor(), Tensor()}, dys);
     }
 };
@@ -343,19 +366,20 @@ Tensor linear(const Tensor &x, const Tensor &w, const OptTensor &bias, c10::Scal
 }
 
 struct Gelu8 : torch::autograd::Function<Gelu8> {
+    enum { TANH, ROWS, COLS, NUMBERS };
     static Tensor forward(AutogradContext *ctx, const Tensor &x, bool tanh_form, bool record)
     {
         const Gelu g = gelu(flat(x), tanh_form, true, false, false, record && wants_grad(x));
-        ctx->save_for_backward({or_undefined(std::get<5>(g)), or_undefined(std::get<6>(g))});
-        ctx->saved_data["tanh"] = tanh_form;
-        ctx->saved_data["shape"] = x.sizes().vec();
-        return std::get<0>(g)->view(x.sizes());
+        ctx->save_for_backward({g.ckpt.bytes});
+        keep<NUMBERS>(ctx, {tanh_form, g.ckpt.rows, g.ckpt.cols}, x.sizes());
+        return viewed(g.y, x.sizes());
     }
     static variable_list backward(AutogradContext *ctx, variable_list dys)
     {
         const variable_list saved = ctx->get_saved_variables();
-        const GeluGrad g = gelu_grad(flat(dys[0]), saved[0], saved[1], ctx->saved_data["tanh"].toBool(), true, torch::kFloat8_e4m3fn, false, false, c10::nullopt);
-        return once({std::get<0>(g)->view(ctx->saved_data["shape"].toIntVector()), Tensor(), Tensor()}, dys);
+        const Kept kept(ctx, NUMBERS);
+        const GeluGrad g = gelu_grad(flat(dys[0]), unpacked(saved[0], kept[ROWS], kept[COLS]), kept[TANH] != 0, true, torch::kFloat8_e4m3fn, false, false, c10::nullopt);
+        return once({viewed(g.dx, kept.shape()), Tensor(), Tensor()}, dys);
     }
 };
 
@@ -367,48 +391,42 @@ Tensor gelu8(const Tensor &x, bool tanh_form)
 }
 
 struct Mlp : torch::autograd::Function<Mlp> {
+    enum { X_TYPE, W1_TYPE, B1_TYPE, W2_TYPE, B2_TYPE, GRAD_TYPE, TANH, HAS_B1, HAS_B2, TOKENS, IN, HIDDEN, OUT, NUMBERS };
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w1, const OptTensor &opt_b1, const Tensor &w2, const OptTensor &opt_b2, bool tanh_form,
                           c10::ScalarType grad_type, bool record)
     {
         const Tensor b1 = or_undefined(opt_b1), b2 = or_undefined(opt_b2);
         const bool need_x = record && wants_grad(x), need_w1 = record && wants_grad(w1), need_b1 = record && wants_grad(b1), need_w2 = record && wants_grad(w2);
         const bool inner = need_x || need_w1 || need_b1;      // whether the gradient goes back through the GELU
-        Both xs = quantized(flat(x), torch::kFloat8_e4m3fn, false, true, need_w1, c10::nullopt);
-        Both w1s = quantized(w1, torch::kFloat8_e4m3fn, true, true, need_x, c10::nullopt);
-        Gelu a = gelu(product(xs.rows, w1s.rows, b1, x.scalar_type(), true), tanh_form, false, true, need_w2, inner);
-        Both w2s = quantized(w2, torch::kFloat8_e4m3fn, true, true, inner, c10::nullopt);
-        const Tensor y = product({*std::get<1>(a), *std::get<2>(a)}, w2s.rows, b2, x.scalar_type());
-        ctx->save_for_backward({xs.cols.data, xs.cols.scales, w1s.cols.data, w1s.cols.scales, or_undefined(std::get<3>(a)), or_undefined(std::get<4>(a)),
-                                or_undefined(std::get<5>(a)), or_undefined(std::get<6>(a)), w2s.cols.data, w2s.cols.scales});
-        ctx->saved_data["shape"] = x.sizes().vec();
-        ctx->saved_data["x"] = (int64_t)x.scalar_type();
-        ctx->saved_data["w1"] = (int64_t)w1.scalar_type();
-        ctx->saved_data["w2"] = (int64_t)w2.scalar_type();
-        ctx->saved_data["b1"] = (int64_t)(b1.defined() ? b1.scalar_type() : x.scalar_type());
-        ctx->saved_data["b2"] = (int64_t)(b2.defined() ? b2.scalar_type() : x.scalar_type());
-        ctx->saved_data["grad"] = (int64_t)grad_type;
-        ctx->saved_data["tanh"] = tanh_form;
-        ctx->saved_data["bias1"] = b1.defined();
-        ctx->saved_data["bias2"] = b2.defined();
+        const Both xs = quantized(flat(x), torch::kFloat8_e4m3fn, false, true, need_w1, c10::nullopt);
+        const Both w1s = quantized(w1, torch::kFloat8_e4m3fn, true, true, need_x, c10::nullopt);
+        const Gelu a = gelu(product(xs.rows, w1s.rows, b1, x.scalar_type(), true), tanh_form, false, true, need_w2, inner);
+        const Both w2s = quantized(w2, torch::kFloat8_e4m3fn, true, true, inner, c10::nullopt);
+        const Tensor y = product(a.rows, w2s.rows, b2, x.scalar_type());
+        ctx->save_for_backward({xs.cols.bytes, w1s.cols.bytes, a.cols.bytes, a.ckpt.bytes, w2s.cols.bytes});
+        keep<NUMBERS>(ctx, {(int64_t)x.scalar_type(), (int64_t)w1.scalar_type(), (int64_t)(b1.defined() ? b1.scalar_type() : x.scalar_type()), (int64_t)w2.scalar_type(),
+                            (int64_t)(b2.defined() ? b2.scalar_type() : x.scalar_type()), (int64_t)grad_type, tanh_form, b1.defined(), b2.defined(), xs.rows.rows, w1.size(1), w1.size(0),
+                            w2.size(0)}, x.sizes());
         return shaped(y, x.sizes());
     }
     static variable_list backward(AutogradContext *ctx, variable_list dys)
     {
         const variable_list s = ctx->get_saved_variables();
-        const bool has_b1 = ctx->saved_data["bias1"].toBool(), has_b2 = ctx->saved_data["bias2"].toBool();
+        const Kept kept(ctx, NUMBERS);
+        const int64_t tokens = kept[TOKENS], hidden = kept[HIDDEN];
+        const bool has_b1 = kept[HAS_B1] != 0, has_b2 = kept[HAS_B2] != 0;
         const size_t at_w2 = has_b1 ? 3 : 2;      // counted over the tensors that there are
         const bool need_x = ctx->needs_input_grad(0), need_w1 = ctx->needs_input_grad(1), need_b1 = has_b1 && ctx->needs_input_grad(2), need_w2 = ctx->needs_input_grad(at_w2),
                    need_b2 = has_b2 && ctx->needs_input_grad(at_w2 + 1), inner = need_x || need_w1 || need_b1;
-        auto type = [&](const char *k) { return (c10::ScalarType)ctx->saved_data[k].toInt(); };
-        const Both g = quantized(flat(dys[0]), type("grad"), false, inner, need_w2 || need_b2, type_of(need_b2, type("b2")));
+        const Both g = quantized(flat(dys[0]), kept.type(GRAD_TYPE), false, inner, need_w2 || need_b2, type_of(need_b2, kept.type(B2_TYPE)));
         Tensor dx, dw1, db1, dw2;
-        if (need_w2) dw2 = weight_grad(g.cols, {s[4], s[5]}, type("w2"));
+        if (need_w2) dw2 = product(g.cols, unpacked(s[2], hidden, tokens), Tensor(), kept.type(W2_TYPE));
         if (inner) {
-            const Tensor da = product(g.rows, {s[8], s[9]}, Tensor(), type("x"), true);
-            const GeluGrad h = gelu_grad(da, s[6], s[7], ctx->saved_data["tanh"].toBool(), false, type("grad"), need_x, need_w1 || need_b1, type_of(need_b1, type("b1")));
-            db1 = or_undefined(std::get<5>(h));
-            if (need_x) dx = product({*std::get<1>(h), *std::get<2>(h)}, {s[2], s[3]}, Tensor(), type("x")).view(ctx->saved_data["shape"].toIntVector());
-            if (need_w1) dw1 = weight_grad({*std::get<3>(h), *std::get<4>(h)}, {s[0], s[1]}, type("w1"));
+            const Tensor da = product(g.rows, unpacked(s[4], hidden, kept[OUT]), Tensor(), kept.type(X_TYPE), true);
+            const GeluGrad h = gelu_grad(da, unpacked(s[3], tokens, hidden), kept[TANH] != 0, false, kept.type(GRAD_TYPE), need_x, need_w1 || need_b1, type_of(need_b1, kept.type(B1_TYPE)));
+            db1 = h.both.sums;
+            if (need_x) dx = viewed(product(h.both.rows, unpacked(s[1], kept[IN], hidden), Tensor(), kept.type(X_TYPE)), kept.shape());
+            if (need_w1) dw1 = product(h.both.cols, unpacked(s[0], kept[IN], tokens), Tensor(), kept.type(W1_TYPE));
         }
         return once({dx, dw1, db1, dw2, g.sums, Tensor(), Tensor(), Tensor()}, dys);
     }
@@ -423,6 +441,12 @@ Tensor mlp(const Tensor &x, const Tensor &w1, const OptTensor &bias1, const Tens
     check_grad_dtype(grad_type, "fp8.mlp");
     check_capture({&x, &w1, &b1, &w2, &b2});
     return Mlp::apply(x, w1, bias1, w2, bias2, tanh_form, grad_type, at::GradMode::is_enabled());
+}
+
+std::tuple<Tensor, Tensor> gelu_quantize(const Tensor &x, bool tanh_form)
+{
+    const Gelu g = gelu(x, tanh_form, false, true, false, false);
+    return {g.rows.data(), g.rows.scales()};
 }
 
 int64_t device_status()
@@ -453,19 +477,21 @@ PyObject *py_quantize(PyObject *, PyObject *const *args, Py_ssize_t n)
     const Tensor &x = tensor_of(args[0]);
     const c10::ScalarType f8 = dtype_of(args[1]);
     const bool square = args[2] == Py_True, both = args[3] == Py_True;
-    Quantized q;
+    Tensor parts[4];
     {
         pybind11::gil_scoped_release no_gil;
-        q = quantize(x, f8, square, true, both, c10::nullopt);
+        const Both q = quantize(x, f8, square, true, both, c10::nullopt);
+        parts[0] = q.rows.data();
+        parts[1] = q.rows.scales();
+        if (both) {
+            parts[2] = q.cols.data();
+            parts[3] = q.cols.scales();
+        }
     }
-    PyObject *out = PyTuple_New(both ? 4 : 2);
+    const int count = both ? 4 : 2;
+    PyObject *out = PyTuple_New(count);
     if (!out) return nullptr;
-    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(*std::get<0>(q))));
-    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(*std::get<1>(q))));
-    if (both) {
-        PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::move(*std::get<2>(q))));
-        PyTuple_SET_ITEM(out, 3, THPVariable_Wrap(std::move(*std::get<3>(q))));
-    }
+    for (int i = 0; i < count; i++) PyTuple_SET_ITEM(out, i, THPVariable_Wrap(std::move(parts[i])));
     return out;
     END_HANDLE_TH_ERRORS
 }
@@ -476,7 +502,7 @@ PyObject *py_matmul(PyObject *, PyObject *const *args, Py_ssize_t n)
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == 6, "matmul(a, a_scales, b, b_scales, bias, dtype)");
     const Tensor &a = tensor_of(args[0]), &sa = tensor_of(args[1]), &b = tensor_of(args[2]), &sb = tensor_of(args[3]);
-    const OptTensor bias = args[4] == Py_None ? c10::nullopt : OptTensor(tensor_of(args[4]));
+    const Tensor bias = args[4] == Py_None ? Tensor() : tensor_of(args[4]);
     const c10::ScalarType type = dtype_of(args[5]);
     Tensor out;
     {
@@ -499,7 +525,7 @@ void define_fp8(pybind11::module &mod)
     using release = pybind11::call_guard<pybind11::gil_scoped_release>;
     if (PyModule_AddFunctions(mod.ptr(), fast_calls) != 0) throw pybind11::error_already_set();
     mod.def("fp8_dequantize", &dequantize, "vnm_fp8_dequantize with its allocation", release());
-    mod.def("fp8_gelu", &gelu, "vnm_fp8_gelu with its allocations", release());
+    mod.def("fp8_gelu_quantize", &gelu_quantize, "GELU of a matrix in 8 bits: (data, scales)", release());
     mod.def("fp8_linear", &linear, "A differentiable linear layer in 8 bits", release());
     mod.def("fp8_gelu8", &gelu8, "GELU with an 8-bit checkpoint for its gradient", release());
     mod.def("fp8_mlp", &mlp, "A differentiable feed-forward block in 8 bits", release());

@@ -233,8 +233,7 @@ class Fp8Mlp(_Held):
         self._refuse_gradients(input)
         _check_input(input, "Fp8Mlp")
         h = matmul(quantize(_flat(input)), self._weight("fc"), self.fc_bias, input.dtype)
-        _, a, sa, _, _, _, _ = _call("fp8_gelu", h, self.tanh_form, False, True, False, False)
-        y = matmul(BlockFp8(a, sa), self._weight("proj"), self.proj_bias, input.dtype)
+        y = matmul(BlockFp8(*_call("fp8_gelu_quantize", h, self.tanh_form)), self._weight("proj"), self.proj_bias, input.dtype)
         return y if input.dim() == 2 else y.reshape(*input.shape[:-1], self.out_features)
 
 
