@@ -46,6 +46,13 @@ def test_quantize_refuses_what_no_launch_can_index(lib):
     assert quantize(lib, rows=big, cols=big, ldx=big, ldd=2 ** 31) == UNSUPPORTED
 
 
+def test_products_that_no_launch_can_index(lib):
+    big = 2 ** 31 - 1
+    assert matmul(lib, M=big, N=big, ldo=big) == UNSUPPORTED
+    assert lib.vnm_fp8_matmul_config(big, big, 64, F16, 1, 0, None, None, None, None) == UNSUPPORTED
+    assert lib.vnm_fp8_matmul_config(8, 8, big, F16, 1, 0, None, None, None, None) == UNSUPPORTED
+
+
 def test_empty_matrices_are_no_work(lib):
     assert quantize(lib, rows=0) == 0
     assert quantize(lib, cols=0) == 0

@@ -199,6 +199,26 @@ def test_rows_that_begin_anywhere(dtype, cols):
         assert bool((y[:start] == 7).all()) and bool((y[start + 11 * cols:] == 7).all())
 
 
+@pytest.mark.parametrize("f8", [E4M3, E5M2])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 9), (257, 511), (128, 512), (1000, 130), (2, 4099)])
+def test_dequantize(rows, cols, dtype, f8):
+    """Every value is exact in 32 bits, so it is rounded once; rows of the result may begin anywhere."""
+    x, t = matrix(rows, cols, 5), TYPES[dtype]
+    x[0, 0] = float("nan")
+    q = fp8.quantize(x, f8)
+    want = value64(x, f8).float().to(t)
+    same = lambda got: bool(((got == want) | (got.isnan() & want.isnan())).all())
+    assert q.dequantize(t).dtype == t and same(q.dequantize(t))
+    code, lib = {"fp16": 1, "bf16": 2, "fp32": 0}[dtype], capi.lib()
+    for shift, ldo in ((1, cols + 3), (2, cols + 6), (0, cols + 8)):
+        base = torch.full((rows * ldo + 8,), 7.0, dtype=t, device="cuda")
+        assert lib.vnm_fp8_dequantize(q.data.data_ptr(), q.data.stride(0), q.scales.data_ptr(), 0 if f8 == E4M3 else 1, rows, cols, base[shift:].data_ptr(), code, ldo,
+                                      torch.cuda.current_stream().cuda_stream) == 0
+        out = base[shift: shift + rows * ldo].view(rows, ldo)
+        assert same(out[:, :cols]) and bool((base[:shift] == 7).all()) and bool((out[:, cols:] == 7).all()) and bool((base[shift + rows * ldo:] == 7).all())
+
+
 def test_quantize_long_rows_and_many_rows():
     """Offsets past 32 bits in the input and the result."""
     free, _ = torch.cuda.mem_get_info()

@@ -1,6 +1,6 @@
 // The block-scaled 8-bit operators in the `spatha` extension: checks, allocations and the C ABI's calls, on torch's current stream, and the
-// differentiable operators as autograd nodes (a step of a small layer takes as long as the host takes to queue it: in Python 85 us for a GELU and its
-// gradient, see fp8.py for what the calls mean).
+// differentiable operators as autograd nodes (see fp8.py for what the calls mean).  A step of a small layer takes as long as the host takes to queue it: a GELU and
+// its gradient 85 us as a Python node, 53 here, of which torch's engine is 45.
 #include <torch/extension.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>

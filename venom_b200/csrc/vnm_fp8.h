@@ -39,7 +39,8 @@ struct Fp8QuantParams {
 cudaError_t launch_fp8_rows(const Fp8QuantParams &p, int type, int op, cudaStream_t stream);
 cudaError_t launch_fp8_tiles(const Fp8QuantParams &p, int type, int op, bool square, cudaStream_t stream);
 cudaError_t launch_fp8_colsum(const float *partial, int blocks, int cols, void *out, int type, cudaStream_t stream);
-cudaError_t launch_fp8_dequantize(const uint8_t *data, int64_t ldd, const uint8_t *scales, int f8, int rows, int cols, void *out, int type, int64_t ldo, cudaStream_t stream);
+cudaError_t launch_fp8_dequantize(const uint8_t *data, int64_t ldd, const uint8_t *scales, int f8, int rows, int cols, void *out, int type, int64_t ldo, int align,
+                                  cudaStream_t stream);
 
 // n / d of 0 <= n < 2^31 by a multiplication: with 2^(s - 1) < d <= 2^s and m = floor(2^(31 + s) / d) + 1, m d - 2^(31 + s) is at most 2^s, so that
 // floor(n m / 2^(31 + s)) is the quotient (Granlund and Montgomery, 1994).

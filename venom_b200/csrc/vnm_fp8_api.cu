@@ -66,6 +66,13 @@ int check_sums(const char *name, const void *colsum, int type, const void *works
     return VNM_OK;
 }
 
+int check_product_size(const char *name, int M, int N, int K)
+{
+    if (K > INT32_MAX - 256 || M > INT32_MAX - 256 || N > INT32_MAX - 256 || ((int64_t)M + 15) / 16 * (((int64_t)N + 127) / 128) > INT32_MAX / 8)
+        return fail(VNM_ERR_UNSUPPORTED, "%s: %d x %d x %d is too large", name, M, N, K);
+    return VNM_OK;
+}
+
 bool pieces(const void *x, int type, int64_t ld) { return aligned(x, 16) && ld * elem_size(type) % 16 == 0; }
 
 int row_alignment(const void *x, int type, int64_t ld)
@@ -201,7 +208,7 @@ extern "C" int vnm_fp8_dequantize(const void *data, int64_t ldd, const void *sca
     VNM_TRY(check_f8(name, "the input", data, ldd, scales, rows, cols));
     VNM_TRY(check_value(name, "the result", out, ldo, out_type, rows, cols));
     return done(launch_fp8_dequantize(static_cast<const uint8_t *>(data), ldd, static_cast<const uint8_t *>(scales), f8_type, rows, cols, out, out_type, ldo,
-                                      static_cast<cudaStream_t>(stream)), name);
+                                      row_alignment(out, out_type, ldo), static_cast<cudaStream_t>(stream)), name);
 }
 
 extern "C" int vnm_fp8_gelu(const void *x, int x_type, int64_t ldx, int rows, int cols, int tanh_form, void *y, int64_t ldy, void *data, int64_t ldd, void *scales,
@@ -270,8 +277,7 @@ extern "C" int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, 
     VNM_TRY(check_f8(name, "B", b, ldb, b_scales, N, K));
     VNM_TRY(check_value(name, "the result", out, ldo, out_type, M, N));
     if (bias && !aligned(bias, (uintptr_t)elem_size(bias_type))) return fail(VNM_ERR_BAD_ARG, "%s: bias is not aligned to its type", name);
-    if (K > INT32_MAX - 256 || M > INT32_MAX - 256 || N > INT32_MAX - 256 || ((int64_t)M + 15) / 16 * (((int64_t)N + 127) / 128) > INT32_MAX / 8)
-        return fail(VNM_ERR_UNSUPPORTED, "%s: %d x %d x %d is too large", name, M, N, K);
+    VNM_TRY(check_product_size(name, M, N, K));
     int *status = nullptr;
     VNM_TRY(device_ready(&status));
     const EncodeTiledFn enc = get_encode_fn();
@@ -308,6 +314,7 @@ extern "C" int vnm_fp8_matmul_config(int M, int N, int K, int out_type, int whol
     const char *name = "vnm_fp8_matmul_config";
     if (M < 1 || N < 1 || K < 1) return fail(VNM_ERR_BAD_ARG, "%s: sizes must be positive (got %d, %d, %d)", name, M, N, K);
     if (!known_type(out_type)) return fail(VNM_ERR_BAD_ARG, "%s: unknown type %d", name, out_type);
+    VNM_TRY(check_product_size(name, M, N, K));
     int *status = nullptr;
     VNM_TRY(device_ready(&status));
     Fp8Plan plan = {};
