@@ -370,17 +370,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
         *abort_flag = 0;
         fence_barrier_init();
     }
-    grid_dependency_wait();
-    if (warp == 3) {
-        tmem_alloc2(tmem_slot, TMEM_COLS);
-        tmem_relinquish2();
-    }
-    tc_fence_before();
-    __syncthreads();
     cluster_sync_all();                                 // both CTAs' barriers exist before anyone arrives on them remotely
-    tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
-    grid_launch_dependents();
+    grid_dependency_wait();
+    // The loads begin at once; whoever uses tensor memory meets behind its allocation.  (The first MMA waits for the scale words of both CTAs, so for both allocations.)
+    if (warp >= 2) {
+        if (warp == 3) {
+            tmem_alloc2(tmem_slot, TMEM_COLS);
+            tmem_relinquish2();
+        }
+        tc_fence_before();
+        named_barrier_sync(1, NUM_THREADS - 64);
+        tc_fence_after();
+        grid_launch_dependents();
+    }
 
     if (warp < 2) {
         // ---------------- loads ----------------
@@ -416,6 +418,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
     } else if (warp == 2) {
         // ---------------- MMA issuer ----------------
         if (leader && elect_one()) {
+            const uint32_t tmem_base = *tmem_slot;
             const uint32_t idesc0 = make_idesc_mxf8(256, BN, p.a_f8, p.b_f8);
             const uint64_t adesc0 = make_smem_desc(smem_u32(a_ring), 16, 1024, 2), bdesc0 = make_smem_desc(smem_u32(b_ring), 16, 1024, 2);
             int s = 0, left = total_it, gleft = my_tiles * groups, set = 0;
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
         __syncwarp();
     } else if (warp >= SCALE_WARP0 && warp < EPI_WARP0) {
         // ---------------- scale words ----------------
-        const uint32_t quarter = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t quarter = *tmem_slot + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t ready = mapa_shared(smem_u32(sf_full), 0);
         uint32_t next[12];
         auto fetch = [&](int tile, int g) {
@@ -488,6 +491,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
         const int q = warp & 3, part = (warp - EPI_WARP0) >> 2;
         constexpr int REST = BN - 128;
         const int cols = part == 0 ? 128 : REST;
+        const uint32_t tmem_base = *tmem_slot;
         uint8_t *own = smem + S * T::STAGE_BYTES + (warp - EPI_WARP0) * T::WARP_BYTES;
         uint4 *stage = reinterpret_cast<uint4 *>(own);
         float4 *bias = reinterpret_cast<float4 *>(own + T::WARP_BYTES - 512);      // 32 columns before: part 1, !WHOLE
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
     cluster_sync_all();      // the peer's shared and tensor memory stay until the leader's last MMA is done: the epilogues have seen its accumulator full
     if (warp == 3) {
         tc_fence_after();
-        tmem_dealloc2(tmem_base, TMEM_COLS);
+        tmem_dealloc2(*tmem_slot, TMEM_COLS);
     }
 }
 

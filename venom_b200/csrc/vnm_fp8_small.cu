@@ -119,16 +119,21 @@ __global__ void __launch_bounds__(SMALL_THREADS, 2) fp8_small_kernel(const __gri
         *fills = 0;
         fence_barrier_init();
     }
-    grid_dependency_wait();
-    if (warp == 3) {
-        tmem_alloc(tmem_slot, T::TMEM_COLS);
-        tmem_relinquish();
-    }
-    tc_fence_before();
     __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
-    grid_launch_dependents();
+    grid_dependency_wait();
+    // The loads begin at once; whoever uses tensor memory meets behind its allocation.
+    uint32_t tmem_base = 0;
+    if (warp >= 2) {
+        if (warp == 3) {
+            tmem_alloc(tmem_slot, T::TMEM_COLS);
+            tmem_relinquish();
+        }
+        tc_fence_before();
+        named_barrier_sync(1, SMALL_THREADS - 64);
+        tc_fence_after();
+        tmem_base = *tmem_slot;
+        grid_launch_dependents();
+    }
 
     if (warp < 2) {
         // ---------------- loads: warp 0 rows of B, warp 1 rows of A ----------------
