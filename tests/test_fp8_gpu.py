@@ -714,6 +714,39 @@ def test_frozen_mlp_and_conversion():
     assert torch.equal(conv[0](x), a) and torch.equal(conv(x), fp8.linear(torch.nn.functional.gelu(a), net[2].weight, net[2].bias))
 
 
+def test_layers_in_files():
+    import io
+    x = matrix(30, 200, 1, torch.float16)
+    fc, proj = torch.nn.Linear(200, 131).half().cuda(), torch.nn.Linear(131, 72).half().cuda()
+    for layer in (fp8.Fp8Linear(fc), fp8.Fp8Mlp(fc, proj), fp8.Fp8Linear(fc, trainable=True)):
+        with torch.no_grad():
+            want = layer(x)                    # views of the bytes exist when it is written
+            f = io.BytesIO()
+            torch.save(layer, f)
+            f.seek(0)
+            assert torch.equal(torch.load(f, weights_only=False)(x), want) and torch.equal(copy.deepcopy(layer)(x), want)
+
+
+def test_one_tensor_in_several_places():
+    q = fp8.quantize(matrix(150, 260, 1, torch.float16))
+    v = q.dequantize().double()
+    y = fp8.matmul(q, q, dtype=torch.float32)
+    assert bool(((y.double() - v @ v.t()).abs() <= 260 * 2.0 ** -23 * (v.abs() @ v.abs().t())).all())
+    x, w, b = matrix(96, 96, 1, torch.float16), matrix(96, 96, 2, torch.float16), matrix(1, 96, 3, torch.float16)[0].clone()
+    dy = matrix(96, 96, 9, torch.float16)
+    # a weight and a bias that both layers share: the sum of what two of their own get
+    apart = [leaf(t) for t in (x, w, b, w, b)]
+    grads = torch.autograd.grad(fp8.mlp(*apart), apart, dy)
+    x1, w1, b1 = leaf(x), leaf(w), leaf(b)
+    got = torch.autograd.grad(fp8.mlp(x1, w1, b1, w1, b1), (x1, w1, b1), dy)
+    assert torch.equal(got[0], grads[0]) and torch.equal(got[1], grads[1] + grads[3]) and torch.equal(got[2], grads[2] + grads[4])
+    # one leaf as input and as weight
+    apart = [leaf(x), leaf(x)]
+    grads = torch.autograd.grad(fp8.linear(*apart), apart, dy)
+    both = leaf(x)
+    assert torch.equal(torch.autograd.grad(fp8.linear(both, both), both, dy)[0], grads[0] + grads[1])
+
+
 def test_layers_in_inference_mode():
     lin, x = torch.nn.Linear(200, 131).half().cuda(), matrix(30, 200, 1, torch.float16)
     want = fp8.Fp8Linear(lin)(x)

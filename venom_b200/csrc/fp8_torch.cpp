@@ -304,6 +304,7 @@ Both quantized(const Tensor &x, c10::ScalarType f8, bool square, bool rows, bool
 // a b^T (+ bias); zeros where there is nothing to sum (a gradient without any token or output)
 Tensor product(const Packed &a, const Packed &b, const Tensor &bias, c10::ScalarType type, bool aligned_rows = false)
 {
+    TORCH_CHECK(a.bytes.device() == b.bytes.device(), "a saved tensor came back from its hooks on another device");
     c10::cuda::CUDAGuard guard(a.bytes.device());
     if (a.cols == 0) return torch::zeros({a.rows, b.rows}, a.bytes.options().dtype(type));
     return multiply(a, b, bias.defined() ? bias.detach().contiguous() : bias, type, a.bytes, aligned_rows);

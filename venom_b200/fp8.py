@@ -163,6 +163,10 @@ class _Held(torch.nn.Module):
             self._views[name] = (cols, data, q)
         return q
 
+    def __getstate__(self):
+        """Copies and files hold the bytes once: views are made anew."""
+        return dict(self.__dict__, _views={name: (view[0], None, None) for name, view in self._views.items()})
+
     def _refuse_gradients(self, x):
         if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
             raise VenomError("%s holds a frozen weight: build it with trainable=True for gradients" % type(self).__name__)
