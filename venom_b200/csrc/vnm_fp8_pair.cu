@@ -26,7 +26,10 @@ constexpr int SCALE_WARP0 = 4, EPI_WARP0 = 8;
 constexpr int TMEM_COLS = 512;
 constexpr int SF_SETS = 2;
 
-constexpr int WINDOW = 11;       // epilogue: 16-byte pieces between the rows of a window (ten are used): an odd number, so that eight rows lie in different banks
+// Epilogue, rows that begin anywhere: words between the rows of the windows (forty are used), an odd number of 16-byte pieces, so that eight rows lie in different banks;
+// every eight rows are a piece further, so that rows of different phases do, too.
+constexpr int WINDOW = 44;
+__host__ __device__ constexpr int window_at(int row) { return row * WINDOW + 4 * (row >> 3); }
 
 template <int BN, bool WHOLE>
 struct Fp8Pair {
@@ -36,7 +39,7 @@ struct Fp8Pair {
     static constexpr int B_BYTES = HALF_N * 128;
     static constexpr int B_SLOT = (B_BYTES + 1023) / 1024 * 1024;
     static constexpr int STAGE_BYTES = A_BYTES + B_SLOT;
-    static constexpr int WARP_BYTES = (WHOLE ? 4096 : 32 * WINDOW * 16) + 640;   // an epilogue warp's 32 rows, and the bias of its columns and 32 before
+    static constexpr int WARP_BYTES = (WHOLE ? 4096 : 4 * window_at(31) + 4 * WINDOW) + 640;   // an epilogue warp's 32 rows, and the bias of its columns and 32 before
     static constexpr int OUT_BYTES = 8 * WARP_BYTES;
     static constexpr int STAGES = (227 * 1024 - OUT_BYTES - 512 - 1024) / STAGE_BYTES;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 512 + 1024;
@@ -99,10 +102,11 @@ __device__ __forceinline__ void tc_mma2_mxf8(uint32_t d_tmem, uint64_t adesc, ui
 // 128 bytes of each row at a time pass through shared memory and leave in pieces of 16 bytes, eight lanes a row.  Exchanging words between lanes instead, so
 // that nothing passes through shared memory, needs 2.4 times the instructions, and the epilogue's eight warps are what short tiles wait for: 16384 x 4096 x
 // 1024 with a bias 83 us.
-// Rows that begin anywhere (odd numbers of columns) leave in the same pieces, aligned where they go and not where they come from: a piece is cut out of two in
-// shared memory.  A row's window there is 32 bytes of the columns before and 128 new ones, so that a sector between two steps is written once and whole;
-// what costs is sectors written in parts (11844 x 15043, K = 116, bf16: 348 us with words of 4 bytes a lane and single values at the edges of each 128 bytes),
-// and only a tile's edges are.
+// Rows that begin anywhere (odd numbers of columns) leave in the same pieces, aligned where they go and not where they come from: the lane that owns a row writes it
+// into its window word by word, as far behind a sector's begin as it will lie in memory (16 bits: words shifted by a half where it begins inside one).  What
+// a step leaves behind its last whole 128 bytes is where the next one begins, so that a sector between two steps is written once and whole; what costs
+// is sectors written in parts (11844 x 15043, K = 116, bf16: 348 us with words of 4 bytes a lane and single values at the edges of each 128 bytes), and only a tile's edges
+// are.  Windows as the columns lie, and pieces cut out of five words when they are read: TODO.
 template <int TYPE>
 __device__ __forceinline__ uint32_t pack16(float a, float b)
 {
@@ -186,8 +190,11 @@ __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n
     uint8_t *out = reinterpret_cast<uint8_t *>(p.out) + row0 * pitch + (int64_t)n0 * SIZE;
     const int rows = p.M - row0 < 32 ? (int)(p.M - row0) : 32;     // that there are; may be none
     const int bytes = (p.N - n0 < cols ? p.N - n0 : cols) * SIZE;   // of a row to store; may be none
-    uint4 *const mine = stage + lane * (WHOLE ? 8 : WINDOW);
-    uint32_t before[8];                                            // !WHOLE: the 32 bytes ahead of these columns
+    uint4 *const mine = stage + lane * 8;                          // WHOLE
+    uint32_t *const words = reinterpret_cast<uint32_t *>(stage), *const own = words + window_at(lane);   // !WHOLE
+    const int phase = (int)(reinterpret_cast<uintptr_t>(out + lane * pitch) & 31), at = phase >> 2;     // of this lane's row in its sector; the same in each step
+    const uint32_t shifted = phase & 2 ? 0x5432u : 0x7654u;        // the word before and this one, or this one
+    uint32_t last = 0;                                             // word before the next one
     if constexpr (!WHOLE) {
         if (part == 1) {                                           // the first part leaves the sector between the two to this one
             uint32_t u[32];
@@ -195,8 +202,13 @@ __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n
             wait_for(u);
             uint32_t w[TYPE == T_F32 ? 32 : 16];
             round32<TYPE, BIAS>(u, bias - 8, w);
+            __syncwarp();                                          // the tile before has been read
 #pragma unroll
-            for (int i = 0; i < 8; i++) before[i] = w[(TYPE == T_F32 ? 24 : 8) + i];
+            for (int i = 1; i < 8; i++) {
+                constexpr int FROM = TYPE == T_F32 ? 24 : 8;
+                if (at - 8 + i >= 0) own[at - 8 + i] = TYPE == T_F32 ? w[FROM + i] : __byte_perm(w[FROM + i - 1], w[FROM + i], shifted);
+            }
+            last = w[TYPE == T_F32 ? 31 : 15];
         }
     }
     uint32_t v[32];
@@ -233,21 +245,25 @@ __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n
             if (h == 0) {
                 __syncwarp();                                      // the columns before have been read
                 if constexpr (!WHOLE) {
-                    mine[0] = make_uint4(before[0], before[1], before[2], before[3]);
-                    mine[1] = make_uint4(before[4], before[5], before[6], before[7]);
+                    if (c0 > 0) {
+                        uint4 *const piece = reinterpret_cast<uint4 *>(own);
+                        const uint4 q0 = piece[8], q1 = piece[9];
+                        piece[0] = q0;
+                        piece[1] = q1;
+                    }
                 }
             }
+            if constexpr (WHOLE) {
 #pragma unroll
-            for (int i = 0; i < PIECES; i++) {
-                const uint4 q = make_uint4(word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
-                if constexpr (WHOLE) mine[(PIECES * h + i) ^ (lane & 7)] = q;
-                else mine[2 + PIECES * h + i] = q;
-            }
-            if constexpr (!WHOLE) {
-                if (h == WIDTH / 32 - 1) {
+                for (int i = 0; i < PIECES; i++) mine[(PIECES * h + i) ^ (lane & 7)] = make_uint4(word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
+            } else if constexpr (TYPE == T_F32) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) before[i] = word[(TYPE == T_F32 ? 24 : 8) + i];
-                }
+                for (int i = 0; i < 32; i++) own[at + i] = word[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) own[at + 16 * h + i] = __byte_perm(i ? word[i ? i - 1 : 0] : last, word[i], shifted);
+                last = word[15];
+                if (h == WIDTH / 32 - 1) own[at + 32] = last >> 16;      // the half that a shift leaves over
             }
         }
         __syncwarp();
@@ -279,51 +295,29 @@ __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n
                 }
             }
         } else if (left > 0) {
-            // Piece q of a row, counted from the sector that these columns begin in (s bytes into it), out of the row's window: five words at a byte offset that
-            // is even.
-            auto cut = [&](const uint32_t *window, int s, int q, uint32_t (&y)[4]) {
-                const int at = 32 + 16 * q - s;
-                const uint32_t *w = window + (at >> 2);
-                const uint32_t half = at & 2 ? 0x5432u : 0x3210u;
-                uint32_t x[5];
-#pragma unroll
-                for (int i = 0; i < 5; i++) x[i] = w[i];
-#pragma unroll
-                for (int i = 0; i < 4; i++) y[i] = __byte_perm(x[i], x[i + 1], half);
-            };
-            const uint32_t *words = reinterpret_cast<const uint32_t *>(stage);
             const bool head = c0 == 0 && part == 0;                                // the sector that the row begins in is another tile's as well
             {
                 uint8_t *row = out + first * pitch;
-                const uint32_t *window = words + first * WINDOW * 4;
 #pragma unroll 4
-                for (int i = 0; i < 8; i++, row += 4 * pitch, window += 16 * WINDOW) {
-                    const int s = (int)(reinterpret_cast<uintptr_t>(row) & 31);
-                    uint32_t y[4];
-                    cut(window, s, piece, y);
-                    if (4 * i + first < rows && 16 * piece >= (head ? s : 0) && 16 * piece + 16 <= s + left)
-                        *reinterpret_cast<uint4 *>(row - s + 16 * piece) = make_uint4(y[0], y[1], y[2], y[3]);
+                for (int i = 0; i < 8; i++, row += 4 * pitch) {
+                    const int r = 4 * i + first, s = (int)(reinterpret_cast<uintptr_t>(row) & 31);
+                    const uint4 q = *reinterpret_cast<const uint4 *>(words + window_at(r) + 4 * piece);
+                    if (r < rows && 16 * piece >= (head ? s : 0) && 16 * piece + 16 <= s + left) *reinterpret_cast<uint4 *>(row - s + 16 * piece) = q;
                 }
             }
             // The last sector, where it is not left to the next columns or the other part; and pieces that begin or end inside: a lane a row.
             const bool tail = left <= 128 && !(part == 0 && p.N - n0 > 128);
             if ((head || tail) && lane < rows) {
-                uint8_t *row = out + lane * pitch;
-                const uint32_t *window = words + lane * WINDOW * 4;
-                const int s = (int)(reinterpret_cast<uintptr_t>(row) & 31), end = s + left;
-                uint32_t y[4];
-                if (head && (s & 15)) {
-                    cut(window, s, s >> 4, y);
-                    store_part(row - s + (s & 16), y, s & 15, end - (s & 16) < 16 ? end - (s & 16) : 16);
-                }
-                if (tail && end >= 144) {
-                    cut(window, s, 8, y);
-                    *reinterpret_cast<uint4 *>(row - s + 128) = make_uint4(y[0], y[1], y[2], y[3]);
-                }
-                if (tail && (end & 15) && !(head && end < ((s + 15) & ~15))) {      // not where head and tail are one piece
-                    cut(window, s, end >> 4, y);
-                    store_part(row - s + (end & ~15), y, 0, end & 15);
-                }
+                uint8_t *row = out + lane * pitch - phase;
+                const int end = phase + left;
+                auto part_of = [&](int q, int from, int to) {
+                    const uint4 v4 = reinterpret_cast<const uint4 *>(own)[q];
+                    const uint32_t y[4] = {v4.x, v4.y, v4.z, v4.w};
+                    store_part(row + 16 * q, y, from, to);
+                };
+                if (head && (phase & 15)) part_of(phase >> 4, phase & 15, end - (phase & 16) < 16 ? end - (phase & 16) : 16);
+                if (tail && end >= 144) *reinterpret_cast<uint4 *>(row + 128) = reinterpret_cast<const uint4 *>(own)[8];
+                if (tail && (end & 15) && !(head && end < ((phase + 15) & ~15))) part_of(end >> 4, 0, end & 15);      // not where head and tail are one piece
             }
         }
     }
