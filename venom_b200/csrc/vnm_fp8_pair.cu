@@ -106,7 +106,8 @@ __device__ __forceinline__ void tc_mma2_mxf8(uint32_t d_tmem, uint64_t adesc, ui
 // into its window word by word, as far behind a sector's begin as it will lie in memory (16 bits: words shifted by a half where it begins inside one).  What
 // a step leaves behind its last whole 128 bytes is where the next one begins, so that a sector between two steps is written once and whole; what costs
 // is sectors written in parts (11844 x 15043, K = 116, bf16: 348 us with words of 4 bytes a lane and single values at the edges of each 128 bytes), and only a tile's edges
-// are.  Windows as the columns lie, and pieces cut out of five words when they are read: TODO.
+// are.  Windows as the columns lie, and pieces cut out of five words when they are read: 8191 x 4095 x 1023, fp16 41.9 us against
+// 37.4, 2978 x 2039 x 1371, fp32 19.0 against 14.3.
 template <int TYPE>
 __device__ __forceinline__ uint32_t pack16(float a, float b)
 {
@@ -138,24 +139,23 @@ __device__ __forceinline__ void add2(uint32_t &a, uint32_t &b, float x, float y)
         : "+r"(a), "+r"(b)
         : "f"(x), "f"(y));
 }
-// What a load of tensor memory has brought is used behind its wait only.
-__device__ __forceinline__ void wait_for(uint32_t (&v)[32])
-{
-    tc_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 32; i++) asm volatile("" : "+r"(v[i]));
-}
-
-// 32 columns from `v` on, rounded and packed.
+// 32 columns of `v`, behind the wait for them, rounded and packed.  The bias is read ahead of the wait.
 template <int TYPE, bool BIAS>
 __device__ __forceinline__ void round32(uint32_t (&v)[32], const float4 *bias, uint32_t (&word)[TYPE == T_F32 ? 32 : 16])
 {
+    float4 b[BIAS ? 8 : 1];
+    if constexpr (BIAS) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) b[i] = bias[i];
+    }
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; i++) asm volatile("" : "+r"(v[i]));
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         if constexpr (BIAS) {
-            const float4 b = bias[i];
-            add2(v[4 * i], v[4 * i + 1], b.x, b.y);
-            add2(v[4 * i + 2], v[4 * i + 3], b.z, b.w);
+            add2(v[4 * i], v[4 * i + 1], b[i].x, b[i].y);
+            add2(v[4 * i + 2], v[4 * i + 3], b[i].z, b[i].w);
         }
         if constexpr (TYPE == T_F32) {
 #pragma unroll
@@ -199,7 +199,6 @@ __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n
         if (part == 1) {                                           // the first part leaves the sector between the two to this one
             uint32_t u[32];
             tc_ld_32x32b_x32(tacc - 32u, u);
-            wait_for(u);
             uint32_t w[TYPE == T_F32 ? 32 : 16];
             round32<TYPE, BIAS>(u, bias - 8, w);
             __syncwarp();                                          // the tile before has been read
@@ -217,7 +216,6 @@ __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n
     if constexpr (HOLD) {
 #pragma unroll
         for (int h = 0; h < 4; h++) {
-            wait_for(v);
             uint32_t word[16];
             round32<TYPE, BIAS>(v, bias + 8 * h, word);
             if (h < 3) tc_ld_32x32b_x32(tacc + (uint32_t)(32 * (h + 1)), v);
@@ -236,7 +234,6 @@ __device__ __forceinline__ void store_columns(uint32_t tacc, int64_t row0, int n
 #pragma unroll
                 for (int i = 0; i < 16; i++) word[i] = held[c0 / 2 + 16 * h + i];
             } else {
-                wait_for(v);
                 round32<TYPE, BIAS>(v, bias + c0 / 4 + 8 * h, word);
                 const int c1 = c0 + 32 * (h + 1);
                 if (c1 < cols) tc_ld_32x32b_x32(tacc + (uint32_t)c1, v);
@@ -579,27 +576,26 @@ cudaError_t fp8_pair_init()
 }
 
 // The cost of a call, us: a start, waves of tiles (between the whole number that the last one makes and the fraction that the power limit sees), and the last
-// tile's epilogue.  A tile takes its k-tiles' time or its epilogue's, whichever is longer (a smooth maximum), or with one accumulator both.  Fitted
-// together with the costs of vnm_fp8_small.cu to steady calls on inputs that change, 431 shapes of 1 to 16384 x 8 to 36864 x 64 to 16384, odd ones and round ones, with and
-// without a bias, fp16 and fp32 results: ratio to the measured time 0.8 to 1.25; over 351 others, in runs long enough for the power limit, the plan chosen from both
-// kernels takes 1.012 of the fastest one's time on average, 1.4 at most (results of 8 to 40 columns).
+// tile's epilogue.  A tile takes its k-tiles' time or its epilogue's, whichever is longer (a smooth maximum), or with one accumulator both.  Both
+// kernels' costs were fitted to steady calls on inputs that change, 802 shapes of 1 to 16384 x 8 to 36864 x 64 to 12288, odd ones and round ones, with and without a bias,
+// fp16 and fp32 results, for the choice that they make: 1.009 of the fastest one's time on average, and 1.012 over 421 others, 1.32 at most (few rows, few columns or few k).
 float fp8_pair_config(int M, int N, int K, bool wide_out, bool whole, bool bias, Fp8Plan *plan)
 {
     if (g_clusters <= 0) return -1.0f;
     static const int widths[4] = {192, 224, 240, 256};
-    static const float ktile[4] = {0.333f, 0.364f, 0.379f, 0.406f};
+    static const float ktile[4] = {0.352f, 0.380f, 0.388f, 0.410f};
     const int64_t mt = ((int64_t)M + 255) / 256;
     const float kt = (float)(((int64_t)K + 127) / 128);
-    const float edge = 1.81f + (wide_out ? 1.28f : 0.0f) + (whole ? 0.0f : wide_out ? 3.16f : 1.88f) + (bias ? 0.62f : 0.0f);
+    const float edge = 1.69f + (wide_out ? 1.20f : 0.0f) + (whole ? 0.0f : 0.98f) + (bias ? 0.58f : 0.0f);
     float best = -1.0f;
     for (int i = 0; i < 4; i++) {
         const int w = widths[i];
         const int64_t nt = ((int64_t)N + w - 1) / w, tiles = mt * nt;
         if (tiles > INT32_MAX / 2) continue;
-        const float waves = 0.72f * (float)((tiles + g_clusters - 1) / g_clusters) + 0.28f * (float)tiles / (float)g_clusters;
+        const float waves = 0.715f * (float)((tiles + g_clusters - 1) / g_clusters) + 0.285f * (float)tiles / (float)g_clusters;
         const float mma = kt * ktile[i], out = edge * (float)w / 240.0f;
-        const float one = w == 256 ? mma + 0.92f * out : powf(powf(mma, 1.233f) + powf(out, 1.233f), 1.0f / 1.233f);
-        const float us = 4.13f + waves * one + 0.21f * out;
+        const float one = w == 256 ? mma + 1.12f * out : powf(powf(mma, 1.1f) + powf(out, 1.1f), 1.0f / 1.1f);
+        const float us = 3.19f + waves * one + 0.26f * out;
         if (best < 0.0f || us < best) {
             best = us;
             plan->bn = w;

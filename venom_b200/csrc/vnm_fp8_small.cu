@@ -316,8 +316,8 @@ cudaError_t fp8_small_init()
 float fp8_small_config(int M, int N, int ktiles, bool wide_out, Fp8Plan *plan)
 {
     struct Cost { float start, kt1, kt2, out, split, bytes; };
-    static const Cost cost[4] = {{1.79f, 0.174f, 0.476f, 1.85f, 0.57f, 0.101f}, {1.92f, 0.173f, 0.477f, 2.79f, 0.65f, 0.091f}, {2.64f, 0.181f, 0.599f, 3.66f, 1.28f, 0.084f},
-                                 {5.27f, 0.253f, 0.911f, 4.00f, 2.91f, 0.106f}};
+    static const Cost cost[4] = {{1.75f, 0.189f, 0.554f, 1.93f, 0.51f, 0.094f}, {1.83f, 0.204f, 0.492f, 2.53f, 0.54f, 0.084f}, {2.46f, 0.257f, 0.496f, 3.95f, 0.21f, 0.077f},
+                                 {5.28f, 0.399f, 0.760f, 2.85f, 1.34f, 0.118f}};
     const int64_t nt = ((int64_t)N + 127) / 128;
     const int sms = g_sms > 0 ? g_sms : 148;
     float best = -1.0f;
