@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 2) fp8_small_kernel(const __gri
     using T = Fp8Small<BN>;
     constexpr int S = T::STAGES;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     uint8_t *w_ring = smem, *x_ring = smem + S * W_TILE_BYTES;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + S * T::STAGE_BYTES);
     uint64_t *freed = full + S;
