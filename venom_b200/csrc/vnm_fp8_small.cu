@@ -311,8 +311,8 @@ cudaError_t fp8_small_init()
 }
 
 // The cost of a call, us: a start, then a CTA's k-tiles (one CTA an SM, or two that share it) or the operands' bytes, whichever takes longer, its epilogue, and the exchange
-// of partial sums.  See fp8_pair_config for what they were fitted to.  (512 x 4096 x 4096: 128 x 64 24.7 us, pairs 14.0;  16 x 36864 x 12288: 128 x 16 71.1, of which
-// the weight's bytes 69.2;  128 x 4096 x 1024: 128 x 32 6.5, pairs 8.2;  8 x 1024 x 1024: 128 x 16 alone 5.0, split by eight 4.1.)
+// of partial sums.  See fp8_pair_config for what they were fitted to.  (512 x 4096 x 4096: 128 x 64 16.2 us, pairs 12.6;  16 x 36864 x 12288: 128 x 16 68.2, all of it
+// the weight's bytes;  128 x 4096 x 1024: 128 x 32 6.2, pairs 6.4;  8 x 1024 x 1024: 128 x 16 alone 4.6, split by eight 3.8.)
 float fp8_small_config(int M, int N, int ktiles, bool wide_out, Fp8Plan *plan)
 {
     struct Cost { float start, kt1, kt2, out, split, bytes; };
