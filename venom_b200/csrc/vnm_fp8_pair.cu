@@ -490,7 +490,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
         const uint32_t tmem_base = *tmem_slot;
         uint8_t *own = smem + S * T::STAGE_BYTES + (warp - EPI_WARP0) * T::WARP_BYTES;
         uint4 *stage = reinterpret_cast<uint4 *>(own);
-        float4 *bias = reinterpret_cast<float4 *>(own + T::WARP_BYTES - 512);      // 32 columns before: part 1, !WHOLE
+        // 32 columns before: part 1, !WHOLE.  Known to be shared memory in every epilogue: 11844 x 15043 x 116 158 -> 148 us.
+        float4 *bias = reinterpret_cast<float4 *>(smem_raw + (-smem_u32(smem_raw) & 1023u) + S * T::STAGE_BYTES + (warp - EPI_WARP0) * T::WARP_BYTES + T::WARP_BYTES - 512);
         // bias of four columns a lane (and of one of the 32 before), on its way while the tile before is stored: as it lies, for a conversion would wait for it
         uint32_t next[5];
         auto fetch = [&](int tile) {
