@@ -685,9 +685,9 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
     uint32_t tile_code = 0;
     bool tile_odd = false;
     if constexpr (SQUARE) {
-        // values that are not negative are ordered like their bits
+        // values that are not negative are ordered like their bits; a thread without a number has NaN, whose bits are above all of them
         auto over_tile = [&](float m) {
-            m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+            m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(m, 0.0f))));
             if (lane == 0) sh.all[warp] = m;
             __syncthreads();
             m = 0.0f;
