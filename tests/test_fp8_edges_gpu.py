@@ -40,3 +40,33 @@ def test_nan_side_by_side_leaves_the_other_values(dtype, f8, where, square):
     q, t = fp8.quantize(x, f8, square=square, both=True)
     check_held(q, x, f8, square)
     check_held(t, x.t(), f8, square)
+
+
+def poisoned(M, N, K, seed):
+    """Operands with NaN and infinities in some rows, and which results they reach."""
+    x, w = matrix(M, K, seed, spread=0.3), matrix(N, K, seed + 1, spread=0.3)
+    bad = torch.zeros((M, N), dtype=torch.bool, device="cuda")
+    for i, v in ((0, math.nan), (M // 2, math.inf), (M - 1, -math.inf)):
+        x[i, (7 * i) % K], bad[i] = v, True
+    for j, v in ((N // 3, math.nan), (N - 1, math.inf)):
+        w[j, (5 * j) % K], bad[:, j] = v, True
+    return x, w, bad
+
+
+# tiles of one SM of every width, split and whole; pairs of every width, rows in whole pieces and not, several tiles for a pair
+@pytest.mark.parametrize("M,N,K", [(16, 136, 512), (17, 128, 640), (33, 1000, 1024), (64, 300, 130), (40, 1000, 4096), (1000, 40, 4096), (2656, 136, 730), (524, 4968, 644), (519, 5680, 632),
+                                   (2306, 5576, 603), (5054, 129, 628), (2049, 4681, 604), (2561, 4993, 670)])
+def test_products_of_values_that_are_not_finite(M, N, K):
+    x, w, bad = poisoned(M, N, K, 1)
+    for dtype in (torch.float16, torch.float32):
+        got = fp8.matmul(fp8.quantize(x), fp8.quantize(w), dtype=dtype)
+        assert torch.equal(got.isnan(), bad)                    # e4m3 holds an infinity as NaN
+    # e5m2 holds it as one: each sum as 64 bits have it
+    a, b = fp8.quantize(x, E5M2), fp8.quantize(w, E5M2)
+    got, xv, wv = fp8.matmul(a, b, dtype=torch.float32), a.dequantize().double(), b.dequantize().double()
+    assert bool(got[~bad].isfinite().all())
+    sums = [(got[i], (xv[i] * wv).sum(1)) for i in (0, M // 2, M - 1)] + [(got[:, j], (xv * wv[j]).sum(1)) for j in (N // 3, N - 1)]
+    for have, want in sums:
+        kinds = lambda t: torch.where(t.isfinite(), 0.0, t.double()).nan_to_num(nan=2.0, posinf=1.0, neginf=-1.0)
+        assert torch.equal(kinds(have), kinds(want))
+    assert fp8.device_status() == 0
