@@ -70,3 +70,60 @@ def test_products_of_values_that_are_not_finite(M, N, K):
         kinds = lambda t: torch.where(t.isfinite(), 0.0, t.double()).nan_to_num(nan=2.0, posinf=1.0, neginf=-1.0)
         assert torch.equal(kinds(have), kinds(want))
     assert fp8.device_status() == 0
+
+
+# ---- frozen layers and their buffers ----
+
+def frozen(cin=200, cout=131, seed=0):
+    torch.manual_seed(seed)
+    return torch.nn.Linear(cin, cout).half().cuda()
+
+
+def test_a_frozen_layer_multiplies_with_the_buffers_that_it_has():
+    """Values or scales replaced alone, by assignment, from a file, or written in place, count in the next call."""
+    x = matrix(30, 200, 1, torch.float16)
+    a, b = fp8.Fp8Linear(frozen(seed=1)), fp8.Fp8Linear(frozen(seed=2))
+    mlp = fp8.Fp8Mlp(frozen(seed=1), frozen(131, 72, 3))
+    y, z = a(x), mlp(x)
+    a.weight_scales = a.weight_scales + 1                                              # every scale twice as large
+    assert torch.equal(a(x), fp8.matmul(fp8.quantize(x), fp8.quantize(2 * frozen(seed=1).weight, square=True), a.bias))
+    a.weight_scales = a.weight_scales - 1
+    assert torch.equal(a(x), y)
+    a.load_state_dict({"weight_scales": a.weight_scales + 1}, strict=False, assign=True)
+    assert not torch.equal(a(x), y)
+    a.load_state_dict({"weight_scales": a.weight_scales - 1}, strict=False)
+    assert torch.equal(a(x), y)
+    a.weight_data, a.weight_scales, a.bias = b.weight_data, b.weight_scales, b.bias
+    assert torch.equal(a(x), b(x))
+    mlp.proj_scales.add_(1)
+    assert not torch.equal(mlp(x), z)
+    mlp.proj_scales = mlp.proj_scales - 1
+    assert torch.equal(mlp(x), z)
+    with pytest.raises(capi.VenomError, match="scales"):
+        b.weight_scales = b.weight_scales[:, :-1]
+        b(x)
+    with pytest.raises(capi.VenomError, match="values"):
+        mlp.fc_data = mlp.fc_data[:, :192]
+        mlp(x)
+
+
+def test_a_frozen_layer_that_leaves_the_device_leaves_its_memory():
+    x = matrix(16, 2048, 1, torch.float16)
+    layer = fp8.Fp8Linear(torch.nn.Linear(2048, 4096).half().cuda())
+    layer(x)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    layer.cpu()
+    assert before - torch.cuda.memory_allocated() >= 2048 * 4096
+    with pytest.raises(capi.VenomError, match="CUDA device"):
+        layer(x)
+    assert layer.cuda()(x).shape == (16, 4096)
+
+
+def test_a_layer_from_a_file_with_views():
+    x, layer = matrix(30, 200, 1, torch.float16), fp8.Fp8Linear(frozen())
+    state = layer.__dict__.copy()
+    state["_views"] = {name: (cols, None, None) for name, cols in state.pop("_cols").items()}
+    old = fp8.Fp8Linear.__new__(fp8.Fp8Linear)
+    old.__setstate__(state)
+    assert torch.equal(old(x), layer(x))

@@ -150,6 +150,7 @@ struct Operand {
     const void *scales;
     c10::ScalarType f8;
     int64_t rows, cols;
+    Operand(const void *data_, int64_t ld_, const void *scales_, c10::ScalarType f8_, int64_t rows_, int64_t cols_) : data(data_), ld(ld_), scales(scales_), f8(f8_), rows(rows_), cols(cols_) {}
     Operand(const Packed &p) : data(p.values()), ld(p.ld), scales(p.scale()), f8(p.f8), rows(p.rows), cols(p.cols) {}
     Operand(const Tensor &d, const Tensor &s) : data(d.data_ptr()), ld(packed_ld(d)), scales(s.data_ptr()), f8(d.scalar_type()), rows(d.size(0)), cols(d.size(1)) {}
 };
@@ -168,15 +169,20 @@ Tensor multiply(const Operand &a, const Operand &b, const Tensor &bias, c10::Sca
     return out;
 }
 
+void check_bias(const Tensor &bias, int64_t rows, const at::Device &device, const char *what)
+{
+    if (bias.defined())
+        TORCH_CHECK(bias.device() == device && bias.dim() == 1 && bias.numel() == rows && bias.is_contiguous(), what, ": bias must be a contiguous vector of ", rows,
+                    " values on the operands' device");
+}
+
 Tensor matmul(const Tensor &a, const Tensor &sa, const Tensor &b, const Tensor &sb, const Tensor &bias, c10::ScalarType type)
 {
     check_packed(a, sa, "fp8.matmul");
     check_packed(b, sb, "fp8.matmul");
     TORCH_CHECK(a.device() == b.device(), "fp8.matmul: operands on one device expected");
     TORCH_CHECK(a.size(1) == b.size(1), "fp8.matmul: ", a.size(1), " and ", b.size(1), " columns do not match");
-    if (bias.defined())
-        TORCH_CHECK(bias.device() == a.device() && bias.dim() == 1 && bias.numel() == b.size(0) && bias.is_contiguous(), "fp8.matmul: bias must be a contiguous vector of ", b.size(0),
-                    " values on the operands' device");
+    check_bias(bias, b.size(0), a.device(), "fp8.matmul");
     c10::cuda::CUDAGuard guard(a.device());
     return multiply({a, sa}, {b, sb}, bias, type, a);
 }
@@ -444,10 +450,45 @@ Tensor mlp(const Tensor &x, const Tensor &w1, const OptTensor &bias1, const Tens
     return Mlp::apply(x, w1, bias1, w2, bias2, tanh_form, grad_type, at::GradMode::is_enabled());
 }
 
-std::tuple<Tensor, Tensor> gelu_quantize(const Tensor &x, bool tanh_form)
+// ---- frozen weights, as modules hold them: e4m3 values as bytes [rows, padded columns], scales as bytes [ceil(columns / 512), rows, 4] ----
+
+Operand held(const Tensor &w, const Tensor &scales, int64_t cols, const Tensor &bias, const at::Device &device, const char *what)
 {
-    const Gelu g = gelu(x, tanh_form, false, true, false, false);
-    return {g.rows.data(), g.rows.scales()};
+    TORCH_CHECK(w.device() == device && scales.device() == device, what, ": the weight's values and scales must be on the input's CUDA device");
+    TORCH_CHECK(w.scalar_type() == torch::kUInt8 && w.dim() == 2 && w.is_contiguous() && w.size(1) == packed(w, 0, cols, torch::kFloat8_e4m3fn).ld, what,
+                ": a weight's values must be bytes in rows of ", cols, " padded to 16");
+    TORCH_CHECK(scales.scalar_type() == torch::kUInt8 && scales.dim() == 3 && scales.is_contiguous() && scales.size(0) == (cols + 511) / 512 && scales.size(1) == w.size(0) &&
+                    scales.size(2) == 4,
+                what, ": a weight's scales must be bytes [ceil(columns / 512), rows, 4]");
+    check_bias(bias, w.size(0), device, what);
+    return {w.data_ptr(), w.size(1), scales.data_ptr(), torch::kFloat8_e4m3fn, w.size(0), cols};
+}
+Packed held_input(const Tensor &x, int64_t features, const char *what)
+{
+    check_input(x, what);
+    TORCH_CHECK(x.size(-1) == features, what, ": ", x.size(-1), " features do not match a weight of ", features);
+    return quantize(flat(x), torch::kFloat8_e4m3fn, false, true, false, c10::nullopt).rows;
+}
+
+Tensor held_linear(const Tensor &x, const Tensor &w, const Tensor &sw, int64_t cols, const OptTensor &bias)
+{
+    const Tensor b = or_undefined(bias);
+    const Packed q = held_input(x, cols, "Fp8Linear");
+    const Operand weight = held(w, sw, cols, b, x.device(), "Fp8Linear");
+    c10::cuda::CUDAGuard guard(x.device());
+    return shaped(multiply(q, weight, b, x.scalar_type(), x), x.sizes());
+}
+
+Tensor held_mlp(const Tensor &x, const Tensor &w1, const Tensor &sw1, int64_t cols1, const OptTensor &bias1, const Tensor &w2, const Tensor &sw2, int64_t cols2, const OptTensor &bias2,
+                bool tanh_form)
+{
+    const Tensor b1 = or_undefined(bias1), b2 = or_undefined(bias2);
+    const Packed q = held_input(x, cols1, "Fp8Mlp");
+    const Operand fc = held(w1, sw1, cols1, b1, x.device(), "Fp8Mlp"), proj = held(w2, sw2, cols2, b2, x.device(), "Fp8Mlp");
+    TORCH_CHECK(fc.rows == cols2, "Fp8Mlp: ", fc.rows, " features do not match a weight of ", cols2);
+    c10::cuda::CUDAGuard guard(x.device());
+    const Gelu g = gelu(multiply(q, fc, b1, x.scalar_type(), x, true), tanh_form, false, true, false, false);
+    return shaped(multiply(g.rows, proj, b2, x.scalar_type(), x), x.sizes());
 }
 
 int64_t device_status()
@@ -526,7 +567,8 @@ void define_fp8(pybind11::module &mod)
     using release = pybind11::call_guard<pybind11::gil_scoped_release>;
     if (PyModule_AddFunctions(mod.ptr(), fast_calls) != 0) throw pybind11::error_already_set();
     mod.def("fp8_dequantize", &dequantize, "vnm_fp8_dequantize with its allocation", release());
-    mod.def("fp8_gelu_quantize", &gelu_quantize, "GELU of a matrix in 8 bits: (data, scales)", release());
+    mod.def("fp8_held_linear", &held_linear, "A linear layer whose weight is held in 8 bits", release());
+    mod.def("fp8_held_mlp", &held_mlp, "A feed-forward block whose weights are held in 8 bits", release());
     mod.def("fp8_linear", &linear, "A differentiable linear layer in 8 bits", release());
     mod.def("fp8_gelu8", &gelu8, "GELU with an 8-bit checkpoint for its gradient", release());
     mod.def("fp8_mlp", &mlp, "A differentiable feed-forward block in 8 bits", release());

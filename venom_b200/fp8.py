@@ -102,11 +102,6 @@ def _check_input(x, what):
         raise VenomError("%s: at least one dimension expected" % what)
 
 
-def _flat(x):
-    """[..., features] as rows."""
-    return x if x.dim() == 2 else x.reshape(x.numel() // max(1, x.shape[-1]), x.shape[-1])
-
-
 def _check_grad_dtype(grad_dtype, what):
     if grad_dtype not in (E4M3, E5M2):
         raise VenomError("%s: gradients are kept in float8_e4m3fn or float8_e5m2, not %s" % (what, grad_dtype))
@@ -152,20 +147,17 @@ class _Held(torch.nn.Module):
         ld = -(-cols // 16) * 16
         self.register_buffer(name + "_data", q.data.view(torch.uint8).as_strided((rows, ld), (ld, 1)))
         self.register_buffer(name + "_scales", q.scales.view(torch.uint8))
-        self._views[name] = (cols, None, None)
+        self._cols[name] = cols
+
+    def __setstate__(self, state):
+        state = dict(state)
+        if "_views" in state:      # of files that kept views beside the buffers
+            state["_cols"] = {name: view[0] for name, view in state.pop("_views").items()}
+        super().__setstate__(state)
 
     def _weight(self, name):
-        """The buffers as an operand; the views are made anew when a buffer was replaced."""
-        cols, of, q = self._views[name]
-        data = self._buffers[name + "_data"]
-        if of is not data:
-            q = BlockFp8(data.view(E4M3)[:, :cols], self._buffers[name + "_scales"].view(torch.float8_e8m0fnu))
-            self._views[name] = (cols, data, q)
-        return q
-
-    def __getstate__(self):
-        """Copies and files hold the bytes once: views are made anew."""
-        return dict(self.__dict__, _views={name: (view[0], None, None) for name, view in self._views.items()})
+        """The bytes that the buffers hold now, their scales, and the columns that they stand for."""
+        return self._buffers[name + "_data"], self._buffers[name + "_scales"], self._cols[name]
 
     def _refuse_gradients(self, x):
         if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
@@ -185,7 +177,7 @@ class Fp8Linear(_Held):
 
     def __init__(self, original, trainable=False, grad_dtype=E4M3):
         super().__init__()
-        self._views = {}
+        self._cols = {}
         _check_grad_dtype(grad_dtype, "Fp8Linear")
         self.in_features, self.out_features = original.in_features, original.out_features
         self.trainable, self.grad_dtype = bool(trainable), grad_dtype
@@ -200,11 +192,7 @@ class Fp8Linear(_Held):
         if self.trainable:
             return linear(input, self.weight, self.bias, self.grad_dtype)
         self._refuse_gradients(input)
-        _check_input(input, "Fp8Linear")
-        flat = _flat(input)
-        q = quantize(flat)
-        y = matmul(q, self._weight("weight"), self.bias, input.dtype)
-        return y if input.dim() == 2 else y.reshape(*input.shape[:-1], self.out_features)
+        return _call("fp8_held_linear", input, *self._weight("weight"), self.bias)
 
     def extra_repr(self):
         return "in_features=%d, out_features=%d, bias=%s, trainable=%s" % (self.in_features, self.out_features, self.bias is not None, self.trainable)
@@ -215,7 +203,7 @@ class Fp8Mlp(_Held):
 
     def __init__(self, fc, proj, approximate="none", trainable=False, grad_dtype=E4M3):
         super().__init__()
-        self._views = {}
+        self._cols = {}
         _check_grad_dtype(grad_dtype, "Fp8Mlp")
         if fc.out_features != proj.in_features:
             raise VenomError("Fp8Mlp: %d features do not match %d" % (fc.out_features, proj.in_features))
@@ -235,10 +223,7 @@ class Fp8Mlp(_Held):
         if self.trainable:
             return mlp(input, self.fc_weight, self.fc_bias, self.proj_weight, self.proj_bias, self.approximate, self.grad_dtype)
         self._refuse_gradients(input)
-        _check_input(input, "Fp8Mlp")
-        h = matmul(quantize(_flat(input)), self._weight("fc"), self.fc_bias, input.dtype)
-        y = matmul(BlockFp8(*_call("fp8_gelu_quantize", h, self.tanh_form)), self._weight("proj"), self.proj_bias, input.dtype)
-        return y if input.dim() == 2 else y.reshape(*input.shape[:-1], self.out_features)
+        return _call("fp8_held_mlp", input, *self._weight("fc"), self.fc_bias, *self._weight("proj"), self.proj_bias, self.tanh_form)
 
 
 def linear_to_fp8(mod, skip=(), trainable=False, grad_dtype=E4M3):
