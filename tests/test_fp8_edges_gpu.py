@@ -120,6 +120,22 @@ def test_a_frozen_layer_that_leaves_the_device_leaves_its_memory():
     assert layer.cuda()(x).shape == (16, 4096)
 
 
+@pytest.mark.parametrize("cin", [8, 24, 200, 208, 513])
+def test_one_weight_always_gives_the_same_bytes(cin):
+    lin = frozen(cin)
+    states = []
+    for fill in (0x5A, 0xC3):
+        room = [torch.full((n,), fill, dtype=torch.uint8, device="cuda") for n in (1 << 18, 1 << 19, 1 << 20)]       # what the allocator hands out next
+        del room
+        states.append(fp8.Fp8Linear(lin).state_dict())
+    assert states[0].keys() == states[1].keys()
+    for k, v in states[0].items():
+        assert torch.equal(v, states[1][k]), k
+        assert v.untyped_storage().nbytes() == v.numel() * v.element_size(), k
+    storages = {v.untyped_storage().data_ptr() for v in states[0].values()}
+    assert len(storages) == len(states[0])
+
+
 def test_a_layer_from_a_file_with_views():
     x, layer = matrix(30, 200, 1, torch.float16), fp8.Fp8Linear(frozen())
     state = layer.__dict__.copy()

@@ -139,14 +139,15 @@ def mlp(x, w1, b1, w2, b2, approximate="none", grad_dtype=E4M3):
 
 class _Held(torch.nn.Module):
     """A frozen weight's 8 bits as buffers.  They are kept as bytes, which Module.half() and its like leave alone, with the rows' padding, which a copy to
-    another device would drop."""
+    another device would drop; the padding is zero, so that one weight always gives the same bytes."""
 
     def _hold(self, name, weight):
         q = quantize(weight.detach(), square=True)
         rows, cols = q.shape
-        ld = -(-cols // 16) * 16
-        self.register_buffer(name + "_data", q.data.view(torch.uint8).as_strided((rows, ld), (ld, 1)))
-        self.register_buffer(name + "_scales", q.scales.view(torch.uint8))
+        data = torch.zeros((rows, max(16, -(-cols // 16) * 16)), dtype=torch.uint8, device=q.device)
+        data[:, :cols] = q.data.view(torch.uint8)
+        self.register_buffer(name + "_data", data)
+        self.register_buffer(name + "_scales", q.scales.view(torch.uint8).clone())      # storages of their own, as files want them
         self._cols[name] = cols
 
     def __setstate__(self, state):
