@@ -96,6 +96,12 @@ struct Fp8MatmulParams {
     int *status;
 };
 
+// What a plan depends on of the device that it is for.
+struct Fp8Device {
+    int sms;
+    int clusters;  // of two CTAs of the pair kernel that run side by side; 0: it does not run here
+};
+
 struct Fp8Plan {
     int bn;        // columns of the accumulator
     int split;
@@ -103,13 +109,13 @@ struct Fp8Plan {
 };
 
 // On pairs of SMs: tiles of 256 x (192 .. 256).
-cudaError_t fp8_pair_init();
+cudaError_t fp8_pair_init(int sms, int *clusters);      // for the current device
 // wide_out: results of 32 bits; whole: their rows are stored in whole pieces (see whole_pieces).  Both return an estimate in microseconds, < 0: not for this problem.
-float fp8_pair_config(int M, int N, int K, bool wide_out, bool whole, bool bias, Fp8Plan *plan);
+float fp8_pair_config(int M, int N, int K, bool wide_out, bool whole, bool bias, const Fp8Device &device, Fp8Plan *plan);
 cudaError_t launch_fp8_pair(const Fp8Plan &plan, const CUtensorMap &map_a, const CUtensorMap &map_b, const Fp8MatmulParams &p, cudaStream_t stream);
 // One SM a tile: 128 rows of B x (16 .. 128) rows of A, k split over a cluster where tiles are few.
 cudaError_t fp8_small_init();
-float fp8_small_config(int M, int N, int ktiles, bool wide_out, Fp8Plan *plan);
+float fp8_small_config(int M, int N, int ktiles, bool wide_out, const Fp8Device &device, Fp8Plan *plan);
 cudaError_t launch_fp8_small(const Fp8Plan &plan, const CUtensorMap &map_a, const CUtensorMap &map_b, const Fp8MatmulParams &p, cudaStream_t stream);
 
 #if defined(__CUDACC__)

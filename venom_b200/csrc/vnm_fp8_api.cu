@@ -99,17 +99,18 @@ int empty_sums(void *colsum, int type, int cols, cudaStream_t stream)
     return done(cudaMemsetAsync(colsum, 0, (size_t)cols * elem_size(type), stream), "column sums of no rows");
 }
 
-// What a device needs once: shared-memory limits, the status word's address.
+// What a device needs once: shared-memory limits, the status word's address, what plans depend on.  Not written again once it is ready.
 constexpr int kMaxDevices = 64;
 struct Device {
     bool ready;
     int *status;
+    Fp8Device plans;
 };
 Device g_devices[kMaxDevices];
 std::mutex g_mutex;
 __device__ int g_status;
 
-int device_ready(int **status)
+int device_ready(const Device **ready)
 {
     int dev = -1;
     cudaError_t e = cudaGetDevice(&dev);
@@ -124,13 +125,14 @@ int device_ready(int **status)
             Relaxed() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
             ~Relaxed() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
         } relaxed;
-        if ((e = fp8_small_init()) != cudaSuccess || (e = fp8_pair_init()) != cudaSuccess) return done(e, "cudaFuncSetAttribute(max dynamic shared memory)");
+        if ((e = cudaDeviceGetAttribute(&d.plans.sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return done(e, "cudaDeviceGetAttribute");
+        if ((e = fp8_small_init()) != cudaSuccess || (e = fp8_pair_init(d.plans.sms, &d.plans.clusters)) != cudaSuccess) return done(e, "cudaFuncSetAttribute(max dynamic shared memory)");
         void *at = nullptr;
         if ((e = cudaGetSymbolAddress(&at, g_status)) != cudaSuccess) return done(e, "cudaGetSymbolAddress");
         d.status = static_cast<int *>(at);
         d.ready = true;
     }
-    *status = d.status;
+    *ready = &d;
     return VNM_OK;
 }
 
@@ -144,10 +146,11 @@ CUresult encode_operand(EncodeTiledFn enc, CUtensorMap *map, const void *data, i
 }
 
 // The kernel and tile with the smaller estimate.
-int choose_plan(int M, int N, int K, bool wide_out, bool whole, bool bias, Fp8Plan *plan, bool *on_pairs)
+int choose_plan(int M, int N, int K, bool wide_out, bool whole, bool bias, const Fp8Device &device, Fp8Plan *plan, bool *on_pairs)
 {
     Fp8Plan small = {}, pair = {};
-    const float small_us = fp8_small_config(M, N, (int)(((int64_t)K + 127) / 128), wide_out, &small), pair_us = fp8_pair_config(M, N, K, wide_out, whole, bias, &pair);
+    const float small_us = fp8_small_config(M, N, (int)(((int64_t)K + 127) / 128), wide_out, device, &small),
+                pair_us = fp8_pair_config(M, N, K, wide_out, whole, bias, device, &pair);
     if (small_us < 0.0f && pair_us < 0.0f) return fail(VNM_ERR_UNSUPPORTED, "vnm_fp8_matmul: no kernel for %d x %d x %d", M, N, K);
     *on_pairs = small_us < 0.0f || (pair_us >= 0.0f && pair_us < small_us);
     *plan = *on_pairs ? pair : small;
@@ -278,8 +281,8 @@ extern "C" int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, 
     VNM_TRY(check_value(name, "the result", out, ldo, out_type, M, N));
     if (bias && !aligned(bias, (uintptr_t)elem_size(bias_type))) return fail(VNM_ERR_BAD_ARG, "%s: bias is not aligned to its type", name);
     VNM_TRY(check_product_size(name, M, N, K));
-    int *status = nullptr;
-    VNM_TRY(device_ready(&status));
+    const Device *device = nullptr;
+    VNM_TRY(device_ready(&device));
     const EncodeTiledFn enc = get_encode_fn();
     if (!enc) return fail(VNM_ERR_CUDA, "cuTensorMapEncodeTiled not available");
     Fp8MatmulParams p = {};
@@ -289,11 +292,11 @@ extern "C" int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, 
     p.whole_pieces = pieces(out, out_type, ldo);
     p.M = M; p.N = N; p.K = K; p.ktiles = (K + 127) / 128;
     p.a_f8 = a_type; p.b_f8 = b_type;
-    p.status = status;
+    p.status = device->status;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     Fp8Plan plan = {};
     bool on_pairs = false;
-    VNM_TRY(choose_plan(M, N, K, out_type == VNM_F32, p.whole_pieces != 0, bias != nullptr, &plan, &on_pairs));
+    VNM_TRY(choose_plan(M, N, K, out_type == VNM_F32, p.whole_pieces != 0, bias != nullptr, device->plans, &plan, &on_pairs));
     CUtensorMap map_a, map_b;
     if (encode_operand(enc, &map_a, a, lda, M, K, on_pairs ? 128 : plan.bn) != CUDA_SUCCESS || encode_operand(enc, &map_b, b, ldb, N, K, on_pairs ? plan.bn / 2 : 128) != CUDA_SUCCESS)
         return fail(VNM_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", name);
@@ -315,11 +318,11 @@ extern "C" int vnm_fp8_matmul_config(int M, int N, int K, int out_type, int whol
     if (M < 1 || N < 1 || K < 1) return fail(VNM_ERR_BAD_ARG, "%s: sizes must be positive (got %d, %d, %d)", name, M, N, K);
     if (!known_type(out_type)) return fail(VNM_ERR_BAD_ARG, "%s: unknown type %d", name, out_type);
     VNM_TRY(check_product_size(name, M, N, K));
-    int *status = nullptr;
-    VNM_TRY(device_ready(&status));
+    const Device *device = nullptr;
+    VNM_TRY(device_ready(&device));
     Fp8Plan plan = {};
     bool on_pairs = false;
-    VNM_TRY(choose_plan(M, N, K, out_type == VNM_F32, whole != 0, bias != 0, &plan, &on_pairs));
+    VNM_TRY(choose_plan(M, N, K, out_type == VNM_F32, whole != 0, bias != 0, device->plans, &plan, &on_pairs));
     if (tile_m) *tile_m = on_pairs ? 256 : plan.bn;
     if (tile_n) *tile_n = on_pairs ? plan.bn : 128;
     if (split) *split = plan.split;
@@ -330,8 +333,10 @@ extern "C" int vnm_fp8_matmul_config(int M, int N, int K, int out_type, int whol
 extern "C" int vnm_fp8_device_status(int *status, void *stream)
 {
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    int *dev = nullptr, got = 0;
-    VNM_TRY(device_ready(&dev));
+    const Device *device = nullptr;
+    VNM_TRY(device_ready(&device));
+    int *const dev = device->status;
+    int got = 0;
     cudaError_t e = cudaMemcpyAsync(&got, dev, sizeof(got), cudaMemcpyDeviceToHost, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     if (e != cudaSuccess) return done(e, "vnm_fp8_device_status");

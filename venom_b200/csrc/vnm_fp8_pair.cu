@@ -547,22 +547,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
     }
 }
 
-int g_clusters = 0;          // co-resident clusters of two CTAs on this device (0 = not queried yet)
-
 }  // namespace
 
 #define VNM_FP8_PAIR(X) X(192, true) X(224, true) X(240, true) X(256, true) X(192, false) X(224, false) X(240, false) X(256, false)
 
-cudaError_t fp8_pair_init()
+cudaError_t fp8_pair_init(int sms, int *clusters)
 {
     cudaError_t e;
 #define VNM_ATTR(BN, WHOLE) \
     if ((e = cudaFuncSetAttribute(fp8_pair_kernel<BN, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8Pair<BN, WHOLE>::SMEM_BYTES)) != cudaSuccess) return e;
     VNM_FP8_PAIR(VNM_ATTR)
 #undef VNM_ATTR
-    int dev = 0, sms = 0;
-    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
-    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)(sms & ~1));
     lc.blockDim = dim3(NUM_THREADS);
@@ -574,10 +569,8 @@ cudaError_t fp8_pair_init()
     attr[0].val.clusterDim.z = 1;
     lc.attrs = attr;
     lc.numAttrs = 1;
-    int clusters = 0;
-    e = cudaOccupancyMaxActiveClusters(&clusters, fp8_pair_kernel<256, true>, &lc);
-    if (e != cudaSuccess) { (void)cudaGetLastError(); clusters = 0; }
-    g_clusters = clusters;
+    e = cudaOccupancyMaxActiveClusters(clusters, fp8_pair_kernel<256, true>, &lc);
+    if (e != cudaSuccess) { (void)cudaGetLastError(); *clusters = 0; }
     return cudaSuccess;
 }
 
@@ -585,9 +578,10 @@ cudaError_t fp8_pair_init()
 // tile's epilogue.  A tile takes its k-tiles' time or its epilogue's, whichever is longer (a smooth maximum), or with one accumulator both.  Both
 // kernels' costs were fitted to steady calls on inputs that change, 802 shapes of 1 to 16384 x 8 to 36864 x 64 to 12288, odd ones and round ones, with and without a bias,
 // fp16 and fp32 results, for the choice that they make: 1.007 of the fastest one's time on average over 371 others, 1.33 at most (few rows, few columns or few k).
-float fp8_pair_config(int M, int N, int K, bool wide_out, bool whole, bool bias, Fp8Plan *plan)
+float fp8_pair_config(int M, int N, int K, bool wide_out, bool whole, bool bias, const Fp8Device &device, Fp8Plan *plan)
 {
-    if (g_clusters <= 0) return -1.0f;
+    const int clusters = device.clusters;
+    if (clusters <= 0) return -1.0f;
     static const int widths[4] = {192, 224, 240, 256};
     static const float ktile[4] = {0.352f, 0.380f, 0.388f, 0.410f};
     const int64_t mt = ((int64_t)M + 255) / 256;
@@ -598,14 +592,14 @@ float fp8_pair_config(int M, int N, int K, bool wide_out, bool whole, bool bias,
         const int w = widths[i];
         const int64_t nt = ((int64_t)N + w - 1) / w, tiles = mt * nt;
         if (tiles > INT32_MAX / 2) continue;
-        const float waves = 0.715f * (float)((tiles + g_clusters - 1) / g_clusters) + 0.285f * (float)tiles / (float)g_clusters;
+        const float waves = 0.715f * (float)((tiles + clusters - 1) / clusters) + 0.285f * (float)tiles / (float)clusters;
         const float mma = kt * ktile[i], out = edge * (float)w / 240.0f;
         const float one = w == 256 ? mma + 1.12f * out : powf(powf(mma, 1.1f) + powf(out, 1.1f), 1.0f / 1.1f);
         const float us = 3.19f + waves * one + 0.26f * out;
         if (best < 0.0f || us < best) {
             best = us;
             plan->bn = w;
-            plan->grid = 2 * (int)(tiles < g_clusters ? tiles : g_clusters);
+            plan->grid = 2 * (int)(tiles < clusters ? tiles : clusters);
         }
     }
     plan->split = 1;

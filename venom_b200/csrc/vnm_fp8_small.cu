@@ -292,8 +292,6 @@ __global__ void __launch_bounds__(SMALL_THREADS, 2) fp8_small_kernel(const __gri
     }
 }
 
-int g_sms = 0;
-
 }  // namespace
 
 #define VNM_FP8_SMALL(X) X(16) X(32) X(64) X(128)
@@ -305,21 +303,19 @@ cudaError_t fp8_small_init()
     if ((e = cudaFuncSetAttribute(fp8_small_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8Small<BN>::SMEM_BYTES)) != cudaSuccess) return e;
     VNM_FP8_SMALL(VNM_ATTR)
 #undef VNM_ATTR
-    int dev = 0;
-    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
-    return cudaDeviceGetAttribute(&g_sms, cudaDevAttrMultiProcessorCount, dev);
+    return cudaSuccess;
 }
 
 // The cost of a call, us: a start, then a CTA's k-tiles (one CTA an SM, or two that share it) or the operands' bytes, whichever takes longer, its epilogue, and the exchange
 // of partial sums.  See fp8_pair_config for what they were fitted to.  (512 x 4096 x 4096: 128 x 64 16.2 us, pairs 12.6;  16 x 36864 x 12288: 128 x 16 68.2, all of it
 // the weight's bytes;  128 x 4096 x 1024: 128 x 32 6.2, pairs 6.4;  8 x 1024 x 1024: 128 x 16 alone 4.6, split by eight 3.8.)
-float fp8_small_config(int M, int N, int ktiles, bool wide_out, Fp8Plan *plan)
+float fp8_small_config(int M, int N, int ktiles, bool wide_out, const Fp8Device &device, Fp8Plan *plan)
 {
     struct Cost { float start, kt1, kt2, out, split, bytes; };
     static const Cost cost[4] = {{1.75f, 0.189f, 0.554f, 1.93f, 0.51f, 0.094f}, {1.83f, 0.204f, 0.492f, 2.53f, 0.54f, 0.084f}, {2.46f, 0.257f, 0.496f, 3.95f, 0.21f, 0.077f},
                                  {5.28f, 0.399f, 0.760f, 2.85f, 1.34f, 0.118f}};
     const int64_t nt = ((int64_t)N + 127) / 128;
-    const int sms = g_sms > 0 ? g_sms : 148;
+    const int sms = device.sms;
     float best = -1.0f;
     for (int i = 0; i < 4; i++) {
         const int bn = 16 << i;
