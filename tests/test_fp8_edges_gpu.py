@@ -143,3 +143,98 @@ def test_a_layer_from_a_file_with_views():
     old = fp8.Fp8Linear.__new__(fp8.Fp8Linear)
     old.__setstate__(state)
     assert torch.equal(old(x), layer(x))
+
+
+# ---- what is kept between the passes ----
+
+def leaf(t):
+    return t.detach().clone().requires_grad_()
+
+
+def bytes_kept(call, of):
+    """Device memory that a graph holds besides its result, the leaves and their like."""
+    torch.cuda.synchronize()
+    start = torch.cuda.memory_allocated()
+    x = of * 1.0                                       # an input that lives only as long as the graph wants it
+    y = call(x)
+    del x
+    kept = torch.cuda.memory_allocated() - start - (y.numel() * y.element_size() + 511) // 512 * 512
+    y.backward(torch.ones_like(y))
+    return kept
+
+
+ROOM = 1 << 16                                         # padding, scales of few rows, the allocator's pieces
+
+
+@pytest.mark.parametrize("tokens,cin,cout", [(256, 2048, 4096), (64, 1024, 4096), (4096, 1024, 1024), (1024, 4096, 1024), (1023, 2048, 1024), (2048, 4096, 4096)])
+def test_a_linear_keeps_no_more_than_in_16_bits(tokens, cin, cout):
+    x, w, b = leaf(matrix(tokens, cin, 1, torch.float16)), leaf(matrix(cout, cin, 2, torch.float16)), leaf(matrix(1, cout, 3, torch.float16)[0])
+    kept, dense = bytes_kept(lambda t: fp8.linear(t, w, b), x), bytes_kept(lambda t: torch.nn.functional.linear(t, w, b), x)
+    assert kept <= (cin * tokens + (cin * cout if cout <= tokens else 0)) * 129 / 128 + ROOM
+    assert kept <= dense + ROOM and dense >= 2 * cin * tokens
+
+
+def test_a_linear_with_32_bit_weights_keeps_no_more_than_a_cast_one():
+    x, w = leaf(matrix(256, 1024, 1, torch.float16)), leaf(matrix(2048, 1024, 2))
+    kept, dense = bytes_kept(lambda t: fp8.linear(t, w), x), bytes_kept(lambda t: torch.nn.functional.linear(t, w.half()), x)
+    assert kept <= 1024 * (256 + 2048) * 129 / 128 + ROOM and 2 * kept <= dense + 2 * ROOM
+
+
+@pytest.mark.parametrize("tokens,cin,hidden", [(256, 1024, 4096), (2048, 1024, 4096), (8192, 512, 2048)])
+def test_a_feed_forward_block_keeps_no_more_than_in_16_bits(tokens, cin, hidden):
+    x, w1, w2 = leaf(matrix(tokens, cin, 1, torch.float16)), leaf(matrix(hidden, cin, 2, torch.float16)), leaf(matrix(cin, hidden, 3, torch.float16))
+    kept = bytes_kept(lambda t: fp8.mlp(t, w1, None, w2, None), x)
+    dense = bytes_kept(lambda t: torch.nn.functional.linear(torch.nn.functional.gelu(torch.nn.functional.linear(t, w1)), w2), x)
+    weights = sum(cin * hidden for rows in (hidden, cin) if rows <= tokens)
+    assert kept <= (tokens * (cin + 2 * hidden) + weights) * 129 / 128 + ROOM and kept <= dense + ROOM
+
+
+@pytest.mark.parametrize("tokens,cin,hidden,cout", [(37, 100, 203, 70), (37, 128, 33, 300), (1, 64, 128, 64), (300, 200, 515, 130), (0, 64, 128, 32)])
+@pytest.mark.parametrize("w_type", ["fp16", "fp32"])
+def test_gradients_are_the_same_whatever_is_kept_of_a_weight(tokens, cin, hidden, cout, w_type):
+    """A leaf, and a weight that some operation made, whose transpose is kept."""
+    t, dy = TYPES[w_type], matrix(tokens, cout, 9, torch.float16)
+    x, w1, w2 = leaf(matrix(tokens, cin, 1, torch.float16)), leaf(matrix(hidden, cin, 2, t, 0.2)), leaf(matrix(cout, hidden, 3, t, 0.2))
+    made = lambda w: w * 1.0
+    a = torch.autograd.grad(fp8.mlp(x, w1, None, w2, None), (x, w1, w2), dy)
+    b = torch.autograd.grad(fp8.mlp(x, made(w1), None, made(w2), None), (x, w1, w2), dy)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    w, dh = w1, matrix(tokens, hidden, 8, torch.float16)
+    y = fp8.linear(x, w)
+    a, again = torch.autograd.grad(y, (x, w), dh, retain_graph=True), torch.autograd.grad(y, (x, w), dh)
+    b = torch.autograd.grad(fp8.linear(x, made(w)), (x, w), dh)
+    only = torch.autograd.grad(fp8.linear(x, w.detach()), x, dh)[0]
+    assert all(torch.equal(p, q) and torch.equal(p, r) for p, q, r in zip(a, b, again)) and torch.equal(only, a[0])
+
+
+def test_a_weight_that_was_written_to_is_refused_or_kept():
+    """Never a gradient of another weight than the forward pass's: few tokens keep the leaf, which torch refuses to use once it was written to; many keep its 8 bits."""
+    for tokens, refused in ((40, True), (72, False), (200, False)):
+        x, w, dy = leaf(matrix(tokens, 96, 1, torch.float16)), leaf(matrix(72, 96, 2, torch.float16)), matrix(tokens, 72, 3, torch.float16)
+        (want,) = torch.autograd.grad(fp8.linear(x, w), x, dy)
+        y = fp8.linear(x, w)
+        with torch.no_grad():
+            w.mul_(2)
+        if refused:
+            with pytest.raises(RuntimeError, match="inplace"):
+                y.backward(dy)
+        else:
+            y.backward(dy)
+            assert torch.equal(x.grad, want)
+
+
+def test_saved_weights_in_another_form_are_refused():
+    x, w = leaf(matrix(37, 100, 1, torch.float16)), leaf(matrix(70, 100, 2, torch.float16))
+    for back in (lambda t: t[:-1] if t.dim() == 2 else t, lambda t: t.cpu() if t.dim() == 2 else t, lambda t: t.double() if t.dim() == 2 else t):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+            y = fp8.linear(x, w)
+        with pytest.raises(RuntimeError, match="another form"):
+            y.backward(torch.ones_like(y))
+
+
+def test_weights_made_in_inference_mode():
+    with torch.inference_mode():
+        w1, w2 = matrix(200, 96, 2, torch.float16), matrix(72, 200, 3, torch.float16)
+    x, dy = leaf(matrix(16, 96, 1, torch.float16)), matrix(16, 72, 9, torch.float16)
+    got = torch.autograd.grad(fp8.mlp(x, w1, None, w2, None), x, dy)[0]
+    assert torch.equal(got, torch.autograd.grad(fp8.mlp(x, w1.clone(), None, w2.clone(), None), x, dy)[0])

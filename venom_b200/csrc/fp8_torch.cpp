@@ -334,18 +334,32 @@ struct Kept {
 };
 Tensor viewed(const Tensor &t, at::IntArrayRef shape) { return t.sizes() == shape ? t : t.view(shape); }
 
+// What a backward pass needs of a weight is its transpose in 8 bits, in . out bytes.  It is written beside the forward operand from one read and kept while that is no
+// more than a 16-bit layer keeps: its input takes in . tokens bytes here and 2 in . tokens there, so for out <= tokens; where input and weight differ in type such a layer keeps a
+// cast weight as well.  Elsewhere a leaf, which lives anyway, is kept itself and quantised again (12288 x 12288 with 2048 tokens: 176 -> 25 MB kept, for a second pass over
+// the weight).  What is not a leaf is kept in 8 bits, half of its own size; so are tensors made in inference mode, which no graph may hold.
+bool again_later(const Tensor &w, const Tensor &x, int64_t tokens) { return w.size(0) > tokens && w.is_leaf() && !w.is_inference() && w.scalar_type() == x.scalar_type(); }
+Packed transposed_weight(const Tensor &saved, bool again, int64_t rows, int64_t cols)
+{
+    if (!again) return unpacked(saved, cols, rows);
+    TORCH_CHECK(saved.defined() && saved.is_cuda() && saved.dim() == 2 && saved.size(0) == rows && saved.size(1) == cols && is_float(saved.scalar_type()),
+                "a saved tensor came back from its hooks in another form");
+    return quantize(saved, torch::kFloat8_e4m3fn, true, false, true, c10::nullopt).cols;
+}
+
 struct Linear : torch::autograd::Function<Linear> {
-    enum { X_TYPE, W_TYPE, BIAS_TYPE, GRAD_TYPE, HAS_BIAS, TOKENS, IN, OUT, NUMBERS };
+    enum { X_TYPE, W_TYPE, BIAS_TYPE, GRAD_TYPE, HAS_BIAS, AGAIN, TOKENS, IN, OUT, NUMBERS };
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &opt_bias, c10::ScalarType grad_type, bool record)
     {
         const Tensor bias = or_undefined(opt_bias);
         const bool need_x = record && wants_grad(x), need_w = record && wants_grad(w);
         const Both xs = quantized(flat(x), torch::kFloat8_e4m3fn, false, true, need_w, c10::nullopt);
-        const Both ws = quantized(w, torch::kFloat8_e4m3fn, true, true, need_x, c10::nullopt);
+        const bool again = need_x && again_later(w, x, xs.rows.rows);
+        const Both ws = quantized(w, torch::kFloat8_e4m3fn, true, true, need_x && !again, c10::nullopt);
         const Tensor y = product(xs.rows, ws.rows, bias, x.scalar_type());
-        ctx->save_for_backward({xs.cols.bytes, ws.cols.bytes});
+        ctx->save_for_backward({xs.cols.bytes, again ? w : ws.cols.bytes});
         keep<NUMBERS>(ctx, {(int64_t)x.scalar_type(), (int64_t)w.scalar_type(), (int64_t)(bias.defined() ? bias.scalar_type() : x.scalar_type()), (int64_t)grad_type, bias.defined(),
-                            xs.rows.rows, w.size(1), w.size(0)}, x.sizes());
+                            again, xs.rows.rows, w.size(1), w.size(0)}, x.sizes());
         return shaped(y, x.sizes());
     }
     static variable_list backward(AutogradContext *ctx, variable_list dys)
@@ -356,7 +370,7 @@ struct Linear : torch::autograd::Function<Linear> {
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = kept[HAS_BIAS] && ctx->needs_input_grad(2);
         const Both g = quantized(flat(dys[0]), kept.type(GRAD_TYPE), false, need_x, need_w || need_b, type_of(need_b, kept.type(BIAS_TYPE)));
         Tensor dx, dw;
-        if (need_x) dx = viewed(product(g.rows, unpacked(saved[1], kept[IN], kept[OUT]), Tensor(), kept.type(X_TYPE)), kept.shape());
+        if (need_x) dx = viewed(product(g.rows, transposed_weight(saved[1], kept[AGAIN] != 0, kept[OUT], kept[IN]), Tensor(), kept.type(X_TYPE)), kept.shape());
         if (need_w) dw = product(g.cols, unpacked(saved[0], kept[IN], kept[TOKENS]), Tensor(), kept.type(W_TYPE));
         return once({dx, dw, g.sums, Tensor(), Tensor()}, dys);
     }
@@ -398,7 +412,7 @@ Tensor gelu8(const Tensor &x, bool tanh_form)
 }
 
 struct Mlp : torch::autograd::Function<Mlp> {
-    enum { X_TYPE, W1_TYPE, B1_TYPE, W2_TYPE, B2_TYPE, GRAD_TYPE, TANH, HAS_B1, HAS_B2, TOKENS, IN, HIDDEN, OUT, NUMBERS };
+    enum { X_TYPE, W1_TYPE, B1_TYPE, W2_TYPE, B2_TYPE, GRAD_TYPE, TANH, HAS_B1, HAS_B2, AGAIN1, AGAIN2, TOKENS, IN, HIDDEN, OUT, NUMBERS };
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w1, const OptTensor &opt_b1, const Tensor &w2, const OptTensor &opt_b2, bool tanh_form,
                           c10::ScalarType grad_type, bool record)
     {
@@ -406,14 +420,15 @@ struct Mlp : torch::autograd::Function<Mlp> {
         const bool need_x = record && wants_grad(x), need_w1 = record && wants_grad(w1), need_b1 = record && wants_grad(b1), need_w2 = record && wants_grad(w2);
         const bool inner = need_x || need_w1 || need_b1;      // whether the gradient goes back through the GELU
         const Both xs = quantized(flat(x), torch::kFloat8_e4m3fn, false, true, need_w1, c10::nullopt);
-        const Both w1s = quantized(w1, torch::kFloat8_e4m3fn, true, true, need_x, c10::nullopt);
+        const bool again1 = need_x && again_later(w1, x, xs.rows.rows), again2 = inner && again_later(w2, x, xs.rows.rows);
+        const Both w1s = quantized(w1, torch::kFloat8_e4m3fn, true, true, need_x && !again1, c10::nullopt);
         const Gelu a = gelu(product(xs.rows, w1s.rows, b1, x.scalar_type(), true), tanh_form, false, true, need_w2, inner);
-        const Both w2s = quantized(w2, torch::kFloat8_e4m3fn, true, true, inner, c10::nullopt);
+        const Both w2s = quantized(w2, torch::kFloat8_e4m3fn, true, true, inner && !again2, c10::nullopt);
         const Tensor y = product(a.rows, w2s.rows, b2, x.scalar_type());
-        ctx->save_for_backward({xs.cols.bytes, w1s.cols.bytes, a.cols.bytes, a.ckpt.bytes, w2s.cols.bytes});
+        ctx->save_for_backward({xs.cols.bytes, again1 ? w1 : w1s.cols.bytes, a.cols.bytes, a.ckpt.bytes, again2 ? w2 : w2s.cols.bytes});
         keep<NUMBERS>(ctx, {(int64_t)x.scalar_type(), (int64_t)w1.scalar_type(), (int64_t)(b1.defined() ? b1.scalar_type() : x.scalar_type()), (int64_t)w2.scalar_type(),
-                            (int64_t)(b2.defined() ? b2.scalar_type() : x.scalar_type()), (int64_t)grad_type, tanh_form, b1.defined(), b2.defined(), xs.rows.rows, w1.size(1), w1.size(0),
-                            w2.size(0)}, x.sizes());
+                            (int64_t)(b2.defined() ? b2.scalar_type() : x.scalar_type()), (int64_t)grad_type, tanh_form, b1.defined(), b2.defined(), again1, again2, xs.rows.rows, w1.size(1),
+                            w1.size(0), w2.size(0)}, x.sizes());
         return shaped(y, x.sizes());
     }
     static variable_list backward(AutogradContext *ctx, variable_list dys)
@@ -429,10 +444,10 @@ struct Mlp : torch::autograd::Function<Mlp> {
         Tensor dx, dw1, db1, dw2;
         if (need_w2) dw2 = product(g.cols, unpacked(s[2], hidden, tokens), Tensor(), kept.type(W2_TYPE));
         if (inner) {
-            const Tensor da = product(g.rows, unpacked(s[4], hidden, kept[OUT]), Tensor(), kept.type(X_TYPE), true);
+            const Tensor da = product(g.rows, transposed_weight(s[4], kept[AGAIN2] != 0, kept[OUT], hidden), Tensor(), kept.type(X_TYPE), true);
             const GeluGrad h = gelu_grad(da, unpacked(s[3], tokens, hidden), kept[TANH] != 0, false, kept.type(GRAD_TYPE), need_x, need_w1 || need_b1, type_of(need_b1, kept.type(B1_TYPE)));
             db1 = h.both.sums;
-            if (need_x) dx = viewed(product(h.both.rows, unpacked(s[1], kept[IN], hidden), Tensor(), kept.type(X_TYPE)), kept.shape());
+            if (need_x) dx = viewed(product(h.both.rows, transposed_weight(s[1], kept[AGAIN1] != 0, hidden, kept[IN]), Tensor(), kept.type(X_TYPE)), kept.shape());
             if (need_w1) dw1 = product(h.both.cols, unpacked(s[0], kept[IN], tokens), Tensor(), kept.type(W1_TYPE));
         }
         return once({dx, dw1, db1, dw2, g.sums, Tensor(), Tensor(), Tensor()}, dys);

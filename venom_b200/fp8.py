@@ -119,7 +119,8 @@ def linear(x, weight, bias=None, grad_dtype=E4M3):
 
     x is rounded in blocks of 128 along its features, the weight in blocks of 128 x 128, gradients in blocks of 128 of `grad_dtype` (float8_e4m3fn
     or float8_e5m2) along whichever way they are summed; the bias's gradient is the sum of unrounded ones.  Kept until the backward pass: the 8-bit
-    transposes of x (where the weight wants a gradient) and of the weight (where x does)."""
+    transpose of x (where the weight wants a gradient), and of the weight (where x does) what takes less: its 8-bit transpose where it has no more rows than x has
+    tokens, another type than x, or is not a leaf; else the weight itself, which may not be written to meanwhile."""
     return _call("fp8_linear", x, weight, bias, grad_dtype)
 
 
@@ -133,7 +134,7 @@ def mlp(x, w1, b1, w2, b2, approximate="none", grad_dtype=E4M3):
     """linear(gelu(linear(x, w1, b1)), w2, b2) for x [..., in], w1 [hidden, in], w2 [out, hidden], differentiable once in all five.
 
     The GELU's result is rounded to 8 bits straight from 32 (there is no copy of it in the type of x), its gradient likewise.  Kept until the
-    backward pass, all in 8 bits: the transposes of x, of the GELU's result and of the weights, and the GELU's input."""
+    backward pass, in 8 bits: the transposes of x and of the GELU's result, and the GELU's input; the weights as in linear."""
     return _call("fp8_mlp", x, w1, b1, w2, b2, _tanh_form(approximate, "fp8.mlp"), grad_dtype)
 
 
