@@ -138,3 +138,17 @@ def test_linear_to_fp8_walks_like_linear_to_spmm():
     assert isinstance(b.a, fp8.Fp8Linear) and b.a.weight is weight and isinstance(b.inner[0], fp8.Fp8Linear) and type(b.head) is torch.nn.Linear
     assert {n for n, _ in b.named_parameters()} == {"a.weight", "a.bias", "head.weight", "head.bias", "inner.0.weight", "inner.0.bias"}
     assert isinstance(fp8.linear_to_fp8(torch.nn.Linear(8, 8), trainable=True), fp8.Fp8Linear)
+
+
+def test_linear_to_fp8_leaves_subclasses():
+    class Doubled(torch.nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    attention = torch.nn.MultiheadAttention(8, 2)
+    projection = attention.out_proj
+    b = torch.nn.ModuleDict({"attention": attention, "own": Doubled(8, 8), "plain": torch.nn.Linear(8, 8)})
+    own = b["own"]
+    fp8.linear_to_fp8(b, trainable=True)
+    assert attention.out_proj is projection and b["own"] is own and isinstance(b["plain"], fp8.Fp8Linear)
+    assert fp8.linear_to_fp8(own, trainable=True) is own

@@ -1,4 +1,5 @@
 """The block-scaled 8-bit operators where values are not finite, buffers change hands and memory counts."""
+import copy
 import math
 
 import pytest
@@ -238,3 +239,26 @@ def test_weights_made_in_inference_mode():
     x, dy = leaf(matrix(16, 96, 1, torch.float16)), matrix(16, 72, 9, torch.float16)
     got = torch.autograd.grad(fp8.mlp(x, w1, None, w2, None), x, dy)[0]
     assert torch.equal(got, torch.autograd.grad(fp8.mlp(x, w1.clone(), None, w2.clone(), None), x, dy)[0])
+
+
+# ---- models of several kinds of layers ----
+
+def relative(a, b):
+    return ((a.float() - b.float()).norm() / b.float().norm()).item()
+
+
+def test_attention_and_encoder_layers_convert():
+    """Frozen linears inside modules that read their children's weights.  Operands in 8 bits are off by 2^-4 at most and 2^-5.8 of a standard deviation on average; two of them in
+    each of two linears behind one another, whose result joins a residual stream of its size at least: 2^-5.8 * 2 = 2^-4.8 of it."""
+    x = matrix(2 * 40, 64, 1, torch.float16, 0.0).reshape(2, 40, 64)
+    torch.manual_seed(4)
+    with torch.no_grad():
+        attention = torch.nn.MultiheadAttention(64, 4, batch_first=True).half().cuda().eval()
+        want = attention(x, x, x, need_weights=False)[0]
+        assert torch.equal(fp8.linear_to_fp8(attention)(x, x, x, need_weights=False)[0], want)
+        layer = torch.nn.TransformerEncoderLayer(64, 4, 256, dropout=0.0, activation="gelu", batch_first=True).half().cuda().eval()
+        for model in (layer, torch.nn.TransformerEncoder(layer, 2, enable_nested_tensor=False)):
+            want = model(x)
+            for trainable in (True, False):
+                got = fp8.linear_to_fp8(copy.deepcopy(model), trainable=trainable)(x)
+                assert 0 < relative(got, want) <= 2.0 ** -4.8 * (2 if model is not layer else 1)

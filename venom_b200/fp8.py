@@ -229,16 +229,21 @@ class Fp8Mlp(_Held):
 
 
 def linear_to_fp8(mod, skip=(), trainable=False, grad_dtype=E4M3):
-    """Replaces every torch.nn.Linear below `mod` by Fp8Linear, but for the names in `skip` (nmv.linear_to_spmm's walk)."""
-    if isinstance(mod, torch.nn.Linear):
+    """Replaces every torch.nn.Linear below `mod` by Fp8Linear, but for the names in `skip` (nmv.linear_to_spmm's walk).
+
+    Subclasses stay as they are: they compute something else, or their owner multiplies with their weight itself (torch.nn.MultiheadAttention.out_proj).  A
+    torch.nn.TransformerEncoderLayer is kept from the fused inference path that takes its linears' weights past them."""
+    if type(mod) is torch.nn.Linear:
         return Fp8Linear(mod, trainable, grad_dtype)
     for name, child in mod.named_children():
         if name in skip:
             continue
-        if isinstance(child, torch.nn.Linear):
+        if type(child) is torch.nn.Linear:
             setattr(mod, name, Fp8Linear(child, trainable, grad_dtype))
         else:
             linear_to_fp8(child, skip, trainable, grad_dtype)
+    if isinstance(mod, torch.nn.TransformerEncoderLayer) and any(isinstance(child, Fp8Linear) for child in mod.children()):
+        mod.activation_relu_or_gelu = 0
     return mod
 
 
