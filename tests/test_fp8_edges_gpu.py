@@ -262,3 +262,24 @@ def test_attention_and_encoder_layers_convert():
             for trainable in (True, False):
                 got = fp8.linear_to_fp8(copy.deepcopy(model), trainable=trainable)(x)
                 assert 0 < relative(got, want) <= 2.0 ** -4.8 * (2 if model is not layer else 1)
+
+
+@pytest.mark.parametrize("pruned_first", [True, False])
+def test_some_linears_pruned_and_the_rest_in_8_bits(pruned_first):
+    """What linear_to_spmm skips becomes 8 bits, in either order; each layer computes what it computes alone."""
+    from venom_b200 import nmv
+    torch.manual_seed(5)
+    net = torch.nn.ModuleDict({"query": torch.nn.Linear(256, 256), "out": torch.nn.Linear(256, 128), "ffn": torch.nn.Sequential(torch.nn.Linear(128, 512), torch.nn.GELU(), torch.nn.Linear(512, 128))})
+    net = net.half().cuda().requires_grad_(False)
+    dense = copy.deepcopy(net)
+    steps = [lambda: nmv.linear_to_spmm(net, v=64, m=8, skip=("out", "ffn")), lambda: fp8.linear_to_fp8(net, skip=("query",))]
+    for step in steps if pruned_first else steps[::-1]:
+        step()
+    assert type(net["query"]) is nmv.SrnmSpmm and all(type(m) is fp8.Fp8Linear for m in (net["out"], net["ffn"][0], net["ffn"][2]))
+    x = matrix(72, 256, 1, torch.float16)
+    h = net["query"](x)
+    assert torch.equal(h, nmv.SrnmSpmm(dense["query"], v=64, m=8)(x))
+    y = net["out"](h)
+    assert torch.equal(y, fp8.linear(h, dense["out"].weight, dense["out"].bias))
+    z = fp8.linear(torch.nn.functional.gelu(fp8.linear(y, dense["ffn"][0].weight, dense["ffn"][0].bias)), dense["ffn"][2].weight, dense["ffn"][2].bias)
+    assert torch.equal(net["ffn"](y), z)
