@@ -283,3 +283,29 @@ def test_some_linears_pruned_and_the_rest_in_8_bits(pruned_first):
     assert torch.equal(y, fp8.linear(h, dense["out"].weight, dense["out"].bias))
     z = fp8.linear(torch.nn.functional.gelu(fp8.linear(y, dense["ffn"][0].weight, dense["ffn"][0].bias)), dense["ffn"][2].weight, dense["ffn"][2].bias)
     assert torch.equal(net["ffn"](y), z)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("trainable", [False, True])
+def test_modules_under_autocast(dtype, trainable):
+    """Results of the type that torch.nn.Linear gives there, those of the input in that type; gradients of the types of what they belong to."""
+    t = TYPES[dtype]
+    torch.manual_seed(6)
+    fc, proj = torch.nn.Linear(96, 200).cuda(), torch.nn.Linear(200, 72).cuda()
+    x, dy = matrix(50, 96, 1), matrix(50, 72, 2, t)
+    for module, own in ((fp8.Fp8Linear(fc, trainable), lambda v: fp8.linear(v, fc.weight, fc.bias)), (fp8.Fp8Mlp(fc, proj, trainable=trainable), lambda v: fp8.mlp(v, fc.weight, fc.bias, proj.weight, proj.bias))):
+        assert module(x).dtype == torch.float32
+        with torch.autocast("cuda", dtype=t):
+            y, dense = module(x), fc(x)
+            with torch.autocast("cuda", enabled=False):
+                assert module(x).dtype == torch.float32
+            assert module(x.to(torch.bfloat16)).dtype == fc(x.to(torch.bfloat16)).dtype == t
+        assert y.dtype == dense.dtype == t and torch.equal(y, own(x.to(t)))
+    if trainable:
+        v = leaf(x)
+        with torch.autocast("cuda", dtype=t):
+            y = module(v)
+        y.backward(dy)
+        assert v.grad.dtype == torch.float32 and fc.weight.grad.dtype == torch.float32
+        (want,) = torch.autograd.grad(own(v.to(t)), v, dy)
+        assert torch.equal(v.grad, want)

@@ -138,6 +138,13 @@ def mlp(x, w1, b1, w2, b2, approximate="none", grad_dtype=E4M3):
     return _call("fp8_mlp", x, w1, b1, w2, b2, _tanh_form(approximate, "fp8.mlp"), grad_dtype)
 
 
+def _autocast(x):
+    """What torch.nn.Linear would multiply: under torch.autocast x in the type that is named there."""
+    if torch.is_autocast_enabled("cuda") and isinstance(x, torch.Tensor) and x.dtype in _FLOATS:
+        return x.to(torch.get_autocast_dtype("cuda"))
+    return x
+
+
 class _Held(torch.nn.Module):
     """A frozen weight's 8 bits as buffers.  They are kept as bytes, which Module.half() and its like leave alone, with the rows' padding, which a copy to
     another device would drop; the padding is zero, so that one weight always gives the same bytes."""
@@ -172,7 +179,7 @@ def _frozen(bias):
 
 
 class Fp8Linear(_Held):
-    """Drop-in replacement of torch.nn.Linear whose products run in 8 bits.
+    """Drop-in replacement of torch.nn.Linear whose products run in 8 bits; results have the type of the input, under torch.autocast the type that it names.
 
     trainable=False: the weight is quantised once and held in 8 bits only, like SrnmSpmm's, for inference; an input that wants a gradient is refused.  trainable=True: the layer keeps the parameters
     of `original`, quantises the weight in every call and is differentiable (see linear)."""
@@ -192,9 +199,9 @@ class Fp8Linear(_Held):
 
     def forward(self, input):
         if self.trainable:
-            return linear(input, self.weight, self.bias, self.grad_dtype)
+            return linear(_autocast(input), self.weight, self.bias, self.grad_dtype)
         self._refuse_gradients(input)
-        return _call("fp8_held_linear", input, *self._weight("weight"), self.bias)
+        return _call("fp8_held_linear", _autocast(input), *self._weight("weight"), self.bias)
 
     def extra_repr(self):
         return "in_features=%d, out_features=%d, bias=%s, trainable=%s" % (self.in_features, self.out_features, self.bias is not None, self.trainable)
@@ -223,9 +230,9 @@ class Fp8Mlp(_Held):
 
     def forward(self, input):
         if self.trainable:
-            return mlp(input, self.fc_weight, self.fc_bias, self.proj_weight, self.proj_bias, self.approximate, self.grad_dtype)
+            return mlp(_autocast(input), self.fc_weight, self.fc_bias, self.proj_weight, self.proj_bias, self.approximate, self.grad_dtype)
         self._refuse_gradients(input)
-        return _call("fp8_held_mlp", input, *self._weight("fc"), self.fc_bias, *self._weight("proj"), self.proj_bias, self.tanh_form)
+        return _call("fp8_held_mlp", _autocast(input), *self._weight("fc"), self.fc_bias, *self._weight("proj"), self.proj_bias, self.tanh_form)
 
 
 def linear_to_fp8(mod, skip=(), trainable=False, grad_dtype=E4M3):
