@@ -266,7 +266,8 @@ int vnm_spmm_config(vnm_handle_t handle, int N, int *tile_m, int *tile_n, int *s
  *   data    8-bit floats, row r at data + r * ld; ld a multiple of 16 and at least cols, base 16-byte aligned.  Entry points that write it also
  *           write zeros up to the next multiple of 8 columns (of 16 for a transpose), those that read it ignore what lies past cols.
  *   scales  one byte for each row and block, the exponent + 127 of a power of two: byte ((kb / 4) * rows + r) * 4 + kb % 4 for
- *           block kb = columns 128 kb .. 128 kb + 127, in all vnm_fp8_scale_bytes(rows, cols); bytes past the last block are 0.  4-byte aligned.
+ *           block kb = columns 128 kb .. 128 kb + 127, in all vnm_fp8_scale_bytes(rows, cols); bytes past the last block are 0.  255, which no entry
+ *           point writes, is NaN.  4-byte aligned.
  * The scale of a block is the smallest power of two s >= 2^-127 with amax / s <= 448 (e4m3) or 57344 (e5m2), amax the largest finite magnitude in it;
  * values are x / s rounded once, to nearest even.  NaN stays NaN, infinities become NaN in e4m3 and stay in e5m2; neither changes the others' scale.
  * A block of zeros has the smallest scale.  x_type and the types of y, dx, out, bias and column sums: VNM_F32, VNM_F16 or VNM_BF16.  ldx >= cols;

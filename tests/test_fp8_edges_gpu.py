@@ -73,6 +73,23 @@ def test_products_of_values_that_are_not_finite(M, N, K):
     assert fp8.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("cols", [40, 300, 1031])
+def test_scales_that_are_not_a_number(dtype, cols):
+    """float8_e8m0fnu has a NaN: a block with that scale has no value, and no product of it has one."""
+    x = matrix(20, cols, 1, spread=0.3)
+    x[3, 5] = 0
+    q, w = fp8.quantize(x), fp8.quantize(matrix(136, cols, 2, spread=0.3))
+    want = q.dequantize(TYPES[dtype])
+    codes = q.scales.view(torch.uint8)
+    codes[0, 3, 0] = 255
+    want[3, :128] = math.nan
+    got = q.dequantize(TYPES[dtype])
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    rows = fp8.matmul(q, w, dtype=torch.float32).isnan()
+    assert bool(rows[3].all()) and int(rows.sum()) == 136
+
+
 # ---- frozen layers and their buffers ----
 
 def frozen(cin=200, cout=131, seed=0):

@@ -265,6 +265,7 @@ __device__ __forceinline__ uint32_t scale_code(float amax)
     return e > 0 ? (uint32_t)e : 0u;
 }
 __device__ __forceinline__ float inverse_scale(uint32_t code) { return __uint_as_float((254u - code) << 23); }
+// 0 stands for 2^-127, which is denormal in fp32.
 __device__ __forceinline__ float scale_value(uint32_t code) { return code ? __uint_as_float(code << 23) : __uint_as_float(0x00400000u); }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < __uint_as_float(0x7F800000u); }
 
@@ -885,7 +886,8 @@ __global__ void __launch_bounds__(ROWS_THREADS) fp8_dequantize_kernel(const uint
 #pragma unroll
         for (int i = 0; i < STEPS; i++) {
             const int c = c0 + 32 * V * i;
-            const float s = scale_value(byte_of(codes, (c >> 7) & 3));
+            const uint32_t code = byte_of(codes, (c >> 7) & 3);
+            const float s = code == 255 ? __uint_as_float(0x7FC00000u) : scale_value(code);      // another's scales may be NaN
             float v[V];
             if constexpr (V == 1) {
                 const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)q[i], F8 == F8_E4M3 ? __NV_E4M3 : __NV_E5M2);
