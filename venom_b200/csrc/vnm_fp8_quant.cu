@@ -880,14 +880,21 @@ __global__ void __launch_bounds__(ROWS_THREADS) fp8_dequantize_kernel(const uint
         const uint8_t *src = data + (int64_t)r * ldd + c0;
         E *dst = reinterpret_cast<E *>(out) + (int64_t)r * ldo + c0;
         const uint32_t codes = __ldg(scales + (int64_t)g * rows + r);
+        // a block's scale as half a word: bf16 has them all, and NaN for 255
+        uint32_t pair[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const __nv_bfloat162_raw b = __nv_cvt_e8m0x2_to_bf162raw((__nv_fp8x2_storage_t)(codes >> (16 * i)));
+            pair[i] = (uint32_t)b.x | ((uint32_t)b.y << 16);
+        }
         Bytes q[STEPS];
 #pragma unroll
         for (int i = 0; i < STEPS; i++) q[i] = c0 + 32 * V * i < cols ? __ldg(reinterpret_cast<const Bytes *>(src + 32 * V * i)) : Bytes{};
 #pragma unroll
         for (int i = 0; i < STEPS; i++) {
             const int c = c0 + 32 * V * i;
-            const uint32_t code = byte_of(codes, (c >> 7) & 3);
-            const float s = code == 255 ? __uint_as_float(0x7FC00000u) : scale_value(code);      // another's scales may be NaN
+            const int kb = ((int)(threadIdx.x & 31) * V + 32 * V * i) >> 7;
+            const float s = __uint_as_float(kb & 1 ? pair[kb >> 1] & 0xFFFF0000u : pair[kb >> 1] << 16);
             float v[V];
             if constexpr (V == 1) {
                 const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)q[i], F8 == F8_E4M3 ? __NV_E4M3 : __NV_E5M2);
