@@ -286,7 +286,7 @@ int vnm_fp8_quantize(const void *x, int x_type, int64_t ldx, int rows, int cols,
 int vnm_fp8_dequantize(const void *data, int64_t ldd, const void *scales, int f8_type, int rows, int cols, void *out, int out_type, int64_t ldo, void *stream);
 
 /* GELU with what its gradient and the following product need, in one pass over x: tanh_form 0 = x Phi(x), 1 = the tanh form.  Ahead
- * of its rounding, a result for negative x is off by at most 1.4e-6 + x^2 2^-24 of itself (the tanh form, with u its argument: 1e-6 + |u| 2^-21).
+ * of its rounding, a result for negative x is off by at most 2.5e-6 (32-bit x: 1.6e-6) + x^2 2^-24 of itself (the tanh form, with u its argument: 1e-6 + |u| 2^-21).
  *   y                 gelu(x) in the type of x (null: not wanted; not together with data_t)
  *   data.., data_t..  gelu(x) in e4m3, rounded from fp32, as vnm_fp8_quantize gives them (null: not wanted)
  *   ckpt, ckpt_scales an e4m3 checkpoint of x for vnm_fp8_gelu_grad (null: not wanted) */

@@ -396,26 +396,38 @@ __device__ __forceinline__ float min_nan(float a, float b)
 // Beyond 64 either form is x or 0 and the derivative 1 or 0: values are cut off there, ahead of squares that would overflow beside a zero.  So -inf gives 0.
 __device__ __forceinline__ float near(float x) { return max_nan(min_nan(x, 64.0f), -64.0f); }
 
-// The exact form: Phi(-a) = t R(t) exp(-a^2 / 2), a = |x|, t = 1 / (1 + 0.3 a), the form of Abramowitz and Stegun, 7.1.26, with a polynomial R that bounds the relative
-// error instead of the absolute one: minimax over 0 <= a <= 14, 1.5e-7, fitted by exchange of the extrema in 40 digits (against 2^q with the rounded constant of q).  7.1.26
-// itself is off by 5e-5 of the value at a = 3 and 1.6e-3 at 5, and one in 1e4 of a GELU's 8-bit results was another than the formula's.  The exponential is
-// the density's as well, which the derivative needs, so one exponential and one reciprocal give both.  gelu(x) = max(x, 0) - a Phi(-a): no cancellation for negative x, where it is
-// off by 1.4e-6 + a^2 2^-24 of itself at most.  The result is S Phi(-a), S = 1 or -1; a is cut off.
-template <int S>
+// The exact form: Phi(-a) = R(t) exp(-a^2 / 2), a = |x|, t = 1 / (1 + p a), the form of Abramowitz and Stegun, 7.1.26, with polynomials R that bound the relative error
+// instead of the absolute one: minimax over 0 <= a <= 13.3, where fp32 ends, by exchange of the extrema in 40 digits (against 2^q with the rounded constant of q).  7.1.26 itself
+// is off by 5e-5 of the value at a = 3 and 1.6e-3 at 5, and one in 1e4 of a GELU's 8-bit results was another than the formula's.  FINE, for values of 32 bits and for the
+// derivative: degree 7, 2.7e-7, and one half at t = 1 to the last bit, because a gradient of 16 bits times the derivative at 0 often lies between two 8-bit values.  Else degree 6,
+// 1.5e-6, a hundredth of fp16's half step (a GELU step of 16384 x 4096 fp16: 133 us if both take it, 137 if neither does).  The exponential is the density's as well, which the
+// derivative needs, so one exponential and one reciprocal give both.  gelu(x) = max(x, 0) - a Phi(-a): no cancellation for negative x, where it is off by 2.5e-6 (FINE:
+// 1.6e-6) + a^2 2^-24 of itself at most.  The result is S Phi(-a), S = 1 or -1; a is cut off.
+template <int S, bool FINE>
 __device__ __forceinline__ float2 normal_tail(float2 a, float2 *e)
 {
-    const float2 d = fma2(both(0.3f), a, both(1.0f));
+    const float2 d = fma2(both(FINE ? 0.255f : 0.2975f), a, both(1.0f));
     const float2 t = make_float2(fast_rcp(d.x), fast_rcp(d.y));
     const float2 q = mul2(mul2(a, a), both(-0.72134752044448170f));
     *e = make_float2(fast_exp2(q.x), fast_exp2(q.y));
-    float2 poly = fma2(both(S * 0.03573678433895111f), t, both(S * -0.15747535228729248f));
-    poly = fma2(poly, t, both(S * 0.20685447752475739f));
-    poly = fma2(poly, t, both(S * -0.05418521910905838f));
-    poly = fma2(poly, t, both(S * 0.12885797023773193f));
-    poly = fma2(poly, t, both(S * 0.0998092070221901f));
-    poly = fma2(poly, t, both(S * 0.12077460438013077f));
-    poly = fma2(poly, t, both(S * 0.1196274608373642f));
-    return mul2(mul2(poly, t), *e);
+    float2 poly;
+    if (FINE) {
+        poly = fma2(both(S * -0.0861255229f), t, both(S * 0.300162017f));
+        poly = fma2(poly, t, both(S * -0.213580772f));
+        poly = fma2(poly, t, both(S * 0.251812041f));
+        poly = fma2(poly, t, both(S * 0.0317303129f));
+        poly = fma2(poly, t, both(S * 0.115937077f));
+        poly = fma2(poly, t, both(S * 0.0999727994f));
+        poly = fma2(poly, t, both(S * 9.20295715e-05f));
+    } else {
+        poly = fma2(both(S * -0.0874843597f), t, both(S * 0.257873505f));
+        poly = fma2(poly, t, both(S * -0.0690223277f));
+        poly = fma2(poly, t, both(S * 0.175907403f));
+        poly = fma2(poly, t, both(S * 0.101962328f));
+        poly = fma2(poly, t, both(S * 0.12088152f));
+        poly = fma2(poly, t, both(S * -0.000118785138f));
+    }
+    return mul2(poly, *e);
 }
 // The tanh form: (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3); x cut off.  -2 u log2 e = x (c1 x^2 + c0).
 __device__ __forceinline__ float2 gelu_sigmoid(float2 x, float2 x2)
@@ -423,7 +435,7 @@ __device__ __forceinline__ float2 gelu_sigmoid(float2 x, float2 x2)
     const float2 q = mul2(x, fma2(both(-0.10294324f), x2, both(-2.3022082f)));
     return make_float2(fast_rcp(1.0f + fast_exp2(q.x)), fast_rcp(1.0f + fast_exp2(q.y)));
 }
-template <bool TANH>
+template <bool TANH, bool FINE>
 __device__ __forceinline__ void gelu2(float &x, float &y)
 {
     float2 r;
@@ -433,7 +445,7 @@ __device__ __forceinline__ void gelu2(float &x, float &y)
     } else {
         const float2 a = make_float2(min_nan(fabsf(x), 64.0f), min_nan(fabsf(y), 64.0f));
         float2 e;
-        const float2 h = normal_tail<-1>(a, &e);
+        const float2 h = normal_tail<-1, FINE>(a, &e);
         r = fma2(a, h, make_float2(max_nan(x, 0.0f), max_nan(y, 0.0f)));
     }
     x = r.x;
@@ -452,7 +464,7 @@ __device__ __forceinline__ void times_gelu_grad2(float &x, float &y, float a, fl
         g = fma2(mul2(mul2(n, s), c), du, make_float2(n.x < 0.0f ? s.x : c.x, n.y < 0.0f ? s.y : c.y));
     } else {
         float2 e;
-        const float2 h = normal_tail<1>(make_float2(fabsf(n.x), fabsf(n.y)), &e);
+        const float2 h = normal_tail<1, true>(make_float2(fabsf(n.x), fabsf(n.y)), &e);
         const float2 far = make_float2(n.x < 0.0f ? h.x : 1.0f - h.x, n.y < 0.0f ? h.y : 1.0f - h.y);
         g = fma2(n, mul2(e, both(0.39894228040143268f)), far);
     }
@@ -567,7 +579,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, TYPE == T_F32 || OP != FP8_PLAIN
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) gelu2<TANH>(v.v[i][j], v.v[i][j + 1]);
+                for (int j = 0; j < 8; j += 2) gelu2<TANH, TYPE == T_F32>(v.v[i][j], v.v[i][j + 1]);
         } else if constexpr (OP == FP8_GELU_GRAD) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -680,7 +692,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8QuantParams &p, TileShared &sh
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) gelu2<TANH>(v.v[j][i], v.v[j][i + 1]);   // of the zeros that pad: zero
+            for (int i = 0; i < 8; i += 2) gelu2<TANH, TYPE == T_F32>(v.v[j][i], v.v[j][i + 1]);   // of the zeros that pad: zero
     }
 
     uint32_t tile_code = 0;

@@ -126,7 +126,7 @@ def linear(x, weight, bias=None, grad_dtype=E4M3):
 
 def gelu(x, approximate="none"):
     """GELU of x [..., features] like torch.nn.functional.gelu, but 0 for -inf; what is kept for the backward pass is x in 8 bits, in blocks of 128
-    features.  For negative x the result is off by 1.4e-6 + x^2 2^-24 of itself at most, besides its rounding (the tanh form, with u its argument: 1e-6 + |u| 2^-21)."""
+    features.  For negative x the result is off by 2.5e-6 (32-bit x: 1.6e-6) + x^2 2^-24 of itself at most, besides its rounding (the tanh form, with u its argument: 1e-6 + |u| 2^-21)."""
     return _call("fp8_gelu8", x, _tanh_form(approximate, "fp8.gelu"))
 
 
