@@ -299,7 +299,7 @@ int vnm_fp8_gelu_grad(const void *dy, int dy_type, int64_t ldy, int rows, int co
                       void *workspace, void *stream);
 
 /* out[m, n] = sum over k of A[m, k] B[n, k] (+ bias[n]), A [M, K] and B [N, K] in 8 bits (types may differ), sums in fp32, rounded once; out [M, N] with
- * leading dimension ldo >= N.  K >= 1. */
+ * leading dimension ldo >= N.  K >= 1.  The tensor core truncates its sums; below 2^-126 they are zero. */
 int vnm_fp8_matmul(const void *a, int64_t lda, const void *a_scales, int a_type, const void *b, int64_t ldb, const void *b_scales, int b_type, int M, int N, int K,
                    const void *bias, int bias_type, void *out, int out_type, int64_t ldo, void *stream);
 /* The plan that vnm_fp8_matmul takes on the current device (for reporting): rows of A and of B a tile, CTAs that share a tile's k, CTAs in all.  whole: rows

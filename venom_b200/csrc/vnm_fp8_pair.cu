@@ -10,8 +10,8 @@
 //   * scale and epilogue warps of the peer arrive remotely on the leader's scale-full and accumulator-empty barriers.
 // Every wait is bounded, and the CTAs meet at a cluster barrier before either leaves.
 //
-// Bound by power: 2048 x 12288 x 12288 246 us in long runs = 2.5 PFLOP/s at 1.0-1.4 GHz, 203 in short ones; 16384 x 4096 x 1024 62 (2.2 PFLOP/s), eight k-tiles for the
-// epilogue of 256 x 240 values.
+// Bound by power: 2048 x 12288 x 12288 239 to 261 us in long runs = 2.4-2.6 PFLOP/s at 1.0-1.4 GHz, 203 in short ones; 16384 x 4096 x 1024 with a bias 62 to 65 by
+// itself (2.2 PFLOP/s), 73 to 81 among other calls: eight k-tiles for the epilogue of 256 x 240 values.
 #include "vnm_fp8.h"
 
 #include <cuda_bf16.h>
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
     using T = Fp8Pair<BN, WHOLE>;
     constexpr int S = T::STAGES;
     extern __shared__ uint8_t smem_raw[];
-    // Through a pointer that the compiler knows to be shared memory: 16384 x 4096 x 256 34.8 -> 31.9 us, with a bias 47 -> 39.  The other epilogues are scheduled worse then
+    // Through a pointer that the compiler knows to be shared memory: 16384 x 4096 x 256 34.9 -> 31.8 us, with a bias 41.3 -> 37.0.  The other epilogues are scheduled worse then
     // (11844 x 15043 x 116 130 -> 140, in tiles of 256 columns 16384 x 4096 x 256 36 -> 41): theirs goes through an integer.
     uint8_t *smem = WHOLE && !T::ONE ? smem_raw + (-smem_u32(smem_raw) & 1023u) : reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *a_ring = smem, *b_ring = smem + S * A_BYTES;
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) fp8_pair_kernel(const __grid_c
         const uint32_t tmem_base = *tmem_slot;
         uint8_t *own = smem + S * T::STAGE_BYTES + (warp - EPI_WARP0) * T::WARP_BYTES;
         uint4 *stage = reinterpret_cast<uint4 *>(own);
-        // 32 columns before: part 1, !WHOLE.  Known to be shared memory in every epilogue: 11844 x 15043 x 116 158 -> 148 us.
+        // 32 columns before: part 1, !WHOLE.  Known to be shared memory in every epilogue: 11844 x 15043 x 116 159 -> 150 us.
         float4 *bias = reinterpret_cast<float4 *>(smem_raw + (-smem_u32(smem_raw) & 1023u) + S * T::STAGE_BYTES + (warp - EPI_WARP0) * T::WARP_BYTES + T::WARP_BYTES - 512);
         // bias of four columns a lane (and of one of the 32 before), on its way while the tile before is stored: as it lies, for a conversion would wait for it
         uint32_t next[5];
@@ -577,7 +577,8 @@ cudaError_t fp8_pair_init(int sms, int *clusters)
 // The cost of a call, us: a start, waves of tiles (between the whole number that the last one makes and the fraction that the power limit sees), and the last
 // tile's epilogue.  A tile takes its k-tiles' time or its epilogue's, whichever is longer (a smooth maximum), or with one accumulator both.  Both
 // kernels' costs were fitted to steady calls on inputs that change, 802 shapes of 1 to 16384 x 8 to 36864 x 64 to 12288, odd ones and round ones, with and without a bias,
-// fp16 and fp32 results, for the choice that they make: 1.007 of the fastest one's time on average over 371 others, 1.33 at most (few rows, few columns or few k).
+// fp16 and fp32 results, for the choice that they make: over 366 others the plan that is taken was measured at 1.014 of the fastest one's time on average, 1.29 at most (few rows,
+// few columns or few k: 4527 x 56 x 560 7.5 us against 5.8, 10 x 21128 x 5102 29.7 against 23.1, where one CTA a tile would do).
 float fp8_pair_config(int M, int N, int K, bool wide_out, bool whole, bool bias, const Fp8Device &device, Fp8Plan *plan)
 {
     const int clusters = device.clusters;

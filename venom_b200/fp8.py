@@ -75,7 +75,7 @@ def quantize(x, dtype=E4M3, square=False, both=False):
     """x [rows, cols] (float16, bfloat16 or float32 on a CUDA device) -> BlockFp8 of float8_e4m3fn or float8_e5m2.
 
     A block's scale is the smallest power of two that brings its largest finite magnitude to at most 448 (e4m3) or 57344 (e5m2); values are
-    rounded to nearest even.  NaN stays NaN, infinities become NaN in e4m3 and stay in e5m2.  Blocks are 128 values of a row, or with `square` 128 x 128,
+    rounded to nearest even.  NaN stays NaN, infinities become NaN in e4m3 and stay in e5m2.  Not differentiable: the result is x's values now.  Blocks are 128 values of a row, or with `square` 128 x 128,
     so that a matrix and its transpose hold the same values.  both: also the transpose, as (BlockFp8 of x, BlockFp8 of x.T), from one read of x."""
     try:
         q = (_ext or _load()).fp8_quantize(x, dtype, bool(square), bool(both))
@@ -86,7 +86,8 @@ def quantize(x, dtype=E4M3, square=False, both=False):
 
 def matmul(a, b, bias=None, dtype=torch.float16):
     """a @ b.T (+ bias): BlockFp8 [M, K] and [N, K] -> [M, N] of `dtype` (float16, bfloat16 or float32).  The 8-bit types of a and b may differ.
-    bias: N values, added in 32 bits."""
+    bias: N values, added in 32 bits.  Not differentiable: the result belongs to no graph, also where the bias wants a gradient (linear is).  Sums have 32 bits, as
+    the tensor core keeps them: they are truncated, not rounded, and zero below 2^-126."""
     try:
         return (_ext or _load()).fp8_matmul(a.data, a.scales, b.data, b.scales, bias, dtype)
     except (RuntimeError, TypeError) as e:
