@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_fp8_gpu import E4M3, E5M2, TYPES, check_held, matrix
+from test_fp8_gpu import E4M3, E5M2, TYPES, check_held, matrix, pow2
 from venom_b200 import capi, fp8
 
 pytestmark = pytest.mark.gpu
@@ -90,6 +90,23 @@ def test_scales_that_are_not_a_number(dtype, cols):
     assert bool(rows[3].all()) and int(rows.sum()) == 136
 
 
+@pytest.mark.parametrize("f8", [E4M3, E5M2])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("cols", [256, 255])
+def test_every_value_with_every_scale(f8, dtype, cols):
+    """All 8-bit values in blocks of all scales, those of denormals and of values past fp32's range among them: rounded to fp32, then to the result's type."""
+    data = torch.arange(256, dtype=torch.uint8, device="cuda")[:cols].repeat(256, 1)
+    padded = torch.zeros((256, 256), dtype=torch.uint8, device="cuda")
+    padded[:, :cols] = data
+    codes = torch.zeros((1, 256, 4), dtype=torch.uint8, device="cuda")
+    codes[0, :, 0] = torch.arange(256, dtype=torch.uint8, device="cuda")
+    codes[0, :, 1] = torch.arange(255, -1, -1, dtype=torch.uint8, device="cuda")
+    got = fp8.BlockFp8(padded.view(f8)[:, :cols], codes.view(torch.float8_e8m0fnu)).dequantize(TYPES[dtype])
+    scales = torch.where(codes[0, :, :2] == 255, math.nan, pow2(codes[0, :, :2].double() - 127)).repeat_interleave(128, 1)[:, :cols]
+    want = (data.view(f8).double() * scales).float().to(TYPES[dtype])
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+
+
 # ---- frozen layers and their buffers ----
 
 def frozen(cin=200, cout=131, seed=0):
@@ -152,6 +169,20 @@ def test_one_weight_always_gives_the_same_bytes(cin):
         assert v.untyped_storage().nbytes() == v.numel() * v.element_size(), k
     storages = {v.untyped_storage().data_ptr() for v in states[0].values()}
     assert len(storages) == len(states[0])
+
+
+def test_frozen_layers_take_inputs_of_any_shape():
+    lin, mlp = fp8.Fp8Linear(frozen()), fp8.Fp8Mlp(frozen(), frozen(131, 72))
+    x = matrix(12, 200, 1, torch.float16)
+    wide = torch.zeros(12, 207, dtype=torch.float16, device="cuda")
+    wide[:, 5:205] = x
+    for layer, out in ((lin, 131), (mlp, 72)):
+        y = layer(x)
+        assert torch.equal(layer(x.reshape(2, 3, 2, 200)), y.reshape(2, 3, 2, out)) and torch.equal(layer(x[0]), y[0]) and torch.equal(layer(wide[:, 5:205]), y)
+        assert layer(x[:0]).shape == (0, out) and layer(x.reshape(2, 6, 200)[:, :0]).shape == (2, 0, out) and torch.equal(layer(x.t().contiguous().t()), y)
+        for bad, match in ((x[:, :199], "do not match"), (x.cpu(), "CUDA"), (x.double(), "expected"), (x.sum(), "dimension"), (None, None)):
+            with pytest.raises(capi.VenomError, match=match):
+                layer(bad)
 
 
 def test_a_layer_from_a_file_with_views():
